@@ -6,8 +6,8 @@
 #include <string>
 #include <vector>
 
-#include <cudaTypedefs.h>
 
+#include "dsmz_host.h"
 #include "dsmz_handoff.cuh"
 #include "dsmz_kernels.cuh"
 #include "dsmz_pi_fused.cuh"
@@ -19,9 +19,9 @@
 
 using namespace dsmz;
 
-namespace {
+namespace dsmz {
 
-thread_local std::string g_err;
+static thread_local std::string g_err;
 
 int fail(int code, const std::string& msg) {
   g_err = msg;
@@ -32,11 +32,22 @@ int cuda_fail(const char* what, cudaError_t e) {
   return fail(DSMZ_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
-#define DSMZ_LAUNCHED(what)                                  \
-  do {                                                        \
-    cudaError_t e_ = cudaGetLastError();                      \
-    if (e_ != cudaSuccess) return cuda_fail((what), e_);      \
-  } while (0)
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+}  // namespace dsmz
+
+namespace {
 
 // ------------------------------------------------------------------ workspace layout
 struct Layout {
@@ -220,20 +231,6 @@ NSArgs make_ns(const dsmz_ns_schedule* s, float floor_) {
 }
 
 // ------------------------------------------------------------------ tensor-core power iteration
-// cuTensorMapEncodeTiled from the driver, looked up once per process.
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
-
 // 2-D tensor map of fp32 or bf16 rows (inner dimension contiguous), no swizzle, zero fill
 // outside: the tile boxes of the streaming kernels' side-1 arrays.
 bool encode_rows_2d(CUtensorMap* m, int dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,

@@ -64,6 +64,20 @@ class PlanDesc(ctypes.Structure):
     ]
 
 
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("m", c_void_p), ("v", c_void_p),
+                ("m_scale", c_void_p), ("v_scale", c_void_p), ("shadow", c_void_p), ("n", c_int64)]
+
+
+class AdamWDesc(ctypes.Structure):
+    _fields_ = [("param_dtype", c_int32), ("grad_dtype", c_int32), ("state_bits", c_int32), ("pad0", c_int32),
+                ("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double),
+                ("weight_decay", c_double), ("step", c_int64), ("lr_device", c_void_p), ("grad_scale", c_void_p),
+                ("step_counter", c_void_p)]
+
+
+ADAMW_BLOCK = 256
+ADAMW_WORKSPACE_BYTES = 64
 MAX_DIRECTIONS = 32
 PI_BASIS_UNCHANGED = 1        # dsmz_step_power_iteration_ex flag (include/dsmezo.h)
 
@@ -135,6 +149,8 @@ SIGNATURES = {
     "dsmz_step_kalman_sums": (c_void_p, [c_void_p]),
     "dsmz_step_update": (c_int32, [c_void_p, c_float, c_float, c_float, c_float, c_float, POINTER(NSSchedule),
                                    c_void_p]),
+    "dsmz_adamw_step": (c_int32, [POINTER(AdamWDesc), POINTER(AdamWTensor), c_int32, c_void_p, c_size_t, c_void_p]),
+    "dsmz_adamw_state_values": (c_int32, [POINTER(AdamWTensor), c_int32, c_void_p]),
     "dsmz_plan_set_probe": (c_int32, [c_void_p, c_int32, POINTER(c_void_p), POINTER(c_void_p), c_int32]),
     "dsmz_plan_probe_count": (c_int32, [c_void_p, c_int32]),
 }

@@ -364,6 +364,50 @@ int dsmz_step_update_directions(const dsmz_plan* plan, const float* dd, int32_t 
                                 dsmz_stream_t stream);
 
 /* ---------------------------------------------------------------------------------
+ * First-order step of an adapter set (no reference counterpart: the reference trains with
+ * zeroth-order updates only).
+ * ------------------------------------------------------------------------------- */
+
+/* AdamW over many tensors:
+ *   m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2   (g times *grad_scale when given)
+ *   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * state_bits 32: m and v are fp32. state_bits 8: m is int8 and v uint8 codes, in blocks of
+ * DSMZ_ADAMW_BLOCK elements counted from the tensor's start with one fp32 scale a block
+ * (ceil(n / DSMZ_ADAMW_BLOCK) of them): m = sign q^2 m_scale with |q| <= 127, sqrt(v) = q^2
+ * v_scale with q <= 255; a positive v never takes code 0, a value on the border of two codes
+ * takes the lower, and the codes are those of 64-bit arithmetic. A block that meets a NaN or
+ * an infinity becomes NaN as a whole. Zeroed codes and scales are the state before step 1.
+ * shadow: bf16 image of the updated fp32 parameter, rounded once (NULL: none).
+ * Tensors are contiguous; those of one call must not overlap. */
+#define DSMZ_ADAMW_BLOCK 256
+#define DSMZ_ADAMW_WORKSPACE_BYTES 64
+typedef struct dsmz_adamw_tensor {
+  void* param;                          /* param_dtype, updated in place */
+  const void* grad;                     /* grad_dtype */
+  void* m; void* v;                     /* states */
+  float* m_scale; float* v_scale;       /* 8-bit states only */
+  void* shadow;                         /* BF16 or NULL (F32 parameters only) */
+  int64_t n;                            /* elements; 0 skips the tensor */
+} dsmz_adamw_tensor;
+typedef struct dsmz_adamw_desc {
+  int32_t param_dtype, grad_dtype;      /* DSMZ_F32 or DSMZ_BF16 */
+  int32_t state_bits, pad0;             /* 32 or 8 */
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;                         /* t of this step, from 1 (unused with step_counter) */
+  const float* lr_device;               /* device scalar in place of lr, or NULL */
+  const float* grad_scale;              /* device scalar, or NULL */
+  int64_t* step_counter;                /* device counter, or NULL: the call adds 1 and takes the sum
+                                           as t, so that a captured call counts on when replayed */
+} dsmz_adamw_desc;
+/* tensors is a host array, read during the call. workspace (device, 16-byte aligned,
+ * DSMZ_ADAMW_WORKSPACE_BYTES) is needed with step_counter or lr_device only. */
+int dsmz_adamw_step(const dsmz_adamw_desc* desc, const dsmz_adamw_tensor* tensors, int32_t n, void* workspace,
+                    size_t workspace_bytes, dsmz_stream_t stream);
+/* The fp32 values of 8-bit states: of every tensor, n floats of m to `param` and n floats of v
+ * to `shadow` from m, v and their scales (`grad` is not read). */
+int dsmz_adamw_state_values(const dsmz_adamw_tensor* tensors, int32_t n, dsmz_stream_t stream);
+
+/* ---------------------------------------------------------------------------------
  * Timing probes: while set, every launch of kernel `kernel` by the grouped step records
  * start[i] / stop[i] (caller-created cudaEvent_t, passed as void*) on the launch stream,
  * for i = 0 .. capacity-1 in launch order. capacity 0 removes the probe.

@@ -1,0 +1,73 @@
+"""The first-order operators without a GPU: what the C entry points and the Python layer
+refuse before any CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from dsmezo_b200 import build
+    build.build()
+    from dsmezo_b200 import _lib
+    return _lib
+
+
+def desc(lib, **kw):
+    d = lib.AdamWDesc(param_dtype=0, grad_dtype=0, state_bits=32, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8,
+                      weight_decay=0.01, step=1)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def tensors(lib, **kw):
+    t = (lib.AdamWTensor * 1)()
+    e = t[0]
+    e.param = e.grad = e.m = e.v = 4096          # never read: every call here is refused
+    e.n = 8
+    for k, v in kw.items():
+        setattr(e, k, v)
+    return t
+
+
+@pytest.mark.parametrize("bad", [dict(param_dtype=2), dict(grad_dtype=-1), dict(state_bits=16), dict(beta1=1.0),
+                                 dict(beta2=-0.1), dict(eps=float("nan")), dict(weight_decay=-1.0),
+                                 dict(lr=float("inf")), dict(step=0)])
+def test_adamw_refuses_descriptors(lib, bad):
+    d = desc(lib, **bad)
+    assert lib.lib().dsmz_adamw_step(ctypes.byref(d), tensors(lib), 1, None, 0, None) == 1
+    assert b"dsmz_adamw_step" in lib.lib().dsmz_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(param=None), dict(grad=None), dict(m=None), dict(v=None), dict(n=-1),
+                                 dict(n=1 << 50), dict(param=4097), dict(m=4098), dict(shadow=4097)])
+def test_adamw_refuses_tensors(lib, bad):
+    d = desc(lib)
+    assert lib.lib().dsmz_adamw_step(ctypes.byref(d), tensors(lib, **bad), 1, None, 0, None) == 1
+    assert b"tensor 0" in lib.lib().dsmz_last_error()
+
+
+def test_adamw_refuses_missing_pieces(lib):
+    L = lib.lib()
+    assert L.dsmz_adamw_step(None, tensors(lib), 1, None, 0, None) == 1
+    d = desc(lib)
+    assert L.dsmz_adamw_step(ctypes.byref(d), None, 1, None, 0, None) == 1
+    assert L.dsmz_adamw_step(ctypes.byref(d), tensors(lib), -1, None, 0, None) == 1
+    d8 = desc(lib, state_bits=8)
+    assert L.dsmz_adamw_step(ctypes.byref(d8), tensors(lib), 1, None, 0, None) == 1         # no scales
+    dc = desc(lib, step_counter=4096)
+    assert L.dsmz_adamw_step(ctypes.byref(dc), tensors(lib), 1, None, 0, None) == 2         # no workspace
+    db = desc(lib, param_dtype=1)
+    assert L.dsmz_adamw_step(ctypes.byref(db), tensors(lib, shadow=4096), 1, None, 0, None) == 1
+    assert L.dsmz_adamw_state_values(tensors(lib), 1, None) == 1
+    # nothing to do is no error, and makes no CUDA call
+    assert L.dsmz_adamw_step(ctypes.byref(d), tensors(lib, n=0), 1, None, 0, None) == 0
+    assert L.dsmz_adamw_step(ctypes.byref(d), None, 0, None, 0, None) == 0
+
+
+def test_adamw_takes_no_cpu_tensors(lib):
+    from dsmezo_b200 import AdamW
+    with pytest.raises(ValueError, match="CUDA"):
+        AdamW([torch.zeros(4)])
