@@ -1,4 +1,5 @@
-// C ABI of the first-order operators declared in dsmezo.h: AdamW over many tensors.
+// C ABI of the first-order operators declared in dsmezo.h: the scoring loss with its gradient
+// and AdamW over many tensors.
 #include <cmath>
 #include <exception>
 #include <vector>
@@ -6,6 +7,7 @@
 #include "dsmezo.h"
 #include "dsmz_adamw.cuh"
 #include "dsmz_host.h"
+#include "dsmz_score_grad.cuh"
 
 using namespace dsmz;
 
@@ -134,9 +136,91 @@ int adamw_run(const dsmz_adamw_desc& d, const dsmz_adamw_tensor* tensors, int32_
       [&](const aw::Args<CAP>& a, int grid) { launch_adamw<CAP>(a, grid, d.param_dtype, d.grad_dtype, d.state_bits, s); });
 }
 
+// ------------------------------------------------------------------ scoring loss with its gradient
+template <typename T>
+int loss_grad(const void* logits, int64_t V, int64_t ld, const int32_t* targets, int64_t ntok, const sg::Seqs& q,
+              double grad_scale, float* loss, void* grad, int64_t ld_grad, double* term, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return cuda_fail("dsmz_contrastive_loss_grad: device query", e);
+  // CTAs a row: enough that a slice stays in L1 between the two passes, and that a few rows
+  // still occupy the machine twice over while a slice is worth a CTA
+  const int64_t row_bytes = V * static_cast<int64_t>(sizeof(T));
+  int C = 1;
+  while (C < 8 && (row_bytes / C > sg::kSliceBytes || (ntok * C < 2 * sms && row_bytes / C > 8192))) C *= 2;
+  const int64_t vecs = (row_bytes / C + 15) / 16;
+  const int threads = vecs >= 1024 ? 512 : (vecs >= 256 ? 256 : 128);
+  if (ntok * C > 0x7fffffff) return fail(DSMZ_ERR_UNSUPPORTED, "dsmz_contrastive_loss_grad: too many tokens");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ntok * C));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(C);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, sg::k_loss_grad<T>, static_cast<const T*>(logits), ld, V, targets, q, grad_scale,
+                         static_cast<T*>(grad), ld_grad, term);
+  if (e != cudaSuccess) return cuda_fail("dsmz_contrastive_loss_grad: rows", e);
+  sg::k_loss_sum<<<1, 256, 0, s>>>(term, ntok, loss);
+  DSMZ_LAUNCHED("dsmz_contrastive_loss_grad: sum");
+  return DSMZ_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+size_t dsmz_contrastive_loss_grad_workspace_bytes(int64_t ntok) {
+  return ntok > 0 ? static_cast<size_t>(ntok) * sizeof(double) : sizeof(double);
+}
+
+int dsmz_contrastive_loss_grad(int32_t kind, const void* logits, int64_t V, int64_t ld, const int32_t* targets,
+                               int64_t ntok, const int64_t* seq_start, const double* advantages, int32_t nseq,
+                               double grad_scale, float* loss, void* grad, int64_t ld_grad, void* workspace,
+                               size_t workspace_bytes, dsmz_stream_t stream) {
+  return guarded("dsmz_contrastive_loss_grad", [&]() -> int {
+    const std::string me = "dsmz_contrastive_loss_grad: ";
+    if (!logits || !targets || !seq_start || !advantages || !loss || !grad || !workspace)
+      return fail(DSMZ_ERR_INVALID, me + "null pointer");
+    if (kind != DSMZ_SCORE_LOGITS_F32 && kind != DSMZ_SCORE_LOGITS_BF16)
+      return fail(DSMZ_ERR_INVALID, me + "kind must be DSMZ_SCORE_LOGITS_F32 or DSMZ_SCORE_LOGITS_BF16");
+    if (nseq < 1 || nseq > sg::kMaxSeqs)
+      return fail(DSMZ_ERR_INVALID, me + "1 <= nseq <= " + std::to_string(sg::kMaxSeqs));
+    if (V < 1 || V > 0x7fffffff || ld < V || ld_grad < V || ld > kMaxElems || ld_grad > kMaxElems)
+      return fail(DSMZ_ERR_INVALID, me + "need 1 <= V < 2^31, ld >= V and ld_grad >= V");
+    if (ntok < 1 || ntok > 0x7fffffff || seq_start[0] != 0 || seq_start[nseq] != ntok)
+      return fail(DSMZ_ERR_INVALID, me + "seq_start must run from 0 to ntok >= 1");
+    if (!std::isfinite(grad_scale)) return fail(DSMZ_ERR_INVALID, me + "grad_scale must be finite");
+    const int64_t es = kind == DSMZ_SCORE_LOGITS_F32 ? 4 : 2;
+    if (!aligned(logits, es) || !aligned(grad, es) || !aligned(targets, 4) || !aligned(loss, 4))
+      return fail(DSMZ_ERR_INVALID, me + "a pointer is not aligned to its element type");
+    const uintptr_t a = reinterpret_cast<uintptr_t>(logits), b = reinterpret_cast<uintptr_t>(grad);
+    const uintptr_t na = static_cast<uintptr_t>(((ntok - 1) * ld + V) * es), nb = static_cast<uintptr_t>(((ntok - 1) * ld_grad + V) * es);
+    if (a < b + nb && b < a + na && !(a == b && (ld == ld_grad || ntok == 1)))
+      return fail(DSMZ_ERR_INVALID, me + "the gradient may overwrite the logits in place, not overlap them otherwise");
+    sg::Seqs q{};
+    q.n = nseq;
+    for (int i = 0; i < nseq; ++i) {
+      const int64_t len = seq_start[i + 1] - seq_start[i];
+      // the reference's mean over a sequence (ds_mezo/controller.py:14-15) has no empty case
+      if (len < 1) return fail(DSMZ_ERR_INVALID, me + "every sequence needs a scored token");
+      q.start[i] = seq_start[i];
+      q.w[i] = advantages[i] / static_cast<double>(len);
+    }
+    q.start[nseq] = ntok;
+    if (workspace_bytes < dsmz_contrastive_loss_grad_workspace_bytes(ntok) || !aligned(workspace, 8))
+      return fail(DSMZ_ERR_WORKSPACE, me + "workspace too small or not 8-byte aligned");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    double* term = static_cast<double*>(workspace);
+    return kind == DSMZ_SCORE_LOGITS_F32
+               ? loss_grad<float>(logits, V, ld, targets, ntok, q, grad_scale, loss, grad, ld_grad, term, s)
+               : loss_grad<__nv_bfloat16>(logits, V, ld, targets, ntok, q, grad_scale, loss, grad, ld_grad, term, s);
+  });
+}
 
 int dsmz_adamw_step(const dsmz_adamw_desc* desc, const dsmz_adamw_tensor* tensors, int32_t n, void* workspace,
                     size_t workspace_bytes, dsmz_stream_t stream) {

@@ -1,0 +1,249 @@
+// Contrastive scoring loss with its gradient in the logits:
+//   loss = sum_i a_i / n_i sum_{t in sequence i} nll_t,   nll_t = log sum_c exp(x_tc) - x_t,target
+//   d loss / d x_tc = a_i / n_i (exp(x_tc) / sum_c exp(x_tc) - [c = target_t])
+// (ds_mezo/controller.py:14-15, 194-201 for the loss; the reference takes no gradient of it).
+//
+// A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary. Pass one
+// over the slice keeps a running maximum and sum of exponentials a thread; the CTAs exchange (max, sum) through distributed shared memory;
+// pass two reads the slice again, from L1 while it is at most kSliceBytes, and writes the
+// gradient. HBM sees each logit once in and each gradient once out, which is the floor.
+// Rows need not be aligned: a slice has a scalar head up to the first 16-byte boundary,
+// 16-byte accesses, and a scalar tail. The target's logit is read before the exchange, so
+// the gradient may overwrite the logits.
+//
+// The maximum is subtracted before the scaling by log2 e: with the product first (one FMA a
+// logit less) masks at the type's lowest value overflow, and logits past 2^24 lose the
+// difference itself. Rows of -inf only, NaN and +inf follow the formula: NaN. A target outside the vocabulary
+// makes the loss and its row of the gradient NaN.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include "dsmz_ptx.cuh"
+
+namespace dsmz {
+namespace sg {
+
+constexpr int kMaxSeqs = 128;
+constexpr int kSliceBytes = 40 * 1024;   // four CTAs of 512 threads an SM keep their slices in L1
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Seqs {
+  int32_t n, pad;
+  int64_t start[kMaxSeqs + 1];           // token rows of sequence i: [start[i], start[i+1])
+  double w[kMaxSeqs];                    // a_i / n_i
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 8-byte store to the same shared variable of CTA `rank` of the cluster.
+__device__ __forceinline__ void st_cluster(void* local, uint32_t rank, float a, float b) {
+  uint32_t addr;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
+}
+
+__device__ __forceinline__ float exp_of(float d) { return ex2(d * kLog2e); }   // d <= 0
+
+// (m, s) <- the pair for both sets: m the larger maximum, s relative to it. An empty set is
+// (-inf, 0).
+__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
+  const float t = fmaxf(m, m2);
+  if (t == -INFINITY) { s += s2; return; }          // -inf logits alone, or NaN: s carries the NaN
+  s = s * exp_of(m - t) + s2 * exp_of(m2 - t);
+  m = t;
+}
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  __device__ static void load(const float* p, float (&x)[4]) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+  }
+  __device__ static void store(float* p, const float (&x)[4]) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
+  }
+  __device__ static float one(const float* p) { return *p; }
+  __device__ static void put(float* p, float x) { *p = x; }
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  __device__ static void load(const __nv_bfloat16* p, float (&x)[8]) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      x[2 * q] = __uint_as_float(w[q] << 16);
+      x[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
+    }
+  }
+  __device__ static void store(__nv_bfloat16* p, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * q], x[2 * q + 1]);
+      w[q] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+  }
+  __device__ static float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  __device__ static void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+};
+
+// grid: ntok * cluster size; row = blockIdx.x / cluster size.
+template <typename T>
+__global__ void __launch_bounds__(512) k_loss_grad(const T* logits, int64_t ld, int64_t V,
+                                                   const int32_t* __restrict__ targets, Seqs seqs, double grad_scale,
+                                                   T* grad, int64_t ld_grad, double* __restrict__ term) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float2 red[16];
+  __shared__ float2 part[8];                          // (max, sum) of every CTA of the cluster
+  const int tid = threadIdx.x, nt = blockDim.x;
+  const uint32_t C = cluster_size(), rank = cluster_rank();
+  const int64_t row = blockIdx.x / C;
+  int si = 0;                                         // the row's sequence
+  while (si + 1 < seqs.n && seqs.start[si + 1] <= row) ++si;
+  const double w = seqs.w[si];
+  const T* x = logits + row * ld;
+  T* g = grad + row * ld_grad;
+  const int32_t target = targets[row];
+  const bool valid = target >= 0 && target < V;
+
+  // this CTA's columns [c0, c1); [v0, v1) of them are whole 16-byte vectors
+  const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T);   // to the row's first boundary
+  const int64_t per = ((V + C - 1) / C + N - 1) / N * N;
+  auto cut = [&](int64_t r) {                         // slices meet at 16-byte boundaries
+    const int64_t c = r == 0 ? 0 : head + r * per;
+    return c < V ? (r == C ? V : c) : V;
+  };
+  const int64_t c0 = cut(rank), c1 = cut(rank + 1);
+  const int64_t v0 = rank == 0 ? (head < c1 ? head : c1) : c0;
+  const int64_t nvec = (c1 - v0) / N, v1 = v0 + nvec * N;
+  const bool same = (reinterpret_cast<uintptr_t>(g + v0) & 15) == 0;   // the gradient's row has the same phase
+
+  const float xt = (rank == 0 && tid == 0 && valid) ? Vec<T>::one(x + target) : 0.f;
+  float m = -INFINITY, s = 0.f;
+  constexpr int UN = 4;
+  for (int64_t i = tid; i < nvec; i += static_cast<int64_t>(UN) * nt) {
+    float y[UN][N];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (i + u * nt < nvec) {
+        Vec<T>::load(x + v0 + (i + u * nt) * N, y[u]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) y[u][k] = -INFINITY;
+      }
+    }
+    float top = y[0][0];
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) top = fmaxf(top, y[u][k]);
+    const float t = fmaxf(m, top);
+    const float b = t == -INFINITY ? 0.f : t;         // -inf logits alone: every exponential is 0
+    float a = 0.f;
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) a += exp_of(y[u][k] - b);
+    s = s * exp_of(m - b) + a;
+    m = t;
+  }
+  if (tid < 2 * N) {                                  // head and tail, one element a thread
+    const int64_t c = tid < N ? c0 + tid : v1 + (tid - N);
+    if (c < (tid < N ? v0 : c1)) {
+      const float y = Vec<T>::one(x + c);
+      merge(m, s, y, y == -INFINITY ? 0.f : (y == y ? 1.f : y));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+  if ((tid & 31) == 0) red[tid >> 5] = make_float2(m, s);
+  __syncthreads();
+  m = red[0].x;
+  s = red[0].y;
+  for (int q = 1; q < nt / 32; ++q) merge(m, s, red[q].x, red[q].y);
+  if (C > 1) {
+    if (tid < static_cast<int>(C)) st_cluster(&part[rank], tid, m, s);
+    cluster_sync();
+    m = part[0].x;
+    s = part[0].y;
+    for (uint32_t q = 1; q < C; ++q) merge(m, s, part[q].x, part[q].y);
+  } else {
+    __syncthreads();                                  // xt is read before any gradient is written
+  }
+  const float bad = __int_as_float(0x7fc00000);
+  if (rank == 0 && tid == 0) {
+    // the difference first: at the type's lowest value even fp64 would swallow log s
+    const double nll = (static_cast<double>(m) - static_cast<double>(xt)) + log(static_cast<double>(s));
+    term[row] = valid ? nll * w : static_cast<double>(bad);
+  }
+  const float wf = valid ? static_cast<float>(w * grad_scale) : bad;
+  const float inv = 1.f / s;
+  auto value = [&](float y, int64_t c) {
+    const float p = exp_of(y - m) * inv;
+    return wf * (c == target ? p - 1.f : p);
+  };
+  for (int64_t i = tid; i < nvec; i += 2 * nt) {
+    float y[2][N];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (i + u * nt < nvec) Vec<T>::load(x + v0 + (i + u * nt) * N, y[u]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (i + u * nt >= nvec) break;
+      const int64_t c = v0 + (i + u * nt) * N;
+#pragma unroll
+      for (int k = 0; k < N; ++k) y[u][k] = value(y[u][k], c + k);
+      if (same) {
+        Vec<T>::store(g + c, y[u]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) Vec<T>::put(g + c + k, y[u][k]);
+      }
+    }
+  }
+  if (tid < 2 * N) {
+    const int64_t c = tid < N ? c0 + tid : v1 + (tid - N);
+    if (c < (tid < N ? v0 : c1)) Vec<T>::put(g + c, value(Vec<T>::one(x + c), c));
+  }
+}
+
+// loss[0] = the terms' sum in fp64 in token order (each thread a contiguous run, the runs in
+// thread order), rounded once.
+__global__ void __launch_bounds__(256) k_loss_sum(const double* __restrict__ term, int64_t ntok, float* loss) {
+  __shared__ double part[256];
+  const int tid = threadIdx.x;
+  const int64_t per = (ntok + 255) / 256;
+  double a = 0.0;
+  for (int64_t i = tid * per; i < min(ntok, (tid + 1) * per); ++i) a += term[i];
+  part[tid] = a;
+  __syncthreads();
+  if (tid == 0) {
+    double s = 0.0;
+    for (int i = 0; i < 256; ++i) s += part[i];
+    loss[0] = static_cast<float>(s);
+  }
+}
+
+}  // namespace sg
+}  // namespace dsmz

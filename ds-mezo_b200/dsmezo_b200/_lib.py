@@ -149,6 +149,10 @@ SIGNATURES = {
     "dsmz_step_kalman_sums": (c_void_p, [c_void_p]),
     "dsmz_step_update": (c_int32, [c_void_p, c_float, c_float, c_float, c_float, c_float, POINTER(NSSchedule),
                                    c_void_p]),
+    "dsmz_contrastive_loss_grad_workspace_bytes": (c_size_t, [c_int64]),
+    "dsmz_contrastive_loss_grad": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, POINTER(c_int64),
+                                             POINTER(c_double), c_int32, c_double, c_void_p, c_void_p, c_int64,
+                                             c_void_p, c_size_t, c_void_p]),
     "dsmz_adamw_step": (c_int32, [POINTER(AdamWDesc), POINTER(AdamWTensor), c_int32, c_void_p, c_size_t, c_void_p]),
     "dsmz_adamw_state_values": (c_int32, [POINTER(AdamWTensor), c_int32, c_void_p]),
     "dsmz_plan_set_probe": (c_int32, [c_void_p, c_int32, POINTER(c_void_p), POINTER(c_void_p), c_int32]),

@@ -4,12 +4,14 @@ The reference pulls every scored token's logprob from vLLM into Python lists and
 ``sum_i adv_i * mean NLL(sequence i)`` for the + and - adapters on the host. Here the
 logits rows that predict the scored tokens (or their logprobs) stay on the GPU and one
 fused pass (log-sum-exp per row, target pick, advantage-weighted mean per sequence, fixed
-summation order) returns the loss as a device fp64 scalar.
+summation order) returns the loss as a device fp64 scalar. ``contrastive_loss_grad`` returns
+the loss with its gradient in the logits, for first-order steps of the adapters (no reference
+counterpart).
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -60,6 +62,53 @@ def contrastive_loss(src: torch.Tensor, seq_tokens: Sequence[int], advantages: S
                                   ws.data_ptr(), wsb, torch.cuda.current_stream(src.device).cuda_stream),
           "dsmz_contrastive_loss")
     return out
+
+
+def contrastive_loss_grad(logits: torch.Tensor, seq_tokens: Sequence[int], advantages: Sequence[float],
+                          targets: torch.Tensor, *, out: Optional[torch.Tensor] = None,
+                          grad_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``contrastive_loss`` of the logits rows and its gradient in them.
+
+    logits (ntok x V, fp32 or bf16, unit column stride), seq_tokens, advantages and targets as
+    for ``contrastive_loss``. Returns (loss, grad): a one-element fp32 tensor and a tensor of
+    the logits' shape and type, grad_scale * d loss / d logits, written on the current stream.
+    out: where the gradient goes; it may be the logits themselves. NaN where a target lies
+    outside the vocabulary (the loss and that row). seq_tokens, advantages and grad_scale are
+    read during the call: a captured call replays with the same ones."""
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
+        raise ValueError("contrastive_loss_grad takes CUDA tensors only (no CPU fallback)")
+    n = len(seq_tokens)
+    if n != len(advantages):
+        raise ValueError("contrastive_loss_grad: one advantage per sequence")
+    ntok = int(sum(seq_tokens))
+    if logits.dim() != 2 or logits.shape[0] != ntok or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("contrastive_loss_grad: logits must be sum(seq_tokens) x V with unit column stride")
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("contrastive_loss_grad: logits must be float32 or bfloat16")
+    if targets.dtype != torch.int32 or targets.numel() != ntok or targets.device != logits.device:
+        raise ValueError("contrastive_loss_grad: targets must be ntok int32 token ids on the logits' device")
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or \
+            (out.shape[1] > 1 and out.stride(1) != 1):
+        raise ValueError("contrastive_loss_grad: out must have the logits' shape, type, device and unit column stride")
+    V = logits.shape[1]
+    ld, ld_out = (max(t.stride(0), V) if ntok == 1 else t.stride(0) for t in (logits, out))
+    tgt = targets.contiguous()
+    start = (ctypes.c_int64 * (n + 1))()
+    for i, k in enumerate(seq_tokens):
+        start[i + 1] = start[i] + int(k)
+    adv = (ctypes.c_double * max(n, 1))(*[float(a) for a in advantages])
+    L = lib()
+    with torch.cuda.device(logits.device):
+        wsb = int(L.dsmz_contrastive_loss_grad_workspace_bytes(ntok))
+        ws = torch.empty(wsb, dtype=torch.uint8, device=logits.device)
+        loss = torch.empty(1, dtype=torch.float32, device=logits.device)
+        check(L.dsmz_contrastive_loss_grad(
+            SCORE_LOGITS_F32 if logits.dtype == torch.float32 else SCORE_LOGITS_BF16, logits.data_ptr(), V, ld,
+            tgt.data_ptr(), ntok, start, adv, n, float(grad_scale), loss.data_ptr(), out.data_ptr(), ld_out,
+            ws.data_ptr(), wsb, torch.cuda.current_stream(logits.device).cuda_stream), "contrastive_loss_grad")
+    return loss, out
 
 
 def projected_gradient(loss_pos: float, loss_neg: float, eps: float) -> float:

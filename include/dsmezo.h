@@ -368,6 +368,21 @@ int dsmz_step_update_directions(const dsmz_plan* plan, const float* dd, int32_t 
  * zeroth-order updates only).
  * ------------------------------------------------------------------------------- */
 
+/* The contrastive scoring loss (dsmz_contrastive_loss) with its gradient in the logits:
+ *   loss[0] (device F32; the terms and their sum are fp64) = sum_i a_i mean_{t in i} nll_t
+ *   grad[t][c] = grad_scale a_i / n_i (softmax(logits row t)[c] - [c == targets[t]])
+ * logits (kind DSMZ_SCORE_LOGITS_F32 / _BF16) and grad have one type and unit column stride,
+ * row pitches ld and ld_grad >= V, any alignment of their element type. grad may be the
+ * logits' own buffer (same pitch); other overlaps are refused. Sequences, advantages and the
+ * order of the sums as for dsmz_contrastive_loss; both are host arrays, so a captured call
+ * keeps the ones it was captured with. A target outside [0, V) makes the loss and its row of
+ * grad NaN. Deterministic. */
+size_t dsmz_contrastive_loss_grad_workspace_bytes(int64_t ntok);
+int dsmz_contrastive_loss_grad(int32_t kind, const void* logits, int64_t V, int64_t ld, const int32_t* targets,
+                               int64_t ntok, const int64_t* seq_start, const double* advantages, int32_t nseq,
+                               double grad_scale, float* loss, void* grad, int64_t ld_grad, void* workspace,
+                               size_t workspace_bytes, dsmz_stream_t stream);
+
 /* AdamW over many tensors:
  *   m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2   (g times *grad_scale when given)
  *   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)

@@ -71,3 +71,36 @@ def test_adamw_takes_no_cpu_tensors(lib):
     from dsmezo_b200 import AdamW
     with pytest.raises(ValueError, match="CUDA"):
         AdamW([torch.zeros(4)])
+
+
+def loss_grad(lib, **kw):
+    a = dict(kind=0, logits=4096, V=8, ld=8, targets=4096, ntok=4, starts=(0, 4), adv=(1.0,), nseq=1, scale=1.0,
+             loss=4096, grad=8192, ld_grad=8, ws=4096, ws_bytes=64)
+    a.update(kw)
+    starts = None if a["starts"] is None else (ctypes.c_int64 * len(a["starts"]))(*a["starts"])
+    adv = None if a["adv"] is None else (ctypes.c_double * len(a["adv"]))(*a["adv"])
+    return lib.lib().dsmz_contrastive_loss_grad(a["kind"], a["logits"], a["V"], a["ld"], a["targets"], a["ntok"], starts,
+                                                adv, a["nseq"], a["scale"], a["loss"], a["grad"], a["ld_grad"], a["ws"],
+                                                a["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("bad", [dict(kind=2), dict(logits=None), dict(targets=None), dict(loss=None), dict(grad=None),
+                                 dict(starts=None), dict(adv=None), dict(V=0), dict(ld=7), dict(ld_grad=7),
+                                 dict(ntok=0, starts=(0, 0)), dict(starts=(1, 4)), dict(starts=(0, 3)),
+                                 dict(nseq=0), dict(nseq=129, starts=(0,) * 129 + (4,), adv=(1.0,) * 129),
+                                 dict(nseq=2, starts=(0, 4, 4), adv=(1.0, 1.0)), dict(scale=float("inf")),
+                                 dict(logits=4098), dict(grad=4100), dict(V=1 << 31, ld=1 << 31, ld_grad=1 << 31)])
+def test_loss_grad_refuses(lib, bad):
+    assert loss_grad(lib, **bad) == 1
+    assert b"dsmz_contrastive_loss_grad" in lib.lib().dsmz_last_error()
+
+
+def test_loss_grad_workspace(lib):
+    assert lib.lib().dsmz_contrastive_loss_grad_workspace_bytes(4) == 32
+    assert loss_grad(lib, ws_bytes=31) == 2 and loss_grad(lib, ws=4097) == 2 and loss_grad(lib, ws=None) == 1
+
+
+def test_loss_grad_takes_no_cpu_tensors(lib):
+    from dsmezo_b200 import scoring
+    with pytest.raises(ValueError, match="CUDA"):
+        scoring.contrastive_loss_grad(torch.zeros(2, 4), [2], [1.0], torch.zeros(2, dtype=torch.int32))
