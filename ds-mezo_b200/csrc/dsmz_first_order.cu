@@ -144,13 +144,13 @@ int loss_grad(const void* logits, int64_t V, int64_t ld, const int32_t* targets,
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return cuda_fail("dsmz_contrastive_loss_grad: device query", e);
-  // CTAs a row: enough that a slice stays in L1 between the two passes, and that a few rows
-  // still occupy the machine twice over while a slice is worth a CTA
+  // CTAs a row: slices of at most kSliceBytes, and more where a few rows would leave SMs idle
+  // while a slice is still worth a CTA
   const int64_t row_bytes = V * static_cast<int64_t>(sizeof(T));
   int C = 1;
   while (C < 8 && (row_bytes / C > sg::kSliceBytes || (ntok * C < 2 * sms && row_bytes / C > 8192))) C *= 2;
   const int64_t vecs = (row_bytes / C + 15) / 16;
-  const int threads = vecs >= 1024 ? 512 : (vecs >= 256 ? 256 : 128);
+  const int threads = vecs >= 256 ? 256 : 128;
   if (ntok * C > 0x7fffffff) return fail(DSMZ_ERR_UNSUPPORTED, "dsmz_contrastive_loss_grad: too many tokens");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ntok * C));

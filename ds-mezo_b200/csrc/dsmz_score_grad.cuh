@@ -4,21 +4,26 @@
 // (ds_mezo/controller.py:14-15, 194-201 for the loss; the reference takes no gradient of it).
 //
 // A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary. Pass one
-// over the slice keeps a running maximum and sum of exponentials a thread; the CTAs exchange (max, sum) through distributed shared memory;
-// pass two reads the slice again, from L1 while it is at most kSliceBytes, and writes the
-// gradient. HBM sees each logit once in and each gradient once out, which is the floor.
+// over the slice keeps a running maximum and sum of exponentials a thread; the CTAs exchange
+// (max, sum) through distributed shared memory; pass two reads the slice again, from L2 (a cluster's barrier empties L1), and writes the
+// gradient. HBM sees each logit once in and each gradient once out, which is the floor: 190 us
+// for 2048 rows of 152064 bf16 logits, of which this takes 273 (0.70). The unit that makes
+// exponentials and packs bf16 pairs is 61% busy (2.5 operations a logit), the rest is the
+// latency of a slice's two passes.
 // Rows need not be aligned: a slice has a scalar head up to the first 16-byte boundary,
 // 16-byte accesses, and a scalar tail. The target's logit is read before the exchange, so
 // the gradient may overwrite the logits.
 //
 // The maximum is subtracted before the scaling by log2 e: with the product first (one FMA a
 // logit less) masks at the type's lowest value overflow, and logits past 2^24 lose the
-// difference itself. Rows of -inf only, NaN and +inf follow the formula: NaN. A target outside the vocabulary
-// makes the loss and its row of the gradient NaN.
+// difference itself. Rows of -inf only, NaN and +inf follow the formula: NaN. A target outside
+// the vocabulary makes the loss and its row of the gradient NaN.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "dsmz_ptx.cuh"
 
@@ -26,7 +31,10 @@ namespace dsmz {
 namespace sg {
 
 constexpr int kMaxSeqs = 128;
-constexpr int kSliceBytes = 40 * 1024;   // four CTAs of 512 threads an SM keep their slices in L1
+// Largest slice of a row. 2048 rows of 152064 bf16 logits (304 KB) took 311, 297, 273 and 345 us
+// with 1, 2, 4 and 8 CTAs of 256 threads a row (293, 279, 361 and 515 us with 512 threads):
+// more CTAs cut the tail of the last wave, and past slices of 76 KB their barriers cost more.
+constexpr int kSliceBytes = 80 * 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Seqs {
@@ -110,11 +118,11 @@ template <> struct Vec<__nv_bfloat16> {
 
 // grid: ntok * cluster size; row = blockIdx.x / cluster size.
 template <typename T>
-__global__ void __launch_bounds__(512) k_loss_grad(const T* logits, int64_t ld, int64_t V,
+__global__ void __launch_bounds__(256) k_loss_grad(const T* logits, int64_t ld, int64_t V,
                                                    const int32_t* __restrict__ targets, Seqs seqs, double grad_scale,
                                                    T* grad, int64_t ld_grad, double* __restrict__ term) {
   constexpr int N = Vec<T>::N;
-  __shared__ float2 red[16];
+  __shared__ float2 red[8];
   __shared__ float2 part[8];                          // (max, sum) of every CTA of the cluster
   const int tid = threadIdx.x, nt = blockDim.x;
   const uint32_t C = cluster_size(), rank = cluster_rank();
@@ -139,35 +147,33 @@ __global__ void __launch_bounds__(512) k_loss_grad(const T* logits, int64_t ld, 
   const int64_t nvec = (c1 - v0) / N, v1 = v0 + nvec * N;
   const bool same = (reinterpret_cast<uintptr_t>(g + v0) & 15) == 0;   // the gradient's row has the same phase
 
-  const float xt = (rank == 0 && tid == 0 && valid) ? Vec<T>::one(x + target) : 0.f;
+  const float xt = (tid == 0 && valid) ? Vec<T>::one(x + target) : 0.f;
   float m = -INFINITY, s = 0.f;
-  constexpr int UN = 4;
-  for (int64_t i = tid; i < nvec; i += static_cast<int64_t>(UN) * nt) {
+  const T* xv = x + v0;
+  const int nv = static_cast<int>(nvec);
+  // UN vectors a thread: one maximum and one rescaling of the running sum for all of them
+  auto block = [&](auto un, int i) {
+    constexpr int UN = decltype(un)::value;
     float y[UN][N];
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      if (i + u * nt < nvec) {
-        Vec<T>::load(x + v0 + (i + u * nt) * N, y[u]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) y[u][k] = -INFINITY;
-      }
-    }
-    float top = y[0][0];
+    for (int u = 0; u < UN; ++u) Vec<T>::load(xv + static_cast<int64_t>(i + u * nt) * N, y[u]);
+    float t = m;
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
-      for (int k = 0; k < N; ++k) top = fmaxf(top, y[u][k]);
-    const float t = fmaxf(m, top);
+      for (int k = 0; k < N; ++k) t = fmaxf(t, y[u][k]);
     const float b = t == -INFINITY ? 0.f : t;         // -inf logits alone: every exponential is 0
-    float a = 0.f;
+    float a[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
-      for (int k = 0; k < N; ++k) a += exp_of(y[u][k] - b);
-    s = s * exp_of(m - b) + a;
+      for (int k = 0; k < N; ++k) a[k & 1] += exp_of(y[u][k] - b);
+    s = s * exp_of(m - b) + (a[0] + a[1]);
     m = t;
-  }
+  };
+  int i = tid;
+  for (; i + 3 * nt < nv; i += 4 * nt) block(std::integral_constant<int, 4>{}, i);
+  for (; i < nv; i += nt) block(std::integral_constant<int, 1>{}, i);
   if (tid < 2 * N) {                                  // head and tail, one element a thread
     const int64_t c = tid < N ? c0 + tid : v1 + (tid - N);
     if (c < (tid < N ? v0 : c1)) {
@@ -179,17 +185,21 @@ __global__ void __launch_bounds__(512) k_loss_grad(const T* logits, int64_t ld, 
   for (int o = 16; o > 0; o >>= 1) merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
   if ((tid & 31) == 0) red[tid >> 5] = make_float2(m, s);
   __syncthreads();
-  m = red[0].x;
-  s = red[0].y;
-  for (int q = 1; q < nt / 32; ++q) merge(m, s, red[q].x, red[q].y);
+  // every warp merges the warps' pairs, then the CTAs' (lanes past them hold the empty pair)
+  const int lane = tid & 31;
+  m = lane < nt / 32 ? red[lane].x : -INFINITY;
+  s = lane < nt / 32 ? red[lane].y : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
   if (C > 1) {
     if (tid < static_cast<int>(C)) st_cluster(&part[rank], tid, m, s);
     cluster_sync();
-    m = part[0].x;
-    s = part[0].y;
-    for (uint32_t q = 1; q < C; ++q) merge(m, s, part[q].x, part[q].y);
-  } else {
-    __syncthreads();                                  // xt is read before any gradient is written
+    m = lane < static_cast<int>(C) ? part[lane].x : -INFINITY;
+    s = lane < static_cast<int>(C) ? part[lane].y : 0.f;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+    m = __shfl_sync(0xffffffffu, m, 0);
+    s = __shfl_sync(0xffffffffu, s, 0);
   }
   const float bad = __int_as_float(0x7fc00000);
   if (rank == 0 && tid == 0) {
@@ -199,33 +209,43 @@ __global__ void __launch_bounds__(512) k_loss_grad(const T* logits, int64_t ld, 
   }
   const float wf = valid ? static_cast<float>(w * grad_scale) : bad;
   const float inv = 1.f / s;
-  auto value = [&](float y, int64_t c) {
-    const float p = exp_of(y - m) * inv;
-    return wf * (c == target ? p - 1.f : p);
-  };
-  for (int64_t i = tid; i < nvec; i += 2 * nt) {
-    float y[2][N];
+  auto value = [&](float y) { return wf * (exp_of(y - m) * inv); };
+  T* gv = g + v0;
+  if (same) {
+    i = tid;
+    for (; i + 3 * nt < nv; i += 4 * nt) {
+      float y[4][N];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (i + u * nt < nvec) Vec<T>::load(x + v0 + (i + u * nt) * N, y[u]);
+      for (int u = 0; u < 4; ++u) Vec<T>::load(xv + static_cast<int64_t>(i + u * nt) * N, y[u]);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (i + u * nt >= nvec) break;
-      const int64_t c = v0 + (i + u * nt) * N;
+      for (int u = 0; u < 4; ++u) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) y[u][k] = value(y[u][k], c + k);
-      if (same) {
-        Vec<T>::store(g + c, y[u]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) Vec<T>::put(g + c + k, y[u][k]);
+        for (int k = 0; k < N; ++k) y[u][k] = value(y[u][k]);
+        Vec<T>::store(gv + static_cast<int64_t>(i + u * nt) * N, y[u]);
       }
+    }
+    for (; i < nv; i += nt) {
+      float y[N];
+      Vec<T>::load(xv + static_cast<int64_t>(i) * N, y);
+#pragma unroll
+      for (int k = 0; k < N; ++k) y[k] = value(y[k]);
+      Vec<T>::store(gv + static_cast<int64_t>(i) * N, y);
+    }
+  } else {
+    for (i = tid; i < nv; i += nt) {
+      float y[N];
+      Vec<T>::load(xv + static_cast<int64_t>(i) * N, y);
+#pragma unroll
+      for (int k = 0; k < N; ++k) Vec<T>::put(gv + static_cast<int64_t>(i) * N + k, value(y[k]));
     }
   }
   if (tid < 2 * N) {
     const int64_t c = tid < N ? c0 + tid : v1 + (tid - N);
-    if (c < (tid < N ? v0 : c1)) Vec<T>::put(g + c, value(Vec<T>::one(x + c), c));
+    if (c < (tid < N ? v0 : c1)) Vec<T>::put(g + c, value(Vec<T>::one(x + c)));
   }
+  __syncthreads();                                    // the target's element, once the slice is written
+  // xt was read before the first barrier, so before any gradient was written
+  if (tid == 0 && valid && target >= c0 && target < c1) Vec<T>::put(g + target, wf * (exp_of(xt - m) * inv - 1.f));
 }
 
 // loss[0] = the terms' sum in fp64 in token order (each thread a contiguous run, the runs in
