@@ -1,11 +1,12 @@
-// C ABI of the first-order operators declared in dsmezo.h: the scoring loss with its gradient
-// and AdamW over many tensors.
+// C ABI of the first-order operators declared in dsmezo.h: products grouped by adapter copy,
+// the scoring loss with its gradient, and AdamW over many tensors.
 #include <cmath>
 #include <exception>
 #include <vector>
 
 #include "dsmezo.h"
 #include "dsmz_adamw.cuh"
+#include "dsmz_grouped.cuh"
 #include "dsmz_host.h"
 #include "dsmz_score_grad.cuh"
 
@@ -136,6 +137,97 @@ int adamw_run(const dsmz_adamw_desc& d, const dsmz_adamw_tensor* tensors, int32_
       [&](const aw::Args<CAP>& a, int grid) { launch_adamw<CAP>(a, grid, d.param_dtype, d.grad_dtype, d.state_bits, s); });
 }
 
+// ------------------------------------------------------------------ products grouped by adapter copy
+// Error word of the grouped products' bounded waits, one per device.
+__device__ int g_grouped_err;
+
+// bf16 tensor map of rank 2 or 3 (inner dimension contiguous, byte strides of the others),
+// 128-byte swizzle, zero fill outside.
+bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                 uint32_t box0, uint32_t box1) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t d[3] = {dims[0], dims[1], rank == 3 ? dims[2] : 1}, st[2] = {strides[0], rank == 3 ? strides[1] : 0};
+  cuuint32_t box[3] = {box0, box1, 1}, es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count(int* sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  return e == cudaSuccess ? 0 : cuda_fail("device query", e);
+}
+
+template <int BNT, int MODE>
+int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, int64_t tiles, int sms, const char* what,
+                   cudaStream_t s) {
+  constexpr int SB = gr::kABytes + BNT * gr::kBK * 2;
+  constexpr int kSmem = 227 * 1024;
+  const int scratch = a.split > 1 ? gr::kBM * (BNT + 4) * 4 : gr::kEpiWarps * 32 * gr::kStagePitch;
+  const int fixed = 1024 + scratch + (((a.G + 3) * 8 + 15) & ~15) + 64 + 16 * 8;
+  a.stages = (kSmem - fixed) / SB;
+  if (a.stages > 8) a.stages = 8;
+  const size_t smem = static_cast<size_t>(fixed) + static_cast<size_t>(a.stages) * SB;
+  auto* kernel = gr::k_grouped<BNT, MODE>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return cuda_fail(what, e);
+  static thread_local int* err = nullptr;
+  static thread_local int err_dev = -1;
+  int dev = 0;
+  e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev != err_dev || !err)) {
+    void* p = nullptr;
+    e = cudaGetSymbolAddress(&p, g_grouped_err);
+    err = static_cast<int*>(p);
+    err_dev = dev;
+  }
+  if (e != cudaSuccess) return cuda_fail(what, e);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.split > 1 ? tiles * a.split : (tiles < sms ? tiles : sms)));
+  cfg.blockDim = dim3(gr::kThreadsG);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(a.split);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, A, B, a, err);
+  return e == cudaSuccess ? DSMZ_OK : cuda_fail(what, e);
+}
+
+template <int MODE>
+int launch_grouped_bn(int bnt, const gr::Args& a, const CUtensorMap& A, const CUtensorMap& B, int64_t tiles, int sms,
+                      const char* what, cudaStream_t s) {
+  if (bnt == 64) return launch_grouped<64, MODE>(a, A, B, tiles, sms, what, s);
+  if (bnt == 128) return launch_grouped<128, MODE>(a, A, B, tiles, sms, what, s);
+  return launch_grouped<256, MODE>(a, A, B, tiles, sms, what, s);
+}
+
+// Accumulator width for n output columns and `rows` row tiles: 256 columns where that still
+// gives every SM a tile.
+int columns_for(int64_t n, int64_t rows, int sms) {
+  if (n <= 64) return 64;
+  if (n <= 128) return 128;
+  return rows * ((n + 255) / 256) >= sms ? 256 : 128;
+}
+// CTAs that share a tile's contraction: as many as one wave of the machine holds, while each
+// still has two k-steps.
+int split_for(int bnt, int64_t tiles, int64_t nk, int sms) {
+  int s = 1;
+  while (s < 8 && bnt <= 128 && tiles * 2 * s <= sms && nk / (2 * s) >= 2) s *= 2;
+  return s;
+}
+
+bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
+}
+
 // ------------------------------------------------------------------ scoring loss with its gradient
 template <typename T>
 int loss_grad(const void* logits, int64_t V, int64_t ld, const int32_t* targets, int64_t ntok, const sg::Seqs& q,
@@ -173,6 +265,142 @@ int loss_grad(const void* logits, int64_t V, int64_t ld, const int32_t* targets,
 }  // namespace
 
 extern "C" {
+
+int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const void* w, int32_t G, int64_t N,
+                        int64_t w_group_stride, int64_t w_ld, int32_t w_n_contiguous, const int32_t* row_offsets,
+                        int32_t out_dtype, void* out, int64_t ld_out, float alpha, uint32_t flags,
+                        dsmz_stream_t stream) {
+  return guarded("dsmz_grouped_matmul", [&]() -> int {
+    const std::string me = "dsmz_grouped_matmul: ";
+    if (M < 0 || K < 1 || N < 1 || G < 1) return fail(DSMZ_ERR_INVALID, me + "need M >= 0, K >= 1, N >= 1 and G >= 1");
+    if (G > DSMZ_MAX_GROUPS || M > DSMZ_MAX_GROUPED_DIM || K > DSMZ_MAX_GROUPED_DIM || N > DSMZ_MAX_GROUPED_DIM)
+      return fail(DSMZ_ERR_UNSUPPORTED, me + "at most DSMZ_MAX_GROUPS groups and DSMZ_MAX_GROUPED_DIM rows or columns");
+    if (out_dtype != DSMZ_F32 && out_dtype != DSMZ_BF16) return fail(DSMZ_ERR_INVALID, me + "out must be DSMZ_F32 or DSMZ_BF16");
+    if (flags & ~(DSMZ_GROUPED_ACCUMULATE | DSMZ_GROUPED_ZERO_REST)) return fail(DSMZ_ERR_INVALID, me + "unknown flag");
+    if (M == 0) return DSMZ_OK;
+    if (!x || !w || !row_offsets || !out) return fail(DSMZ_ERR_INVALID, me + "null pointer");
+    const int64_t wi = w_n_contiguous ? N : K, wo = w_n_contiguous ? K : N;      // inner and outer width of W_g
+    const int es = out_dtype == DSMZ_F32 ? 4 : 2;
+    if (ld_x < K || w_ld < wi || ld_out < N || (G > 1 && w_group_stride < 1) || ld_x > kMaxElems || w_ld > kMaxElems ||
+        ld_out > kMaxElems || w_group_stride > kMaxElems)
+      return fail(DSMZ_ERR_INVALID, me + "a pitch is smaller than its row, or a stride is out of range");
+    if (!aligned(x, 16) || !aligned(w, 16) || ld_x % 8 || w_ld % 8 || (G > 1 && w_group_stride % 8))
+      return fail(DSMZ_ERR_INVALID, me + "x and w need 16-byte aligned bases and strides that are multiples of 8 elements");
+    if (!aligned(out, es) || !aligned(row_offsets, 4)) return fail(DSMZ_ERR_INVALID, me + "a pointer is not aligned to its type");
+    if (!std::isfinite(alpha)) return fail(DSMZ_ERR_INVALID, me + "alpha must be finite");
+    const int64_t nout = ((M - 1) * ld_out + N) * es;
+    if (overlaps(out, nout, x, ((M - 1) * ld_x + K) * 2) || overlaps(out, nout, w, ((G - 1) * w_group_stride + (wo - 1) * w_ld + wi) * 2))
+      return fail(DSMZ_ERR_INVALID, me + "out overlaps an operand");
+    int sms = 0, rc = sm_count(&sms);
+    if (rc) return rc;
+    gr::Args a{};
+    a.offsets = row_offsets;
+    a.G = G;
+    a.M = M;
+    a.ndim = static_cast<int32_t>(N);
+    a.kdim = static_cast<int32_t>(K);
+    a.b_mn = w_n_contiguous ? 1 : 0;
+    a.out = out;
+    a.ld = ld_out;
+    a.out_f32 = out_dtype == DSMZ_F32;
+    a.accumulate = (flags & DSMZ_GROUPED_ACCUMULATE) ? 1 : 0;
+    a.zero_rest = (flags & DSMZ_GROUPED_ZERO_REST) && !a.accumulate;
+    a.vec = aligned(out, 16) && (ld_out * es) % 16 == 0;
+    a.alpha = alpha;
+    a.chunk = a.out_f32 ? gr::kChunk : 0x3fffffff;
+    const int64_t rows = (M + gr::kBM - 1) / gr::kBM + (G < M ? G : M) - 1;      // most row tiles the groups can have
+    const int bnt = columns_for(N, rows, sms);
+    a.bn = static_cast<int32_t>(N >= bnt ? bnt : (N + 15) / 16 * 16);
+    a.ntn = static_cast<int32_t>((N + a.bn - 1) / a.bn);
+    a.split = split_for(bnt, rows * a.ntn, (K + gr::kBK - 1) / gr::kBK, sms);
+    // short groups: boxes of 32 rows, so that a tile does not fetch 128
+    a.arows = M / G >= 96 ? gr::kBM : 32;
+    const int64_t tiles = (rows + 2) * a.ntn;                                    // and the rows outside the groups
+    if (tiles > (1 << 27)) return fail(DSMZ_ERR_UNSUPPORTED, me + "too many tiles");
+    CUtensorMap A, B;
+    const uint64_t da[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(M)}, sa[1] = {static_cast<uint64_t>(ld_x) * 2};
+    const uint64_t db[3] = {static_cast<uint64_t>(wi), static_cast<uint64_t>(wo), static_cast<uint64_t>(G)};
+    const uint64_t sb[2] = {static_cast<uint64_t>(w_ld) * 2,
+                            static_cast<uint64_t>(G > 1 ? w_group_stride : (w_ld * wo + 7) / 8 * 8) * 2};
+    if (!encode_bf16(&A, x, 2, da, sa, gr::kBK, static_cast<uint32_t>(a.arows)) ||
+        !encode_bf16(&B, w, 3, db, sb, 64, w_n_contiguous ? 64 : static_cast<uint32_t>(a.bn)))
+      return fail(DSMZ_ERR_CUDA, me + "the driver refused a tensor map");
+    return launch_grouped_bn<0>(bnt, a, A, B, tiles, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
+  });
+}
+
+int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, const void* dy, int64_t N, int64_t ld_dy,
+                             int32_t G, const int32_t* row_offsets, float* out, float alpha, uint32_t flags,
+                             dsmz_stream_t stream) {
+  return guarded("dsmz_grouped_weight_grad", [&]() -> int {
+    const std::string me = "dsmz_grouped_weight_grad: ";
+    if (M < 0 || K < 1 || N < 1 || G < 1) return fail(DSMZ_ERR_INVALID, me + "need M >= 0, K >= 1, N >= 1 and G >= 1");
+    if (G > DSMZ_MAX_GROUPS || M > DSMZ_MAX_GROUPED_DIM || K > DSMZ_MAX_GROUPED_DIM || N > DSMZ_MAX_GROUPED_DIM)
+      return fail(DSMZ_ERR_UNSUPPORTED, me + "at most DSMZ_MAX_GROUPS groups and DSMZ_MAX_GROUPED_DIM rows or columns");
+    if (flags & ~DSMZ_GROUPED_ACCUMULATE) return fail(DSMZ_ERR_INVALID, me + "unknown flag");
+    if (!out || (M > 0 && (!x || !dy || !row_offsets))) return fail(DSMZ_ERR_INVALID, me + "null pointer");
+    if (!aligned(out, 4) || !aligned(row_offsets, 4)) return fail(DSMZ_ERR_INVALID, me + "a pointer is not aligned to its type");
+    if (!std::isfinite(alpha)) return fail(DSMZ_ERR_INVALID, me + "alpha must be finite");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (M == 0) {
+      if (flags & DSMZ_GROUPED_ACCUMULATE) return DSMZ_OK;
+      cudaError_t e = cudaMemsetAsync(out, 0, static_cast<size_t>(G) * K * N * sizeof(float), s);
+      return e == cudaSuccess ? DSMZ_OK : cuda_fail("dsmz_grouped_weight_grad", e);
+    }
+    if (ld_x < K || ld_dy < N || ld_x > kMaxElems || ld_dy > kMaxElems)
+      return fail(DSMZ_ERR_INVALID, me + "a pitch is smaller than its row, or out of range");
+    if (!aligned(x, 16) || !aligned(dy, 16) || ld_x % 8 || ld_dy % 8)
+      return fail(DSMZ_ERR_INVALID, me + "x and dy need 16-byte aligned bases and pitches that are multiples of 8 elements");
+    const int64_t nout = static_cast<int64_t>(G) * K * N * 4;
+    if (overlaps(out, nout, x, ((M - 1) * ld_x + K) * 2) || overlaps(out, nout, dy, ((M - 1) * ld_dy + N) * 2))
+      return fail(DSMZ_ERR_INVALID, me + "out overlaps an operand");
+    int sms = 0, rc = sm_count(&sms);
+    if (rc) return rc;
+    const bool xw = K >= N;                              // the wider operand gives the tile's 128 rows
+    const int64_t wide = xw ? K : N, narrow = xw ? N : K;
+    gr::Args a{};
+    a.offsets = row_offsets;
+    a.G = G;
+    a.M = M;
+    a.mdim = static_cast<int32_t>(wide);
+    a.ndim = static_cast<int32_t>(narrow);
+    a.out = out;
+    a.ld = N;
+    a.gstride = K * N;
+    a.transposed = xw ? 0 : 1;
+    a.out_f32 = 1;
+    a.accumulate = (flags & DSMZ_GROUPED_ACCUMULATE) ? 1 : 0;
+    a.vec = aligned(out, 16) && N % 4 == 0;
+    a.alpha = alpha;
+    a.chunk = gr::kChunk;
+    a.mtn = static_cast<int32_t>((wide + gr::kBM - 1) / gr::kBM);
+    const int bnt = columns_for(narrow, static_cast<int64_t>(G) * a.mtn, sms);
+    a.bn = static_cast<int32_t>(narrow >= bnt ? bnt : (narrow + 15) / 16 * 16);
+    a.ntn = static_cast<int32_t>((narrow + a.bn - 1) / a.bn);
+    const int64_t tiles = static_cast<int64_t>(G) * a.mtn * a.ntn;
+    if (tiles > (1 << 27)) return fail(DSMZ_ERR_UNSUPPORTED, me + "too many tiles");
+    a.split = split_for(bnt, tiles, (M / G + gr::kBK - 1) / gr::kBK, sms);
+    CUtensorMap A, B;
+    const uint64_t dx[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(M)}, sx[1] = {static_cast<uint64_t>(ld_x) * 2};
+    const uint64_t dd[2] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M)}, sd[1] = {static_cast<uint64_t>(ld_dy) * 2};
+    if (!encode_bf16(xw ? &A : &B, x, 2, dx, sx, 64, 64) || !encode_bf16(xw ? &B : &A, dy, 2, dd, sd, 64, 64))
+      return fail(DSMZ_ERR_CUDA, me + "the driver refused a tensor map");
+    return launch_grouped_bn<1>(bnt, a, A, B, tiles, sms, "dsmz_grouped_weight_grad", s);
+  });
+}
+
+int32_t dsmz_grouped_device_error(dsmz_stream_t stream) {
+  int v = -1, zero = 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cudaMemcpyFromSymbolAsync(&v, g_grouped_err, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return -1;
+  if (v != 0) {
+    cudaMemcpyToSymbolAsync(g_grouped_err, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
+    cudaStreamSynchronize(s);
+  }
+  return v;
+}
 
 size_t dsmz_contrastive_loss_grad_workspace_bytes(int64_t ntok) {
   return ntok > 0 ? static_cast<size_t>(ntok) * sizeof(double) : sizeof(double);

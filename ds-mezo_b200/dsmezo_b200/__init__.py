@@ -7,11 +7,14 @@
 * ``dsmezo_b200.sharding`` - layer-sharded step over ranks (NCCL).
 * ``dsmezo_b200.calibration`` - first-step basis width (optimal hard threshold) and the
   batched randomized SVD of the bases (``AdapterSet.calibrate``).
+* ``dsmezo_b200.grouped`` - matrix products grouped by adapter copy with ragged rows, their
+  gradients, and the adapters' rank-r products built from them.
 * ``dsmezo_b200.optim`` - AdamW over many tensors, states in fp32 or 8 bits.
 
 All compute runs in libdsmezo.so (C ABI in include/dsmezo.h); there is no CPU path.
 """
 from . import calibration  # noqa: F401
+from . import grouped  # noqa: F401
 from . import kernels  # noqa: F401
 from . import optim  # noqa: F401
 from . import scoring  # noqa: F401
@@ -26,4 +29,4 @@ from .sharding import ShardedStep, ShardLayout, partition_layers, shard_layout  
 __all__ = ["kernels", "rloo_direction_scalars", "AdapterSet", "ZOController", "ModuleShape", "BasisShape", "transformer_adapter_shapes",
            "draw_increments", "device_layout", "kalman_beta_q", "DsmzError", "lib", "ShardedStep", "ShardLayout",
            "partition_layers", "shard_layout", "ShrinkageRLOO", "eps_from_norms", "calibration",
-           "calibration_rank", "optim", "AdamW", "AdamWState"]
+           "calibration_rank", "grouped", "optim", "AdamW", "AdamWState"]

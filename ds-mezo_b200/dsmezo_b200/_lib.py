@@ -76,6 +76,8 @@ class AdamWDesc(ctypes.Structure):
                 ("step_counter", c_void_p)]
 
 
+MAX_GROUPS = 1024
+GROUPED_ACCUMULATE, GROUPED_ZERO_REST = 1, 2
 ADAMW_BLOCK = 256
 ADAMW_WORKSPACE_BYTES = 64
 MAX_DIRECTIONS = 32
@@ -149,6 +151,11 @@ SIGNATURES = {
     "dsmz_step_kalman_sums": (c_void_p, [c_void_p]),
     "dsmz_step_update": (c_int32, [c_void_p, c_float, c_float, c_float, c_float, c_float, POINTER(NSSchedule),
                                    c_void_p]),
+    "dsmz_grouped_matmul": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64,
+                                      c_int32, c_void_p, c_int32, c_void_p, c_int64, c_float, c_uint32, c_void_p]),
+    "dsmz_grouped_weight_grad": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32,
+                                           c_void_p, c_void_p, c_float, c_uint32, c_void_p]),
+    "dsmz_grouped_device_error": (c_int32, [c_void_p]),
     "dsmz_contrastive_loss_grad_workspace_bytes": (c_size_t, [c_int64]),
     "dsmz_contrastive_loss_grad": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, POINTER(c_int64),
                                              POINTER(c_double), c_int32, c_double, c_void_p, c_void_p, c_int64,

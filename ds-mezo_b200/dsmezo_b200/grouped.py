@@ -1,0 +1,161 @@
+"""Matrix products grouped by adapter copy, with ragged rows (no reference counterpart).
+
+A scoring batch holds the rollouts of the + and - copies one behind the other (2K copies with
+K directions): rows sorted by copy, a device vector of row offsets, and one factor matrix a
+copy. ``grouped_matmul`` multiplies every group of rows by its own matrix, ``grouped_weight_grad``
+forms the gradient of every matrix, and ``adapter_forward`` / ``adapter_backward`` combine them
+to the rank-r product of an adapter and its gradients. One launch for all groups; bf16
+operands, fp32 sums on the tensor cores. The same entry points serve any set of experts.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from ._lib import DSMZ_BF16, DSMZ_F32, GROUPED_ACCUMULATE, GROUPED_ZERO_REST, MAX_GROUPS, check, lib
+
+__all__ = ["grouped_matmul", "grouped_weight_grad", "adapter_forward", "adapter_backward", "device_error"]
+
+_DT = {torch.float32: DSMZ_F32, torch.bfloat16: DSMZ_BF16}
+
+
+def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """t (rows x width, bf16) as the kernels read it: unit column stride, 16-byte aligned rows.
+    Any other layout is copied to one."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise ValueError(f"{what}: CUDA tensors only (no CPU fallback)")
+    if t.dim() != 2 or t.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: operands are 2-D bfloat16 tensors")
+    if t.shape[1] < 1:
+        raise ValueError(f"{what}: an operand has no columns")
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    width = t.shape[1]
+    return t.new_empty(t.shape[0], (width + 7) // 8 * 8)[:, :width].copy_(t)
+
+
+def _weights(w: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
+    """(tensor, group stride, row pitch, whether N is the contiguous dimension) of w: G x K x N."""
+    G, K, N = w.shape
+    for nc, inner, outer in ((0, 1, 2), (1, 2, 1)):
+        if w.stride(inner) == 1 and w.stride(outer) % 8 == 0 and w.stride(outer) >= w.shape[inner] and \
+                (G == 1 or (w.stride(0) % 8 == 0 and w.stride(0) > 0)) and w.data_ptr() % 16 == 0:
+            return w, w.stride(0), w.stride(outer), nc
+    nc = 0 if w.stride(1) < w.stride(2) else 1                     # keep the faster dimension
+    inner = K if nc == 0 else N
+    pad = (inner + 7) // 8 * 8
+    c = w.new_empty(G, N if nc == 0 else K, pad)[:, :, :inner]
+    c = c.transpose(1, 2) if nc == 0 else c
+    return c.copy_(w), c.stride(0), pad, nc
+
+
+def _offsets(row_offsets: torch.Tensor, G: int, device, what: str) -> torch.Tensor:
+    if not 1 <= G <= MAX_GROUPS:
+        raise ValueError(f"{what}: 1 to {MAX_GROUPS} groups")
+    if row_offsets.dtype != torch.int32 or row_offsets.dim() != 1 or row_offsets.numel() != G + 1 or \
+            row_offsets.device != device or not row_offsets.is_contiguous():
+        raise ValueError(f"{what}: row_offsets must be a contiguous int32 vector of groups + 1 on the operands' device")
+    return row_offsets
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, row_offsets: torch.Tensor, *, out: Optional[torch.Tensor] = None,
+                   out_dtype: torch.dtype = torch.bfloat16, alpha: float = 1.0, accumulate: bool = False) -> torch.Tensor:
+    """y[i] = alpha * x[i] @ w[g] for every row i of group g, rows [row_offsets[g], row_offsets[g+1]).
+
+    x: M x K bf16. w: G x K x N bf16 with either of its last two dimensions contiguous (a stack
+    of nn.Linear weights as ``weight.transpose(1, 2)``; the same stack untransposed gives the
+    input gradient). row_offsets: G + 1 int32 on the device, ascending; values beyond [0, M]
+    or below an earlier one are clamped. out: M x N, bf16 or fp32, any row pitch; rows outside
+    every group stay as they are. Without out a new tensor of ``out_dtype`` is returned whose
+    rows outside every group are zero. accumulate: add to out (fp32 sum, rounded once)."""
+    me = "grouped_matmul"
+    x = _rows(x, me)
+    if not isinstance(w, torch.Tensor) or w.dim() != 3 or w.dtype != torch.bfloat16 or w.device != x.device:
+        raise ValueError(f"{me}: w must be a G x K x N bfloat16 tensor on x's device")
+    M, K = x.shape
+    G, Kw, N = w.shape
+    if Kw != K or N < 1:
+        raise ValueError(f"{me}: x is M x K and w is G x K x N")
+    row_offsets = _offsets(row_offsets, G, x.device, me)
+    flags = GROUPED_ACCUMULATE if accumulate else 0
+    if out is None:
+        if accumulate:
+            raise ValueError(f"{me}: accumulate needs out")
+        if out_dtype not in _DT:
+            raise TypeError(f"{me}: out_dtype must be float32 or bfloat16")
+        out = torch.empty(M, N, dtype=out_dtype, device=x.device)
+        flags |= GROUPED_ZERO_REST
+    elif tuple(out.shape) != (M, N) or out.dtype not in _DT or out.device != x.device or \
+            (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+        raise ValueError(f"{me}: out must be M x N float32 or bfloat16 with unit column stride, on x's device")
+    if M == 0:
+        return out
+    w, gs, ld, nc = _weights(w, me)
+    with torch.cuda.device(x.device):
+        check(lib().dsmz_grouped_matmul(x.data_ptr(), M, K, x.stride(0) if M > 1 else (K + 7) // 8 * 8, w.data_ptr(), G, N, gs, ld,
+                                        nc, row_offsets.data_ptr(), _DT[out.dtype], out.data_ptr(),
+                                        out.stride(0) if M > 1 else N, float(alpha), flags,
+                                        torch.cuda.current_stream(x.device).cuda_stream), me)
+    return out
+
+
+def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, row_offsets: torch.Tensor, *,
+                        out: Optional[torch.Tensor] = None, alpha: float = 1.0, accumulate: bool = False) -> torch.Tensor:
+    """dw[g] = alpha * x[rows of g].T @ dy[rows of g]: the gradient of ``grouped_matmul`` in w.
+
+    x: M x K and dy: M x N, bf16. out: G x K x N contiguous fp32 (new unless given); a group
+    without rows gives zeros. accumulate: add to out."""
+    me = "grouped_weight_grad"
+    x, dy = _rows(x, me), _rows(dy, me)
+    M, K = x.shape
+    N = dy.shape[1]
+    if dy.shape[0] != M or dy.device != x.device:
+        raise ValueError(f"{me}: x is M x K and dy is M x N, on one device")
+    G = row_offsets.numel() - 1
+    row_offsets = _offsets(row_offsets, G, x.device, me)
+    if out is None:
+        if accumulate:
+            raise ValueError(f"{me}: accumulate needs out")
+        out = torch.empty(G, K, N, dtype=torch.float32, device=x.device)
+    elif tuple(out.shape) != (G, K, N) or out.dtype != torch.float32 or out.device != x.device or not out.is_contiguous():
+        raise ValueError(f"{me}: out must be a contiguous G x K x N float32 tensor on the operands' device")
+    with torch.cuda.device(x.device):
+        check(lib().dsmz_grouped_weight_grad(x.data_ptr(), M, K, x.stride(0) if M > 1 else (K + 7) // 8 * 8, dy.data_ptr(), N,
+                                             dy.stride(0) if M > 1 else (N + 7) // 8 * 8, G, row_offsets.data_ptr(), out.data_ptr(),
+                                             float(alpha), GROUPED_ACCUMULATE if accumulate else 0,
+                                             torch.cuda.current_stream(x.device).cuda_stream), me)
+    return out
+
+
+def adapter_forward(x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, row_offsets: torch.Tensor, *,
+                    out: Optional[torch.Tensor] = None, alpha: float = 1.0,
+                    accumulate: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The adapters' share of a module's output: y[i] = alpha * (x[i] @ B[g].T) @ A[g].T.
+
+    x: M x d_in; A: G x d_out x r and B: G x r x d_in (one copy a group), all bf16. Returns
+    (y, t) with t = x @ B[g].T in bf16, which ``adapter_backward`` takes. out / accumulate: add
+    the share to a base output in place. Rows outside every group as for ``grouped_matmul``."""
+    t = grouped_matmul(x, B.transpose(1, 2), row_offsets)
+    y = grouped_matmul(t, A.transpose(1, 2), row_offsets, out=out, alpha=alpha, accumulate=accumulate)
+    return y, t
+
+
+def adapter_backward(dy: torch.Tensor, x: torch.Tensor, t: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+                     row_offsets: torch.Tensor, *, alpha: float = 1.0, dA: Optional[torch.Tensor] = None,
+                     dB: Optional[torch.Tensor] = None, accumulate: bool = False, need_dx: bool = True):
+    """Gradients of ``adapter_forward``: (dx, dA, dB) with dx bf16 (None without need_dx), dA
+    G x d_out x r and dB G x r x d_in fp32 (into the tensors given; accumulate adds to them).
+    The gradient in t is rounded to bf16, as t is."""
+    dt = grouped_matmul(dy, A, row_offsets, alpha=alpha)
+    dx = grouped_matmul(dt, B, row_offsets) if need_dx else None
+    dA = grouped_weight_grad(dy, t, row_offsets, out=dA, alpha=alpha, accumulate=accumulate)
+    dB = grouped_weight_grad(dt, x, row_offsets, out=dB, accumulate=accumulate)
+    return dx, dA, dB
+
+
+def device_error(device=None) -> int:
+    """Reads and clears the device's error word of the grouped products (synchronises the
+    current stream): nonzero when a kernel's barrier wait ran out of time."""
+    with torch.cuda.device(device):
+        return int(lib().dsmz_grouped_device_error(torch.cuda.current_stream().cuda_stream))

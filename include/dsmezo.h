@@ -368,6 +368,37 @@ int dsmz_step_update_directions(const dsmz_plan* plan, const float* dd, int32_t 
  * zeroth-order updates only).
  * ------------------------------------------------------------------------------- */
 
+/* Matrix products grouped by adapter copy (tcgen05, bf16 operands, fp32 sums). The rows of x
+ * (M x K, pitch ld_x) are sorted by group: group g owns rows [row_offsets[g],
+ * row_offsets[g+1]); row_offsets is a device array of G + 1 (the rows of the + and - copies of
+ * a scoring batch, or of a set of experts). Offsets are clamped to [0, M] and to their running
+ * maximum, so no value of theirs leads out of bounds.
+ *   y[i] = alpha x[i] W_g (+ y[i]),  W_g (K x N) with element (k, n) at
+ *     w + g * w_group_stride + n * w_ld + k   (w_n_contiguous 0: an nn.Linear weight), or
+ *     w + g * w_group_stride + k * w_ld + n   (w_n_contiguous 1; the input gradient of the
+ *                                              first with the same memory)
+ * y: BF16 or F32, pitch ld_out. Rows outside every group stay as they are, or become zero
+ * with DSMZ_GROUPED_ZERO_REST. x and w: 16-byte aligned, pitches and group stride multiples
+ * of 8 elements (K and N themselves may be any size). y must not overlap x or w.
+ * Deterministic; no workspace. */
+#define DSMZ_MAX_GROUPS 1024
+#define DSMZ_MAX_GROUPED_DIM 1073741824
+#define DSMZ_GROUPED_ACCUMULATE 1u
+#define DSMZ_GROUPED_ZERO_REST 2u
+int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const void* w, int32_t G, int64_t N,
+                        int64_t w_group_stride, int64_t w_ld, int32_t w_n_contiguous, const int32_t* row_offsets,
+                        int32_t out_dtype, void* out, int64_t ld_out, float alpha, uint32_t flags,
+                        dsmz_stream_t stream);
+/* The gradient in the weights: out[g] (K x N contiguous F32, G of them) = alpha X_g^T dY_g
+ * (+ out[g] with DSMZ_GROUPED_ACCUMULATE); a group without rows gives zeros. */
+int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, const void* dy, int64_t N, int64_t ld_dy,
+                             int32_t G, const int32_t* row_offsets, float* out, float alpha, uint32_t flags,
+                             dsmz_stream_t stream);
+/* Reads and clears the current device's error word of the grouped products (synchronises the
+ * stream): 1 when a kernel gave up on a barrier wait after its time limit, -1 when the word
+ * could not be read. */
+int32_t dsmz_grouped_device_error(dsmz_stream_t stream);
+
 /* The contrastive scoring loss (dsmz_contrastive_loss) with its gradient in the logits:
  *   loss[0] (device F32; the terms and their sum are fp64) = sum_i a_i mean_{t in i} nll_t
  *   grad[t][c] = grad_scale a_i / n_i (softmax(logits row t)[c] - [c == targets[t]])

@@ -104,3 +104,50 @@ def test_loss_grad_takes_no_cpu_tensors(lib):
     from dsmezo_b200 import scoring
     with pytest.raises(ValueError, match="CUDA"):
         scoring.contrastive_loss_grad(torch.zeros(2, 4), [2], [1.0], torch.zeros(2, dtype=torch.int32))
+
+
+def product(lib, **kw):
+    a = dict(x=1 << 20, M=10, K=16, ld_x=16, w=1 << 21, G=2, N=24, gs=384, w_ld=24, nc=1, offsets=4096, dt=1, out=1 << 22,
+             ld=24, alpha=1.0, flags=0)
+    a.update(kw)
+    return lib.lib().dsmz_grouped_matmul(a["x"], a["M"], a["K"], a["ld_x"], a["w"], a["G"], a["N"], a["gs"], a["w_ld"], a["nc"],
+                                         a["offsets"], a["dt"], a["out"], a["ld"], a["alpha"], a["flags"], None)
+
+
+@pytest.mark.parametrize("bad,code", [(dict(M=-1), 1), (dict(K=0), 1), (dict(N=0), 1), (dict(G=0), 1), (dict(G=1025), 4),
+                                      (dict(M=1 << 31), 4), (dict(dt=2), 1), (dict(flags=4), 1), (dict(x=None), 1),
+                                      (dict(w=None), 1), (dict(out=None), 1), (dict(offsets=None), 1), (dict(ld_x=8), 1),
+                                      (dict(w_ld=16), 1), (dict(ld=23), 1), (dict(gs=0), 1), (dict(gs=-8), 1),
+                                      (dict(x=(1 << 20) + 8), 1), (dict(w=(1 << 21) + 2), 1), (dict(ld_x=20), 1),
+                                      (dict(gs=388), 1), (dict(out=(1 << 22) + 1), 1), (dict(offsets=4098), 1),
+                                      (dict(alpha=float("nan")), 1), (dict(out=(1 << 20) + 16), 1),
+                                      (dict(out=(1 << 21) + 2), 1)])
+def test_grouped_matmul_refuses(lib, bad, code):
+    assert product(lib, **bad) == code
+    assert b"dsmz_grouped_matmul" in lib.lib().dsmz_last_error()
+
+
+def weight_grad(lib, **kw):
+    a = dict(x=1 << 20, M=10, K=16, ld_x=16, dy=1 << 21, N=24, ld_dy=24, G=2, offsets=4096, out=1 << 22, alpha=1.0, flags=0)
+    a.update(kw)
+    return lib.lib().dsmz_grouped_weight_grad(a["x"], a["M"], a["K"], a["ld_x"], a["dy"], a["N"], a["ld_dy"], a["G"],
+                                              a["offsets"], a["out"], a["alpha"], a["flags"], None)
+
+
+@pytest.mark.parametrize("bad,code", [(dict(M=-1), 1), (dict(K=0), 1), (dict(N=0), 1), (dict(G=0), 1), (dict(G=1025), 4),
+                                      (dict(flags=2), 1), (dict(x=None), 1), (dict(dy=None), 1), (dict(out=None), 1),
+                                      (dict(offsets=None), 1), (dict(ld_x=8), 1), (dict(ld_dy=16), 1), (dict(ld_dy=28), 1),
+                                      (dict(x=(1 << 20) + 8), 1), (dict(out=(1 << 22) + 2), 1), (dict(offsets=4097), 1),
+                                      (dict(alpha=float("inf")), 1), (dict(out=(1 << 20) + 16), 1)])
+def test_grouped_weight_grad_refuses(lib, bad, code):
+    assert weight_grad(lib, **bad) == code
+    assert b"dsmz_grouped_weight_grad" in lib.lib().dsmz_last_error()
+
+
+def test_grouped_products_take_no_cpu_tensors(lib):
+    from dsmezo_b200 import grouped
+    x, w, o = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(1, 8, 8, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        grouped.grouped_matmul(x, w, o)
+    with pytest.raises(ValueError, match="CUDA"):
+        grouped.grouped_weight_grad(x, x, o)
