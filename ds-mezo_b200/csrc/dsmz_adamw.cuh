@@ -13,12 +13,17 @@
 // takes the code 0, so a denominator never falls to eps because its block has one large
 // gradient. A value takes the lower of its two codes when it lies on their border. The codes are
 // those of 64-bit arithmetic: a warp forms its block in fp32 with a bound on every rounding
-// made, and where a value lies within that bound of a border (a block in fifteen) forms the
-// block again in fp64. All in fp64, the step of a 7B set took 1634 us: 158 instructions an
-// element and 39% of the conversion unit; in fp32 923 us. A block with a NaN or an infinity gets
+// made, decides the elements that lie within that bound of a border (one block in thirty has
+// one) in fp64, and takes the scales from the one or two elements that can be the largest,
+// formed again in fp64. The 161.5 M elements of a 7B set (bf16 gradients and shadow, 16 bytes
+// an element, 394 us at the measured copy rate) took 1634 us with everything in fp64, 1376 in
+// fp32 with blocks near a border done again whole, 634 with single elements done again, no
+// conversions, and a path without bounds for whole blocks. What bounds it is instruction
+// issue (83%): some 60 instructions an element.
+// A block with a NaN or an infinity gets
 // a scale that makes every element of the block NaN: the whole block, not one element.
 //
-// One CTA takes 2048 elements of one tensor, a warp one block of 256: its lanes own elements
+// One CTA takes a tile of one tensor, a warp one block of 256: its lanes own elements
 // 4 l .. 4 l + 3 and 128 + 4 l .. + 3, so that every access of a warp is contiguous. The pass
 // is bound by HBM: 28 to 30 bytes an element with fp32 states, 12 to 18 with 8-bit ones.
 #pragma once
@@ -32,8 +37,8 @@ namespace dsmz {
 namespace aw {
 
 constexpr int kBlock = 256;      // elements of one scale
-constexpr int kTile = 2048;      // elements of one CTA
 constexpr int kThreadsAW = 256;
+constexpr int kTile = 8 * kThreadsAW;   // elements of one CTA
 
 struct Tensor {
   void* p;                       // parameter (state_values: fp32 m out)
@@ -54,12 +59,14 @@ struct Coef {
 // Tensors of one launch, by value: a captured launch carries them, no table is uploaded.
 template <int CAP>
 struct Args {
-  double b1, omb1, b2, omb2;
+  double b1, omb1, b2, omb2;     // 1 - b formed in fp64
+  float fb1, fo1, fb2, fo2;      // the same rounded once
   float eps;
   Coef c;
   const Coef* dc;                // device coefficients (a step counter on the device), or NULL: c
   const float* grad_scale;       // device scalar, or NULL
   int32_t n;
+  int32_t tiles;                 // kTile-element tiles of one CTA
   int32_t tile0[CAP + 1];        // first CTA of each tensor
   uint8_t vec[CAP];              // every array of the tensor takes 4-element accesses
   Tensor t[CAP];
@@ -147,17 +154,26 @@ __device__ __forceinline__ void store4b(void* base, int64_t i, int nv, bool vec,
 __device__ __forceinline__ int code_i8(uint32_t u, int c) { return static_cast<int>(static_cast<int8_t>(u >> (8 * c))); }
 __device__ __forceinline__ int code_u8(uint32_t u, int c) { return static_cast<int>((u >> (8 * c)) & 0xFFu); }
 
-__device__ __forceinline__ float sqrt_approx(float x) {
+__device__ __forceinline__ float sqrt_ftz(float x) {        // relative error 2^-23; below 2^-126: 0
   float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Integer 0 <= i < 2^23 as fp32 without the conversion unit.
-__device__ __forceinline__ float small_float(int i) {
-  return __fsub_rn(__uint_as_float(0x4B000000u | static_cast<uint32_t>(i)), 8388608.f);
+__device__ __forceinline__ float rcp_ftz(float x) {         // relative error 2^-23
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-__device__ __forceinline__ float rint_small(float x) {     // |x| < 2^22
-  return __fsub_rn(__fadd_rn(x, 12582912.f), 12582912.f);
+// The low bytes of four words in one.
+__device__ __forceinline__ uint32_t pack4(const uint32_t (&c)[4]) {
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+// 2^23 + byte k of u, without the conversion unit.
+__device__ __forceinline__ float byte_float(uint32_t u, int k) {
+  return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440u + static_cast<uint32_t>(k)));
+}
+__device__ __forceinline__ float floor_small(float x) {     // 0 <= x < 2^22
+  return __fadd_rd(x, 8388608.f) - 8388608.f;
 }
 constexpr float kU = 0x1p-24f;   // half a step of fp32: one rounding
 
@@ -191,15 +207,39 @@ __device__ __forceinline__ float new_param(float p, float m, float v, const Coef
   return __fsub_rn(__fmul_rn(p, c.decay), __fmul_rn(__fdiv_rn(m, den), c.step));
 }
 
-// A block of 8-bit states in fp64, from memory (nothing of it has been stored yet): codes
-// ceil(127 sqrt(|m| / top) - 1/2) and ceil(255 sqrt(sqrt(v) / top) - 1/2), one rounding per
-// operation in the order of the formulas, so that values that lie on a border by their own
-// arithmetic (codes and bf16 gradients in small ratios do) are decided alike everywhere.
+// New m and v of one element of 8-bit states in fp64, one rounding per operation.
+__device__ __forceinline__ double mean64(int q, float scale, float g, double gs, double b1, double omb1) {
+  return __dadd_rn(__dmul_rn(__dmul_rn(static_cast<double>(q * abs(q)), static_cast<double>(scale)), b1),
+                   __dmul_rn(__dmul_rn(static_cast<double>(g), gs), omb1));
+}
+__device__ __forceinline__ double root64(int q, float scale, float g, double gs, double b2, double omb2) {
+  const double root = __dmul_rn(static_cast<double>(q * q), static_cast<double>(scale));
+  const double gg = __dmul_rn(static_cast<double>(g), gs);
+  return __dadd_rn(__dmul_rn(__dmul_rn(root, root), b2), __dmul_rn(__dmul_rn(gg, omb2), gg));
+}
+
+// Codes in fp64, one rounding per operation in the order of the formulas, so that values that
+// lie on a border by their own arithmetic (codes and bf16 gradients in small ratios do) are
+// decided alike everywhere: ceil(127 sqrt(|m| / top) - 1/2) and, with root_top = sqrt(top v),
+// ceil(255 sqrt(sqrt(v) / root_top) - 1/2).
+__device__ __forceinline__ int mean_code(double a, double top) {
+  const int q = top > 0.0 ? static_cast<int>(ceil(__dadd_rn(__dmul_rn(127.0, __dsqrt_rn(__ddiv_rn(a, top))), -0.5))) : 0;
+  return min(max(q, 0), 127);
+}
+__device__ __forceinline__ int root_code(double v, double root_top) {
+  const int q = root_top > 0.0
+                    ? static_cast<int>(ceil(__dadd_rn(__dmul_rn(255.0, __dsqrt_rn(__ddiv_rn(__dsqrt_rn(v), root_top))), -0.5)))
+                    : 0;
+  return min(max(q, v > 0.0 ? 1 : 0), 255);
+}
+
+// A block of 8-bit states in fp64, from memory (nothing of it has been stored yet): blocks
+// outside fp32's range, with NaN or infinities, or whose means cancel throughout.
 template <typename G>
 __device__ __noinline__ void exact_block(const Tensor& t, int64_t base, int lane, double b1, double omb1, double b2,
                                          double omb2, const float* grad_scale, uint32_t (&um)[2], uint32_t (&uv)[2],
                                          float& m_scale, float& v_scale) {
-  const double ms = static_cast<double>(t.ms[base / kBlock]), vs = static_cast<double>(t.vs[base / kBlock]);
+  const float ms = t.ms[base / kBlock], vs = t.vs[base / kBlock];
   const double gs = grad_scale ? static_cast<double>(*grad_scale) : 1.0;
   const int8_t* mq = reinterpret_cast<const int8_t*>(t.m);
   const uint8_t* vq = reinterpret_cast<const uint8_t*>(t.v);
@@ -209,11 +249,8 @@ __device__ __noinline__ void exact_block(const Tensor& t, int64_t base, int lane
     if (i >= t.n) return;                            // past the tensor: a NaN scale must not count there
     const float gf = sizeof(G) == 4 ? reinterpret_cast<const float*>(t.g)[i]
                                     : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(t.g)[i]);
-    const double g = __dmul_rn(static_cast<double>(gf), gs);
-    const int qm = mq[i], qv = vq[i];
-    const double root = __dmul_rn(static_cast<double>(qv * qv), vs);
-    m = __dadd_rn(__dmul_rn(__dmul_rn(static_cast<double>(qm * abs(qm)), ms), b1), __dmul_rn(g, omb1));
-    v = __dadd_rn(__dmul_rn(__dmul_rn(root, root), b2), __dmul_rn(__dmul_rn(g, omb2), g));
+    m = mean64(mq[i], ms, gf, gs, b1, omb1);
+    v = root64(vq[i], vs, gf, gs, b2, omb2);
   };
   double mt = 0.0, vt = 0.0;
 #pragma unroll 1
@@ -231,10 +268,7 @@ __device__ __noinline__ void exact_block(const Tensor& t, int64_t base, int lane
   for (int e = 0; e < 8; ++e) {
     double m, v;
     at(e, m, v);
-    int qm = mt > 0.0 ? static_cast<int>(ceil(__dadd_rn(__dmul_rn(127.0, __dsqrt_rn(__ddiv_rn(fabs(m), mt))), -0.5))) : 0;
-    int qv = rt > 0.0 ? static_cast<int>(ceil(__dadd_rn(__dmul_rn(255.0, __dsqrt_rn(__ddiv_rn(__dsqrt_rn(v), rt))), -0.5))) : 0;
-    qm = min(max(qm, 0), 127);
-    qv = min(max(qv, v > 0.0 ? 1 : 0), 255);
+    const int qm = mean_code(fabs(m), mt), qv = root_code(v, rt);
     const uint32_t cm = (static_cast<uint32_t>(m < 0.0 ? -qm : qm) & 0xFFu) << (8 * (e & 3));
     const uint32_t cv = static_cast<uint32_t>(qv) << (8 * (e & 3));
     if (e < 4) { um[0] |= cm; uv[0] |= cv; } else { um[1] |= cm; uv[1] |= cv; }
@@ -244,15 +278,10 @@ __device__ __noinline__ void exact_block(const Tensor& t, int64_t base, int lane
 }
 
 // P, G: float or __nv_bfloat16 (parameter and gradient types); BITS: 32 or 8.
-template <int CAP, typename P, typename G, int BITS>
-__global__ void __launch_bounds__(kThreadsAW) k_adamw(const __grid_constant__ Args<CAP> a) {
-  const int ti = tensor_of(a, static_cast<int>(blockIdx.x));
-  const Tensor& t = a.t[ti];
-  const int lane = threadIdx.x & 31;
-  const int64_t base = static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.tile0[ti]) * kTile +
-                       (threadIdx.x >> 5) * kBlock;
-  if (base >= t.n) return;                         // the whole warp: no element of this block exists
-  const bool vec = a.vec[ti] != 0;
+// FULL: the block lies inside the tensor and every array takes 4-element accesses.
+template <int CAP, typename P, typename G, int BITS, bool FULL>
+__device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, int64_t base, int lane, bool vec_) {
+  const bool vec = FULL ? true : vec_;
   int64_t i[2];
   int nv[2];
   float p[2][4], g[2][4];
@@ -260,15 +289,14 @@ __global__ void __launch_bounds__(kThreadsAW) k_adamw(const __grid_constant__ Ar
   for (int h = 0; h < 2; ++h) {
     i[h] = base + 128 * h + 4 * lane;
     const int64_t left = t.n - i[h];
-    nv[h] = left >= 4 ? 4 : (left > 0 ? static_cast<int>(left) : 0);
+    nv[h] = FULL || left >= 4 ? 4 : (left > 0 ? static_cast<int>(left) : 0);
     load4<P>(t.p, i[h], nv[h], vec, p[h]);
     load4<G>(t.g, i[h], nv[h], vec, g[h]);
   }
   Coef c = a.c;
   if (a.dc) c = *a.dc;
   if (BITS == 32) {
-    const float b1 = static_cast<float>(a.b1), o1 = static_cast<float>(a.omb1);
-    const float b2 = static_cast<float>(a.b2), o2 = static_cast<float>(a.omb2);
+    const float b1 = a.fb1, o1 = a.fo1, b2 = a.fb2, o2 = a.fo2;
     float m[2][4], v[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -287,6 +315,8 @@ __global__ void __launch_bounds__(kThreadsAW) k_adamw(const __grid_constant__ Ar
       }
       store4<float>(t.m, i[h], nv[h], vec, m[h]);
       store4<float>(t.v, i[h], nv[h], vec, v[h]);
+      store4<P>(t.p, i[h], nv[h], vec, p[h]);
+      if (sizeof(P) == 4 && t.shadow) store4<__nv_bfloat16>(t.shadow, i[h], nv[h], vec, p[h]);
     }
   } else {
     const int64_t blk = base / kBlock;
@@ -294,76 +324,145 @@ __global__ void __launch_bounds__(kThreadsAW) k_adamw(const __grid_constant__ Ar
     uint32_t mq[2], vq[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      mq[h] = load4b(t.m, i[h], nv[h], vec);
+      mq[h] = load4b(t.m, i[h], nv[h], vec) ^ 0x80808080u;               // q + 128
       vq[h] = load4b(t.v, i[h], nv[h], vec);
+      if (a.b2 == 0.0 || vs == 0.f) vq[h] = 0;                           // no old second moment
     }
-    const float gs = a.grad_scale ? *a.grad_scale : 1.f;
-    const float b1 = static_cast<float>(a.b1), o1 = static_cast<float>(a.omb1);
-    const float b2 = static_cast<float>(a.b2), o2 = static_cast<float>(a.omb2);
-    float m[2][4], v[2][4], e[2][4], root[2][4];
-    uint32_t mtb = 0, vtb = 0, etb = 0, positive = 0;
+    if (a.grad_scale) {
+      const float gs = *a.grad_scale;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) g[h][k] *= gs;
+    }
+    const float o1 = a.fo1, o2 = a.fo2, cm = ms * a.fb1, cv = (vs * vs) * a.fb2;
+    float m[2][4], v[2][4];
+    uint32_t mtb = 0, vtb = 0, gtb = 0, pos[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const bool in = k < nv[h];                     // past the tensor: a NaN scale must not count there
-        const float gg = __fmul_rn(g[h][k], gs);
-        const int qm = code_i8(mq[h], k), qv = code_u8(vq[h], k);
-        const float q2 = __fmul_rn(small_float(qm * qm), ms), old = __fmul_rn(small_float(qv * qv), vs);
-        const float x = __fmul_rn(qm < 0 ? -q2 : q2, b1), y = __fmul_rn(gg, o1);
-        m[h][k] = in ? __fadd_rn(x, y) : 0.f;
-        e[h][k] = in ? __fadd_rn(fabsf(x), fabsf(y)) : 0.f;      // |m|'s error is at most 4 kU e
-        v[h][k] = in ? __fadd_rn(__fmul_rn(__fmul_rn(old, old), b2), __fmul_rn(__fmul_rn(gg, o2), gg)) : 0.f;   // 6 kU
-        if ((old != 0.f && b2 != 0.f) || gg != 0.f) positive |= 1u << (4 * h + k);
-        mtb = max(mtb, __float_as_uint(fabsf(m[h][k])));         // as integers: a NaN wins
-        vtb = max(vtb, __float_as_uint(v[h][k]));
-        etb = max(etb, __float_as_uint(e[h][k]));
-        // the update itself with the one-instruction root and quotient (2 and 4 kU): its error
+        const float qm = byte_float(mq[h], k) - 8388736.f, qv = byte_float(vq[h], k) - 8388608.f;
+        const float q2 = qv * qv;
+        // |error| of the mean: at most 3 kU of the old term, 3 kU of the new, kU of the sum
+        float mm = fmaf(g[h][k], o1, (qm * fabsf(qm)) * cm);
+        float vv = fmaf(g[h][k] * g[h][k], o2, (q2 * q2) * cv);           // 6 kU
+        if (!FULL && k >= nv[h]) mm = vv = 0.f;        // past the tensor: a NaN scale must not count there
+        m[h][k] = mm;
+        v[h][k] = vv;
+        pos[h] |= (fabsf(g[h][k]) + qv > 0.f) ? 1u << (8 * k) : 0u;
+        mtb = max(mtb, __float_as_uint(fabsf(mm)));    // as integers: a NaN wins
+        vtb = max(vtb, __float_as_uint(vv));
+        gtb = max(gtb, __float_as_uint(fabsf(g[h][k])));
+        // the update itself with the one-instruction root and reciprocal (2 kU each): its error
         // is far below that of the 8-bit states it is made from
-        root[h][k] = sqrt_approx(v[h][k]);
-        p[h][k] = __fsub_rn(__fmul_rn(p[h][k], c.decay),
-                            __fmul_rn(__fdividef(m[h][k], fmaf(root[h][k], c.inv_root, a.eps)), c.step));
+        p[h][k] = fmaf(-c.step, mm * rcp_ftz(fmaf(sqrt_ftz(vv), c.inv_root, a.eps)), p[h][k] * c.decay);
       }
+      store4<P>(t.p, i[h], nv[h], vec, p[h]);
+      if (sizeof(P) == 4 && t.shadow) store4<__nv_bfloat16>(t.shadow, i[h], nv[h], vec, p[h]);
+    }
     const float mt = __uint_as_float(__reduce_max_sync(0xffffffffu, mtb));
     const float vt = __uint_as_float(__reduce_max_sync(0xffffffffu, vtb));
-    const float et = __uint_as_float(__reduce_max_sync(0xffffffffu, etb));
+    // no |old term| + |new term| of the block is above et
+    const float et = 1.0001f * fmaf(__uint_as_float(__reduce_max_sync(0xffffffffu, gtb)), o1, 16129.f * cm);
     // fp32 carries the block where its largest values are well inside the range and the means
     // do not cancel throughout; an all-zero block is exact
-    const bool mok = (mt > 0x1p-90f && mt < 0x1p100f && et <= 16.f * mt) || et == 0.f;
-    const bool vok = (vt > 0x1p-70f && vt < 0x1p100f) || (vt == 0.f && !__any_sync(0xffffffffu, positive != 0));
-    bool near = !(mok && vok);
-    const float im = mt > 0.f ? __fdividef(16129.f, mt) : 0.f, iv = vt > 0.f ? __fdividef(4228250625.f, vt) : 0.f;
-    const float ir = sqrt_approx(iv);
-    // error of y = |m| im: 4 kU e im from m, and relative 4 kU et / mt from the top, 4 kU from
-    // the quotient, its product and the top's own
-    const float ey = kU * (4.f * __fdividef(et, mt) + 6.f);
+    const bool mok = (mt > 0x1p-90f && mt < 0x1p100f && et <= 32.f * mt) || et == 0.f;
+    const bool vok = (vt > 0x1p-70f && vt < 0x1p100f && (vs == 0.f || vs > 0x1p-60f)) ||
+                     (vt == 0.f && !__any_sync(0xffffffffu, (pos[0] | pos[1]) != 0));
+    uint32_t near = 0;             // elements next to a border: bits 0-7 for m, 8-15 for v
+    const float im = mt > 0.f ? 16129.f * rcp_ftz(mt) : 0.f, iv = vt > 0.f ? 4228250625.f * rcp_ftz(vt) : 0.f;
+    const float ir = sqrt_ftz(iv);
+    // error of y = |m| im: at most 4 kU et im from m, and relative 4 kU et / mt from the top, 3 kU
+    // from the quotient, 1 from the product and 2 of second order
+    const float e0 = 4.f * kU * im * et, ey = kU * (4.f * et * rcp_ftz(mt) + 6.f);
     uint32_t um[2], uv[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      um[h] = uv[h] = 0;
+      uint32_t qm[4], qv[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        // the border (j + 1/2)^2 nearest to y = (127 sqrt(|m| / top))^2 splits codes j and j + 1
+        // y = (127 sqrt(|m| / top))^2 lies next to the border b^2, b = floor(sqrt(y)) + 1/2, which
+        // splits the codes b - 1/2 and b + 1/2
         const float y = fabsf(m[h][k]) * im;
-        const float j = fmaxf(rint_small(sqrt_approx(y) - 0.5f), 0.f);
-        const float bj = (j + 0.5f) * (j + 0.5f);                            // exact
-        near |= fabsf(y - bj) <= fmaf(4.f * kU * im, e[h][k], ey * y);
-        const int qm = min(static_cast<int>(__float_as_uint(j + 8388608.f) & 0xFFu) + (y > bj ? 1 : 0), 127);
-        // likewise (j + 1/2)^4 and (255 sqrt(sqrt(v) / top))^4: relative 6 kU for v, 6 for the
-        // top, 4 for the quotient and its product, 2 for the border
+        const float b = floor_small(sqrt_ftz(y)) + 0.5f;
+        const float d = y - b * b;                                        // b^2 is exact
+        if (fabsf(d) <= fmaf(ey, y, e0)) near |= 1u << (4 * h + k);
+        // the low byte of 1.5 2^23 + q is q's two's complement
+        qm[k] = __float_as_uint(copysignf(b + copysignf(0.5f, d), m[h][k]) + 12582912.f);
+        // likewise b^4 and z = (255 sqrt(sqrt(v) / top))^4: relative 6 kU for v, 6 for the top, 4
+        // for the quotient and its product, 2 for the border
         const float z = v[h][k] * iv;
-        const float jv = fmaxf(rint_small(sqrt_approx(root[h][k] * ir) - 0.5f), 0.f);
-        const float b2j = (jv + 0.5f) * (jv + 0.5f), b4 = b2j * b2j;
-        near |= fabsf(z - b4) <= 20.f * kU * b4;
-        int qv = min(static_cast<int>(__float_as_uint(jv + 8388608.f) & 0xFFu) + (z > b4 ? 1 : 0), 255);
-        if (qv == 0 && (positive >> (4 * h + k) & 1u)) qv = 1;
-        um[h] |= (static_cast<uint32_t>(m[h][k] < 0.f ? -qm : qm) & 0xFFu) << (8 * k);
-        uv[h] |= static_cast<uint32_t>(qv) << (8 * k);
+        const float r = floor_small(sqrt_ftz(sqrt_ftz(v[h][k]) * ir)) + 0.5f;
+        const float r4 = (r * r) * (r * r);
+        const float f = z - r4;
+        if (fabsf(f) <= 20.f * kU * r4) near |= 256u << (4 * h + k);
+        qv[k] = __float_as_uint(r + copysignf(0.5f, f) + 8388608.f);
+      }
+      um[h] = pack4(qm);
+      uv[h] = __vmaxu4(pack4(qv), pos[h]);                                // a positive v keeps a code
+    }
+    float msn = 0.f, vsn = 0.f;
+    if (!(mok && vok)) {
+      exact_block<G>(t, base, lane, a.b1, a.omb1, a.b2, a.omb2, a.grad_scale, um, uv, msn, vsn);
+    } else {
+      // The scales come from the largest values in fp64. Lanes whose largest could be it in spite
+      // of the roundings (nearly always one): their eight elements are formed again, side by side
+      // on eight lanes, lanes 0-7 for m and 8-15 for v.
+      uint32_t cand_m = __ballot_sync(0xffffffffu, __uint_as_float(mtb) >= mt - 8.f * kU * et);
+      uint32_t cand_v = __ballot_sync(0xffffffffu, __uint_as_float(vtb) >= vt * (1.f - 16.f * kU));
+      const double gs64 = a.grad_scale ? static_cast<double>(*a.grad_scale) : 1.0;
+      auto grad_at = [&](int64_t at) {
+        return sizeof(G) == 4 ? reinterpret_cast<const float*>(t.g)[at]
+                              : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(t.g)[at]);
+      };
+      auto m64_at = [&](int64_t at) {
+        return mean64(reinterpret_cast<const int8_t*>(t.m)[at], ms, grad_at(at), gs64, a.b1, a.omb1);
+      };
+      auto v64_at = [&](int64_t at) {
+        return root64(reinterpret_cast<const uint8_t*>(t.v)[at], vs, grad_at(at), gs64, a.b2, a.omb2);
+      };
+      double top64 = 0.0;
+      while ((cand_m | cand_v) != 0) {
+        const int src = __ffs(static_cast<int>((lane & 8) ? cand_v : cand_m)) - 1;
+        const int64_t at = base + 128 * ((lane >> 2) & 1) + 4 * src + (lane & 3);
+        if (src >= 0 && lane < 16 && (FULL || at < t.n)) top64 = fmax(top64, (lane & 8) ? v64_at(at) : fabs(m64_at(at)));
+        cand_m &= cand_m - 1;
+        cand_v &= cand_v - 1;
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) top64 = fmax(top64, __shfl_xor_sync(0xffffffffu, top64, o));
+      msn = static_cast<float>(top64 * (1.0 / 16129.0));                  // lanes 0-7
+      // lanes 8-15: two Newton steps take the fp32 root (2^-23) to fp64's last bits
+      const float r0 = sqrt_ftz(static_cast<float>(top64));
+      const double half = static_cast<double>(0.5f * rcp_ftz(r0));
+      double r1 = static_cast<double>(r0);
+      if (r0 > 0.f) {
+        r1 = fma(fma(-r1, r1, top64), half, r1);
+        r1 = fma(fma(-r1, r1, top64), half, r1);
+      }
+      vsn = __shfl_sync(0xffffffffu, static_cast<float>(r1 * (1.0 / 65025.0)), 8);
+      if (__any_sync(0xffffffffu, near != 0)) {
+        // codes of the elements next to a border (a block in thirty has one) from fp64
+        const double mt64 = __shfl_sync(0xffffffffu, top64, 0), vt64 = __shfl_sync(0xffffffffu, top64, 8);
+        while (near != 0) {
+          const int e = __ffs(static_cast<int>(near)) - 1, k = e & 3;
+          near &= near - 1;
+          const int64_t at = base + 128 * ((e >> 2) & 1) + 4 * lane + k;
+          uint32_t q, clear = ~(0xFFu << (8 * k));
+          if (e < 8) {
+            const double m64 = m64_at(at);
+            const int qi = mean_code(fabs(m64), mt64);
+            q = (static_cast<uint32_t>(m64 < 0.0 ? -qi : qi) & 0xFFu) << (8 * k);
+            if (e < 4) um[0] = (um[0] & clear) | q; else um[1] = (um[1] & clear) | q;
+          } else {
+            q = static_cast<uint32_t>(root_code(v64_at(at), __dsqrt_rn(vt64))) << (8 * k);
+            if (e < 12) uv[0] = (uv[0] & clear) | q; else uv[1] = (uv[1] & clear) | q;
+          }
+        }
+        __syncwarp();
       }
     }
-    float msn = __fmul_rn(mt, 1.f / 16129.f), vsn = __fmul_rn(__fsqrt_rn(vt), 1.f / 65025.f);
-    if (__any_sync(0xffffffffu, near))
-      exact_block<G>(t, base, lane, a.b1, a.omb1, a.b2, a.omb2, a.grad_scale, um, uv, msn, vsn);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       store4b(t.m, i[h], nv[h], vec, um[h]);
@@ -374,10 +473,19 @@ __global__ void __launch_bounds__(kThreadsAW) k_adamw(const __grid_constant__ Ar
       t.vs[blk] = vsn;
     }
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    store4<P>(t.p, i[h], nv[h], vec, p[h]);
-    if (sizeof(P) == 4 && t.shadow) store4<__nv_bfloat16>(t.shadow, i[h], nv[h], vec, p[h]);
+}
+
+template <int CAP, typename P, typename G, int BITS>
+__global__ void __launch_bounds__(kThreadsAW) k_adamw(const __grid_constant__ Args<CAP> a) {
+  const int ti = tensor_of(a, static_cast<int>(blockIdx.x));
+  const Tensor& t = a.t[ti];
+  const int lane = threadIdx.x & 31;
+  const bool vec = a.vec[ti] != 0;
+  int64_t base = (static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.tile0[ti]) * a.tiles) * kTile +
+                 (threadIdx.x >> 5) * kBlock;
+  for (int j = 0; j < a.tiles && base < t.n; ++j, base += kTile) {     // uniform in the warp
+    if (vec && base + kBlock <= t.n) step_block<CAP, P, G, BITS, true>(a, t, base, lane, true);
+    else step_block<CAP, P, G, BITS, false>(a, t, base, lane, vec);
   }
 }
 
@@ -387,27 +495,28 @@ __global__ void __launch_bounds__(kThreadsAW) k_adamw_values(const __grid_consta
   const int ti = tensor_of(a, static_cast<int>(blockIdx.x));
   const Tensor& t = a.t[ti];
   const int lane = threadIdx.x & 31;
-  const int64_t base = static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.tile0[ti]) * kTile +
-                       (threadIdx.x >> 5) * kBlock;
-  if (base >= t.n) return;
   const bool vec = a.vec[ti] != 0;
-  const double ms = static_cast<double>(t.ms[base / kBlock]), vs = static_cast<double>(t.vs[base / kBlock]);
+  int64_t base = (static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.tile0[ti]) * a.tiles) * kTile +
+                 (threadIdx.x >> 5) * kBlock;
+  for (int j = 0; j < a.tiles && base < t.n; ++j, base += kTile) {
+    const double ms = static_cast<double>(t.ms[base / kBlock]), vs = static_cast<double>(t.vs[base / kBlock]);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t i = base + 128 * h + 4 * lane;
-    const int64_t left = t.n - i;
-    const int nv = left >= 4 ? 4 : (left > 0 ? static_cast<int>(left) : 0);
-    const uint32_t um = load4b(t.m, i, nv, vec), uv = load4b(t.v, i, nv, vec);
-    float m[4], v[4];
+    for (int h = 0; h < 2; ++h) {
+      const int64_t i = base + 128 * h + 4 * lane;
+      const int64_t left = t.n - i;
+      const int nv = left >= 4 ? 4 : (left > 0 ? static_cast<int>(left) : 0);
+      const uint32_t um = load4b(t.m, i, nv, vec), uv = load4b(t.v, i, nv, vec);
+      float m[4], v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int qm = code_i8(um, k), qv = code_u8(uv, k);
-      const double root = static_cast<double>(qv * qv) * vs;
-      m[k] = static_cast<float>(static_cast<double>(qm * abs(qm)) * ms);
-      v[k] = static_cast<float>(root * root);
+      for (int k = 0; k < 4; ++k) {
+        const int qm = code_i8(um, k), qv = code_u8(uv, k);
+        const double root = static_cast<double>(qv * qv) * vs;
+        m[k] = static_cast<float>(static_cast<double>(qm * abs(qm)) * ms);
+        v[k] = static_cast<float>(root * root);
+      }
+      store4<float>(t.p, i, nv, vec, m);
+      store4<float>(t.shadow, i, nv, vec, v);
     }
-    store4<float>(t.p, i, nv, vec, m);
-    store4<float>(t.shadow, i, nv, vec, v);
   }
 }
 

@@ -38,6 +38,10 @@ bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 // Tensors per launch: the argument block (by value) of the small form is 0.6 KB, so that a
 // call on a few tensors does not pay for copying the large one (18 KB).
 constexpr int kSmall = 8, kLarge = 256;
+// Reading states back takes four tiles a CTA where that still fills the machine four times over
+// (289 -> 267 us for a 7B set: a tile is short against finding its tensor in the arguments).
+// The step does not: a second tile's loads would wait for the first (8-bit 634 -> 784 us).
+constexpr int64_t kManyTiles = 148 * 4 * 4;
 
 template <int CAP>
 void launch_adamw(const aw::Args<CAP>& a, int grid, int pdt, int gdt, int bits, cudaStream_t s) {
@@ -58,19 +62,23 @@ void launch_adamw(const aw::Args<CAP>& a, int grid, int pdt, int gdt, int bits, 
 
 // Launches over tensors[0..n): as many per launch as CAP and the grid limit allow.
 template <int CAP, typename Fill, typename Launch>
-int chunked(const dsmz_adamw_tensor* tensors, int32_t n, const char* what, Fill fill, Launch launch) {
+int chunked(const dsmz_adamw_tensor* tensors, int32_t n, int tiles_max, const char* what, Fill fill, Launch launch) {
   auto box = std::vector<aw::Args<CAP>>(1);
   aw::Args<CAP>& a = box[0];
+  int64_t all = 0;
+  for (int32_t k = 0; k < n; ++k) all += (tensors[k].n + aw::kTile - 1) / aw::kTile;
+  a.tiles = all >= tiles_max * kManyTiles ? tiles_max : 1;
+  const int64_t per = static_cast<int64_t>(a.tiles) * aw::kTile;
   int32_t i = 0;
   while (i < n) {
     a.n = 0;
     int64_t tiles = 0;
     for (; i < n && a.n < CAP; ++i) {
       if (tensors[i].n == 0) continue;
-      const int64_t nt = (tensors[i].n + aw::kTile - 1) / aw::kTile;
+      const int64_t nt = (tensors[i].n + per - 1) / per;
       if (tiles + nt > 0x7fffffff) {
         if (a.n > 0) break;
-        return fail(DSMZ_ERR_UNSUPPORTED, std::string(what) + ": a tensor of more than 2^42 elements");
+        return fail(DSMZ_ERR_UNSUPPORTED, std::string(what) + ": a tensor with too many elements");
       }
       fill(a, a.n, tensors[i]);
       a.tile0[a.n] = static_cast<int32_t>(tiles);
@@ -108,7 +116,7 @@ int check_tensors(const char* what, const dsmz_adamw_tensor* t, int32_t n, int b
 template <int CAP>
 int adamw_values(const dsmz_adamw_tensor* tensors, int32_t n, cudaStream_t s) {
   return chunked<CAP>(
-      tensors, n, "dsmz_adamw_state_values",
+      tensors, n, 4, "dsmz_adamw_state_values",
       [](aw::Args<CAP>& a, int k, const dsmz_adamw_tensor& t) {
         a.t[k] = aw::Tensor{t.param, nullptr, t.m, t.v, t.m_scale, t.v_scale, t.shadow, t.n};
         a.vec[k] = aligned(t.param, 16) && aligned(t.shadow, 16) && aligned(t.m, 4) && aligned(t.v, 4);
@@ -122,10 +130,12 @@ int adamw_run(const dsmz_adamw_desc& d, const dsmz_adamw_tensor* tensors, int32_
   const size_t pa = d.param_dtype == DSMZ_F32 ? 16 : 8, ga = d.grad_dtype == DSMZ_F32 ? 16 : 8;
   const size_t sa = d.state_bits == 32 ? 16 : 4;
   return chunked<CAP>(
-      tensors, n, "dsmz_adamw_step",
+      tensors, n, 1, "dsmz_adamw_step",
       [&](aw::Args<CAP>& a, int k, const dsmz_adamw_tensor& t) {
         a.b1 = d.beta1; a.omb1 = 1.0 - d.beta1;
         a.b2 = d.beta2; a.omb2 = 1.0 - d.beta2;
+        a.fb1 = static_cast<float>(a.b1); a.fo1 = static_cast<float>(a.omb1);
+        a.fb2 = static_cast<float>(a.b2); a.fo2 = static_cast<float>(a.omb2);
         a.eps = static_cast<float>(d.eps);
         a.c = c;
         a.dc = dc;
@@ -461,6 +471,8 @@ int dsmz_adamw_step(const dsmz_adamw_desc* desc, const dsmz_adamw_tensor* tensor
     if (!(d.beta1 >= 0.0 && d.beta1 < 1.0 && d.beta2 >= 0.0 && d.beta2 < 1.0) || !(d.eps >= 0.0) || !(d.weight_decay >= 0.0) ||
         !std::isfinite(d.eps) || !std::isfinite(d.weight_decay) || (!d.lr_device && !std::isfinite(d.lr)))
       return fail(DSMZ_ERR_INVALID, "dsmz_adamw_step: need 0 <= beta < 1, eps >= 0, weight_decay >= 0 and a finite lr");
+    if (d.state_bits == 8 && d.eps < 1e-12)
+      return fail(DSMZ_ERR_INVALID, "dsmz_adamw_step: 8-bit states need eps >= 1e-12 (their denominators drop v below 2^-126)");
     if (!d.step_counter && d.step < 1) return fail(DSMZ_ERR_INVALID, "dsmz_adamw_step: steps count from 1");
     int rc = check_tensors("dsmz_adamw_step", tensors, n, d.state_bits, false, d.param_dtype, d.grad_dtype);
     if (rc) return rc;

@@ -86,12 +86,15 @@ class AdamW:
         if int(step) < 0:
             raise ValueError("AdamW: step counts from 0")
         n = len(self.params)
+        self._numels = [p.numel() for p in self.params]
         self.device, self.lr, self.betas = p0.device, float(lr), (b1, b2)
         self.eps, self.weight_decay = float(eps), float(weight_decay)
         self.states = [AdamWState.zeros(p, state_bits) for p in self.params] if states is None else list(states)
         if len(self.states) != n:
             raise ValueError("AdamW: one state a parameter")
         self.state_bits = self.states[0].bits
+        if self.state_bits == 8 and self.eps < 1e-12:
+            raise ValueError("AdamW: 8-bit states need eps >= 1e-12")
         for p, s in zip(self.params, self.states):
             self._check_state(p, s)
         self.shadows = [None] * n if shadows is None else list(shadows)
@@ -204,13 +207,13 @@ class AdamW:
         n = len(self.params)
         if len(m_out) != n or len(v_out) != n:
             raise ValueError("AdamW: one output a parameter")
-        table = (AdamWTensor * n)()
-        for e, b, a, v in zip(table, self._table, m_out, v_out):
-            for t in (a, v):
-                if t.dtype != torch.float32 or t.numel() != b.n or t.device != self.device or not t.is_contiguous():
-                    raise ValueError("AdamW: state values go to contiguous float32 tensors of the parameters' sizes")
-            e.param, e.shadow, e.m, e.v, e.m_scale, e.v_scale, e.n = (a.data_ptr(), v.data_ptr(), b.m, b.v, b.m_scale,
-                                                                      b.v_scale, b.n)
+        for outs in (m_out, v_out):
+            if [t.numel() for t in outs] != self._numels or any(
+                    t.dtype != torch.float32 or t.device != self.device or not t.is_contiguous() for t in outs):
+                raise ValueError("AdamW: state values go to contiguous float32 tensors of the parameters' sizes")
+        table = type(self._table).from_buffer_copy(self._table)
+        for e, a, v in zip(table, m_out, v_out):
+            e.param, e.shadow = a.data_ptr(), v.data_ptr()
         with torch.cuda.device(self.device):
             check(lib().dsmz_adamw_state_values(table, n, torch.cuda.current_stream(self.device).cuda_stream),
                   "adamw_state_values")

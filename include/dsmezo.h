@@ -422,7 +422,7 @@ int dsmz_contrastive_loss_grad(int32_t kind, const void* logits, int64_t V, int6
  * (ceil(n / DSMZ_ADAMW_BLOCK) of them): m = sign q^2 m_scale with |q| <= 127, sqrt(v) = q^2
  * v_scale with q <= 255; a positive v never takes code 0, a value on the border of two codes
  * takes the lower, and the codes are those of 64-bit arithmetic. A block that meets a NaN or
- * an infinity becomes NaN as a whole. Zeroed codes and scales are the state before step 1.
+ * an infinity becomes NaN as a whole; eps must be at least 1e-12. Zeroed codes and scales are the state before step 1.
  * shadow: bf16 image of the updated fp32 parameter, rounded once (NULL: none).
  * Tensors are contiguous; those of one call must not overlap. */
 #define DSMZ_ADAMW_BLOCK 256
