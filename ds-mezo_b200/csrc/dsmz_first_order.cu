@@ -151,15 +151,16 @@ int adamw_run(const dsmz_adamw_desc& d, const dsmz_adamw_tensor* tensors, int32_
 // Error word of the grouped products' bounded waits, one per device.
 __device__ int g_grouped_err;
 
-// bf16 tensor map of rank 2 or 3 (inner dimension contiguous, byte strides of the others),
-// 128-byte swizzle, zero fill outside.
-bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
-                 uint32_t box0, uint32_t box1) {
+// Tensor map of rank 2 or 3 (inner dimension contiguous, byte strides of the others), 128-byte
+// swizzle, zero fill outside; bf16, or fp32.
+bool encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                uint32_t box0, uint32_t box1, bool f32 = false) {
   auto fn = encode_fn();
   if (!fn) return false;
   cuuint64_t d[3] = {dims[0], dims[1], rank == 3 ? dims[2] : 1}, st[2] = {strides[0], rank == 3 ? strides[1] : 0};
   cuuint32_t box[3] = {box0, box1, 1}, es[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, box, es,
+  return fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
+            const_cast<void*>(base), d, st, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -172,11 +173,11 @@ int sm_count(int* sms) {
 }
 
 template <int BNT, int MODE>
-int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, int64_t tiles, int sms, const char* what,
+int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, int64_t tiles, int sms, const char* what,
                    cudaStream_t s) {
   constexpr int SB = gr::kABytes + BNT * gr::kBK * 2;
   constexpr int kSmem = 227 * 1024;
-  const int scratch = a.split > 1 ? gr::kBM * (BNT + 4) * 4 : gr::kEpiWarps * 32 * gr::kStagePitch;
+  const int scratch = a.split > 1 ? gr::kBM * BNT * 4 : gr::kEpiWarps * gr::kStageBytes;
   const int fixed = 1024 + scratch + (((a.G + 3) * 8 + 15) & ~15) + 64 + 16 * 8;
   a.stages = (kSmem - fixed) / SB;
   if (a.stages > 8) a.stages = 8;
@@ -206,16 +207,16 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, int64
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = a.split > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, A, B, a, err);
+  e = cudaLaunchKernelEx(&cfg, kernel, A, B, C, a, err);
   return e == cudaSuccess ? DSMZ_OK : cuda_fail(what, e);
 }
 
 template <int MODE>
-int launch_grouped_bn(int bnt, const gr::Args& a, const CUtensorMap& A, const CUtensorMap& B, int64_t tiles, int sms,
-                      const char* what, cudaStream_t s) {
-  if (bnt == 64) return launch_grouped<64, MODE>(a, A, B, tiles, sms, what, s);
-  if (bnt == 128) return launch_grouped<128, MODE>(a, A, B, tiles, sms, what, s);
-  return launch_grouped<256, MODE>(a, A, B, tiles, sms, what, s);
+int launch_grouped_bn(int bnt, const gr::Args& a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C,
+                      int64_t tiles, int sms, const char* what, cudaStream_t s) {
+  if (bnt == 64) return launch_grouped<64, MODE>(a, A, B, C, tiles, sms, what, s);
+  if (bnt == 128) return launch_grouped<128, MODE>(a, A, B, C, tiles, sms, what, s);
+  return launch_grouped<256, MODE>(a, A, B, C, tiles, sms, what, s);
 }
 
 // Accumulator width for n output columns and `rows` row tiles: 256 columns where that still
@@ -310,6 +311,7 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     a.ndim = static_cast<int32_t>(N);
     a.kdim = static_cast<int32_t>(K);
     a.b_mn = w_n_contiguous ? 1 : 0;
+    a.n_inner = K <= 256 ? 1 : 0;
     a.out = out;
     a.ld = ld_out;
     a.out_f32 = out_dtype == DSMZ_F32;
@@ -327,15 +329,20 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     a.arows = M / G >= 96 ? gr::kBM : 32;
     const int64_t tiles = (rows + 2) * a.ntn;                                    // and the rows outside the groups
     if (tiles > (1 << 27)) return fail(DSMZ_ERR_UNSUPPORTED, me + "too many tiles");
-    CUtensorMap A, B;
+    CUtensorMap A, B, C{};
     const uint64_t da[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(M)}, sa[1] = {static_cast<uint64_t>(ld_x) * 2};
     const uint64_t db[3] = {static_cast<uint64_t>(wi), static_cast<uint64_t>(wo), static_cast<uint64_t>(G)};
     const uint64_t sb[2] = {static_cast<uint64_t>(w_ld) * 2,
                             static_cast<uint64_t>(G > 1 ? w_group_stride : (w_ld * wo + 7) / 8 * 8) * 2};
-    if (!encode_bf16(&A, x, 2, da, sa, gr::kBK, static_cast<uint32_t>(a.arows)) ||
-        !encode_bf16(&B, w, 3, db, sb, 64, w_n_contiguous ? 64 : static_cast<uint32_t>(a.bn)))
+    if (!encode_map(&A, x, 2, da, sa, gr::kBK, static_cast<uint32_t>(a.arows)) ||
+        !encode_map(&B, w, 3, db, sb, 64, w_n_contiguous ? 64 : static_cast<uint32_t>(a.bn)))
       return fail(DSMZ_ERR_CUDA, me + "the driver refused a tensor map");
-    return launch_grouped_bn<0>(bnt, a, A, B, tiles, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
+    if (a.vec && !a.accumulate && a.split == 1) {
+      const uint64_t dc[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M), 1};
+      const uint64_t sc[2] = {static_cast<uint64_t>(ld_out) * es, static_cast<uint64_t>(ld_out) * es * M};
+      a.tma_out = encode_map(&C, out, 3, dc, sc, 128 / es, 32, a.out_f32 != 0);
+    }
+    return launch_grouped_bn<0>(bnt, a, A, B, C, tiles, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -390,12 +397,17 @@ int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, 
     const int64_t tiles = static_cast<int64_t>(G) * a.mtn * a.ntn;
     if (tiles > (1 << 27)) return fail(DSMZ_ERR_UNSUPPORTED, me + "too many tiles");
     a.split = split_for(bnt, tiles, (M / G + gr::kBK - 1) / gr::kBK, sms);
-    CUtensorMap A, B;
+    CUtensorMap A, B, C{};
     const uint64_t dx[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(M)}, sx[1] = {static_cast<uint64_t>(ld_x) * 2};
     const uint64_t dd[2] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M)}, sd[1] = {static_cast<uint64_t>(ld_dy) * 2};
-    if (!encode_bf16(xw ? &A : &B, x, 2, dx, sx, 64, 64) || !encode_bf16(xw ? &B : &A, dy, 2, dd, sd, 64, 64))
+    if (!encode_map(xw ? &A : &B, x, 2, dx, sx, 64, 64) || !encode_map(xw ? &B : &A, dy, 2, dd, sd, 64, 64))
       return fail(DSMZ_ERR_CUDA, me + "the driver refused a tensor map");
-    return launch_grouped_bn<1>(bnt, a, A, B, tiles, sms, "dsmz_grouped_weight_grad", s);
+    if (a.vec && !a.accumulate && !a.transposed && a.split == 1) {
+      const uint64_t dc[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(K), static_cast<uint64_t>(G)};
+      const uint64_t sc[2] = {static_cast<uint64_t>(N) * 4, static_cast<uint64_t>(K) * N * 4};
+      a.tma_out = encode_map(&C, out, 3, dc, sc, 32, 32, true);
+    }
+    return launch_grouped_bn<1>(bnt, a, A, B, C, tiles, sms, "dsmz_grouped_weight_grad", s);
   });
 }
 

@@ -9,10 +9,14 @@
 // outside every group are left as they were, or zeroed where the caller asks.
 //
 // A tile is 128 x BN: MODE 0 128 rows of one group, MODE 1 128 features of the wider operand.
-// Ten warps:
-//   warp 0     TMA producer (one lane): 64-wide k-steps of A and B into a ring of stages
-//   warp 1     TMEM owner and MMA issuer (kind::f16, M = 128, N = BN), two accumulators
-//   warps 2-9  epilogue: TMEM -> registers -> (staged, coalesced) stores
+// Twelve warps:
+//   warps 0, 2   TMA producers of A and of B (one lane each; issuing a copy costs a thread
+//                some 150 cycles, so one producer for both held the loop at 450): 64-wide
+//                k-steps into a ring of stages; warp 2 scans the offsets first
+//   warp 1       TMEM owner and MMA issuer (one lane; kind::f16, M = 128, N = BN), two
+//                accumulators
+//   warps 4-11   epilogue: TMEM -> registers -> shared memory -> TMA stores (whole 32-row
+//                pieces of a group) or masked, coalesced stores (its last rows, accumulation)
 // A tile that reaches past its group reads the neighbour's rows: harmless in MODE 0 (each
 // output row depends on its own input row; rows past the group are not stored), and cleared
 // in shared memory before the last k-step's MMAs in MODE 1, where they would be summed.
@@ -23,8 +27,8 @@
 // the value) do not need it.
 //
 // Few tiles (narrow outputs): a cluster of 2, 4 or 8 CTAs splits the contraction; each CTA
-// sends its partial tile to the CTA that owns the rows through distributed shared memory, and
-// the owner adds the partials in rank order. No atomics: results are the same on every run.
+// sends its partial tile to the CTA that owns the rows (st.async into its shared memory, which
+// counts the bytes on its barrier), and the owner adds the partials in rank order. No atomics: results are the same on every run.
 //
 // Every mbarrier wait gives up after ~1 s, sets the error word, and lets each role finish its
 // own copies before the CTA frees its TMEM.
@@ -45,9 +49,11 @@ using tc::kBM;
 
 constexpr int kMaxGroups = 1024;
 constexpr int kEpiWarps = 8;
-constexpr int kThreadsG = 64 + 32 * kEpiWarps;
+constexpr int kFirstEpi = 4;            // first epilogue warp (a multiple of 4: warp % 4 is the TMEM lane quadrant)
+constexpr int kThreadsG = 32 * (kFirstEpi + kEpiWarps);
 constexpr int kChunk = 8;               // k-steps (512 products) an accumulator takes for fp32 outputs
 constexpr int kStagePitch = 80;         // bytes of a staged 64-byte row piece (conflict-free 16-byte accesses)
+constexpr int kStageBytes = 4096;       // staging of an epilogue warp: 32 rows of 128 bytes
 constexpr int kABytes = kBM * kBK * 2;
 
 struct Args {
@@ -58,6 +64,7 @@ struct Args {
   int32_t bn;                           // MMA N (multiple of 16) = columns of a tile
   int32_t ntn, mtn;                     // column tiles; MODE 1: feature tiles
   int32_t b_mn;                         // MODE 0: W is contiguous along N
+  int32_t n_inner;                      // MODE 0: concurrent tiles run along the columns, not the rows
   int32_t arows;                        // MODE 0: rows of an A box
   int32_t stages, split;
   int32_t chunk;                        // k-steps per accumulator
@@ -65,6 +72,7 @@ struct Args {
   int64_t ld, gstride;                  // output pitch; MODE 1: elements between groups
   int32_t transposed;                   // MODE 1: element (m, n) at n * ld + m
   int32_t out_f32, accumulate, zero_rest, vec;
+  int32_t tma_out;                      // mapC is valid: whole pieces leave by TMA
   float alpha;
 };
 
@@ -93,20 +101,35 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, int
       "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+// 32 rows of 128 swizzled bytes from shared memory to (x, y, z) of a 3-D tensor map.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];\n cp.async.bulk.commit_group;" ::"l"(m),
+               "r"(x), "r"(y), "r"(z), "r"(smem_u32(src))
+               : "memory");
 }
+__device__ __forceinline__ void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void st_remote(uint32_t addr, float4 v) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+// 16 bytes to another CTA's shared memory, counted on that CTA's barrier when they land.
+__device__ __forceinline__ void st_async(uint32_t addr, uint32_t bar, float4 v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "f"(v.x),
+               "f"(v.y), "f"(v.z), "f"(v.w), "r"(bar)
                : "memory");
 }
-__device__ __forceinline__ void arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
 }
 // Bounded wait with cluster-scope acquire (arrivals come from other CTAs).
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
@@ -189,7 +212,8 @@ __device__ __forceinline__ Tile tile_of(const Args& a, const int32_t* bnd, const
     }
     const int nm = tile0[lo + 1] - tile0[lo];
     const int local = t - tile0[lo] * a.ntn;
-    const int nt = local / nm, mt = local - nt * nm;   // rows first: concurrent tiles share W's columns
+    int nt, mt;
+    if (a.n_inner) { mt = local / a.ntn; nt = local - mt * a.ntn; } else { nt = local / nm; mt = local - nt * nm; }
     x.seg = lo;
     x.m0 = bnd[lo] + mt * kBM;
     x.n0 = nt * a.bn;
@@ -253,25 +277,28 @@ __device__ __forceinline__ void put1(const Args& a, char* base, int64_t i, float
   }
 }
 
-// BNT: columns of the accumulators (64, 128 or 256; a.bn <= BNT).
+// BNT: columns of the accumulators (64, 128 or 256; a.bn <= BNT). mapC: the output (3-D, boxes
+// of 32 rows x 128 bytes) where a.tma_out.
 template <int BNT, int MODE>
 __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant__ CUtensorMap mapA,
                                                          const __grid_constant__ CUtensorMap mapB,
+                                                         const __grid_constant__ CUtensorMap mapC,
                                                          const __grid_constant__ Args a, int* err) {
-  constexpr int CPW = BNT / 2;          // columns of an epilogue warp
+  // columns of an epilogue warp: half a tile, or all of a narrow one (whole 128-byte bf16 rows)
+  constexpr int CPW = BNT == 64 ? 64 : BNT / 2;
   constexpr int SB = kABytes + BNT * kBK * 2;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int S = a.split;
-  unsigned char* scratch = smem + a.stages * SB;
+  const int S = a.split, stages = a.stages;
+  unsigned char* scratch = smem + stages * SB;
   // split: partial tiles of the S CTAs for this CTA's rows; else: the epilogue's staging
-  const int scratch_bytes = S > 1 ? kBM * (BNT + 4) * 4 : kEpiWarps * 32 * kStagePitch;
+  const int scratch_bytes = S > 1 ? kBM * BNT * 4 : kEpiWarps * kStageBytes;
   int32_t* bnd = reinterpret_cast<int32_t*>(scratch + scratch_bytes);
   int32_t* tile0 = bnd + a.G + 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(
       reinterpret_cast<unsigned char*>(tile0) + (((a.G + 3) * 8 + 15) & ~15) - (a.G + 3) * 4);
-  uint64_t* empty = full + a.stages;
-  uint64_t* tfull = empty + a.stages;   // [2]
+  uint64_t* empty = full + stages;
+  uint64_t* tfull = empty + stages;     // [2]
   uint64_t* tempty = tfull + 2;         // [2]
   uint64_t* red_full = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_full + 1);
@@ -280,73 +307,93 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
   const int rank = S > 1 ? static_cast<int>(blockIdx.x) % S : 0;
   const int first = static_cast<int>(blockIdx.x) / S, step = static_cast<int>(gridDim.x) / S;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, kEpiWarps); }
-    const int rows = kBM / S;
-    mbar_init(red_full, static_cast<uint32_t>(S * 2 * (rows >= 32 ? rows / 32 : 1)));
-    mbar_init_fence();
-  }
-  if (warp == 1) {
+  if (warp == 2) {
+    scan_groups(a.offsets, a.G, static_cast<int>(a.M), a.zero_rest != 0, bnd, tile0, lane);
+  } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (warp == 0 && lane == 0) {
+    for (int s = 0; s < stages; ++s) { mbar_init(full + s, 2); mbar_init(empty + s, 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, kEpiWarps); }
+    mbar_init(red_full, 1);
+    mbar_init_fence();
+    // the partial tiles of this CTA's rows: a.bn columns from each of the S CTAs
+    if (S > 1) mbar_expect_tx(red_full, static_cast<uint32_t>(kBM * a.bn * 4));
+  } else if (warp == 3 && lane == 0) {
+    prefetch_map(&mapA);
+    prefetch_map(&mapB);
+    if (a.tma_out) prefetch_map(&mapC);
   }
-  if (warp == 2) scan_groups(a.offsets, a.G, static_cast<int>(a.M), a.zero_rest != 0, bnd, tile0, lane);
+  __syncwarp();
   tc::tc_fence_before();
-  if (S > 1) cluster_sync_all(); else __syncthreads();
+  if (S > 1) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int total = MODE == 0 ? tile0[a.G + 2] * a.ntn : a.G * a.mtn * a.ntn;
-  const int nbox_b = a.b_mn || MODE == 1 ? (a.bn + 63) / 64 : 1;
-  const uint32_t b_bytes = a.b_mn || MODE == 1 ? static_cast<uint32_t>(nbox_b * 8192) : static_cast<uint32_t>(a.bn * 128);
-  auto k_begin = [&](int nk) { return static_cast<int>(static_cast<int64_t>(nk) * rank / S); };
-  auto k_end = [&](int nk) { return static_cast<int>(static_cast<int64_t>(nk) * (rank + 1) / S); };
+  const bool b_mn = MODE == 1 || a.b_mn != 0;
+  const int nbox_b = b_mn ? (a.bn + 63) / 64 : 1;
+  auto k_begin = [&](int nk) { return S == 1 ? 0 : nk * rank / S; };
+  auto k_end = [&](int nk) { return S == 1 ? nk : nk * (rank + 1) / S; };
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {
     if (lane == 0) {
-      int g = 0;                        // k-steps issued (position in the ring)
+      const bool is_a = warp == 0;
+      int s = 0, n = 0;                 // stage, k-steps issued
+      uint32_t ph = 1;                  // parity of the wait for an empty stage (the first round passes)
       bool ok = true;
       for (int t = first; t < total && ok; t += step) {
         const Tile x = tile_of<MODE>(a, bnd, tile0, t);
         const int nba = MODE == 0 ? (x.valid + a.arows - 1) / a.arows : 2;
-        const uint32_t bytes = b_bytes + (MODE == 0 ? static_cast<uint32_t>(nba * a.arows * 128) : 16384u);
-        for (int k = k_begin(x.nk); k < k_end(x.nk); ++k) {
-          const int s = g % a.stages;
-          const uint32_t u = static_cast<uint32_t>(g / a.stages);
-          if (g >= a.stages && !mbar_wait(empty + s, (u & 1u) ^ 1u, err)) { ok = false; break; }
-          unsigned char* As = smem + s * SB;
-          unsigned char* Bs = As + kABytes;
+        const uint32_t bytes = !is_a ? (b_mn ? static_cast<uint32_t>(nbox_b * 8192) : static_cast<uint32_t>(a.bn * 128))
+                                     : (MODE == 0 ? static_cast<uint32_t>(nba * a.arows * 128) : 16384u);
+        const int ke = k_end(x.nk);
+        for (int k = k_begin(x.nk); k < ke; ++k) {
+          if (!mbar_wait(empty + s, ph, err)) { ok = false; break; }
+          unsigned char* dst = smem + s * SB + (is_a ? 0 : kABytes);
           mbar_expect_tx(full + s, bytes);
           if (MODE == 0) {
-            for (int i = 0; i < nba; ++i)
-              tma_load_2d(As + i * a.arows * 128, &mapA, k * kBK, x.m0 + i * a.arows, full + s);
-            if (a.b_mn) {
-              for (int j = 0; j < nbox_b; ++j) tma_load_3d(Bs + j * 8192, &mapB, x.n0 + 64 * j, k * kBK, x.seg - 1, full + s);
+            if (is_a) {
+              for (int i = 0; i < nba; ++i)
+                tma_load_2d(dst + i * a.arows * 128, &mapA, k * kBK, x.m0 + i * a.arows, full + s);
+            } else if (b_mn) {
+              for (int j = 0; j < nbox_b; ++j) tma_load_3d(dst + j * 8192, &mapB, x.n0 + 64 * j, k * kBK, x.seg - 1, full + s);
             } else {
-              tma_load_3d(Bs, &mapB, k * kBK, x.n0, x.seg - 1, full + s);
+              tma_load_3d(dst, &mapB, k * kBK, x.n0, x.seg - 1, full + s);
             }
           } else {
             const int r = x.r0 + k * kBK;
-            tma_load_2d(As, &mapA, x.m0, r, full + s);
-            tma_load_2d(As + 8192, &mapA, x.m0 + 64, r, full + s);
-            for (int j = 0; j < nbox_b; ++j) tma_load_2d(Bs + j * 8192, &mapB, x.n0 + 64 * j, r, full + s);
+            if (is_a) {
+              tma_load_2d(dst, &mapA, x.m0, r, full + s);
+              tma_load_2d(dst + 8192, &mapA, x.m0 + 64, r, full + s);
+            } else {
+              for (int j = 0; j < nbox_b; ++j) tma_load_2d(dst + j * 8192, &mapB, x.n0 + 64 * j, r, full + s);
+            }
           }
-          ++g;
+          ++n;
+          if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }
+      // on an error: let the loads already issued land before the CTA can exit
       if (!ok)
-        for (int i = (g > a.stages ? g - a.stages : 0); i < g; ++i)
-          mbar_drain(full + (i % a.stages), static_cast<uint32_t>(i / a.stages) & 1u);
+        for (int i = (n > stages ? n - stages : 0); i < n; ++i)
+          mbar_drain(full + (i % stages), static_cast<uint32_t>(i / stages) & 1u);
     }
   } else if (warp == 1) {
-    const uint32_t idesc = tc::idesc_bf16(a.bn, MODE, MODE == 1 ? 1 : a.b_mn);
-    int g = 0, u = 0;                   // k-steps consumed, accumulators begun
+    // The whole warp walks the loop, with every branch on a vote or a broadcast, so that stages
+    // and descriptors stay in uniform registers; one elected lane issues.
+    const uint32_t idesc = tc::idesc_bf16(a.bn, MODE, b_mn ? 1 : 0);
+    // descriptors of stage 0; addresses advance in units of 16 bytes
+    const uint64_t a0 = MODE == 0 ? tc::sdesc(smem_u32(smem), 16, 1024) : tc::sdesc(smem_u32(smem), 8192, 1024);
+    const uint64_t b0 = b_mn ? tc::sdesc(smem_u32(smem) + kABytes, 8192, 1024) : tc::sdesc(smem_u32(smem) + kABytes, 16, 1024);
+    const uint32_t ka = MODE == 0 ? 2 : 128, kb_ = b_mn ? 128 : 2;        // a 16-wide slice of the k-step
+    int s = 0, u = 0, last = -1;        // stage, accumulators begun, the last one committed
+    uint32_t ph = 0;
     bool ok = true;
-    int last = -1;
     for (int t = first; t < total && ok; t += step) {
       const Tile x = tile_of<MODE>(a, bnd, tile0, t);
-      const int kb = k_begin(x.nk), ke = k_end(x.nk);
+      const int nk = __shfl_sync(0xffffffffu, x.nk, 0), cnt = __shfl_sync(0xffffffffu, x.cnt, 0);
+      const int kb = k_begin(nk), ke = k_end(nk);
       for (int c = kb; c < ke && ok; c += a.chunk, ++u) {
         const int b = u & 1;
         if (u >= 2) ok = __all_sync(0xffffffffu, mbar_wait(tempty + b, static_cast<uint32_t>((u >> 1) - 1) & 1u, err));
@@ -355,49 +402,44 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
         const uint32_t acc = tmem + static_cast<uint32_t>(b * BNT);
         const int cend = min(ke, c + a.chunk);
         for (int k = c; k < cend; ++k) {
-          const int s = g % a.stages;
-          ok = __all_sync(0xffffffffu, mbar_wait(full + s, static_cast<uint32_t>(g / a.stages) & 1u, err));
+          ok = __all_sync(0xffffffffu, mbar_wait(full + s, ph, err));
           if (!ok) break;
-          unsigned char* As = smem + s * SB;
+          const uint64_t da = a0 + static_cast<uint32_t>(s * (SB >> 4)), db = b0 + static_cast<uint32_t>(s * (SB >> 4));
+          const uint32_t more = k > c ? 1u : 0u;
           int nkk = kBK / 16;
-          if (MODE == 1) {
-            const int v = x.cnt - k * kBK;           // rows of the group in this k-step
-            if (v < kBK) {                           // the rest belongs to the next group: cleared
-              nkk = (v + 15) / 16;
-              const int lo = v * 8, hi = nkk * 128;  // 16-byte units of a box
-              for (int j = 0; j < 2 + nbox_b; ++j) {
-                uint4* p = reinterpret_cast<uint4*>(j < 2 ? As + j * 8192 : As + kABytes + (j - 2) * 8192);
-                for (int i = lo + lane; i < hi; i += 32) p[i] = make_uint4(0u, 0u, 0u, 0u);
-              }
-              tc::fence_proxy_async_smem();
-              __syncwarp();
+          if (MODE == 1 && cnt - k * kBK < kBK) {
+            // the group ends inside this k-step: its last 16-row slice is filled up with zeros
+            const int v = cnt - k * kBK;
+            nkk = (v + 15) / 16;
+            for (int j = 0; j < 2 + nbox_b; ++j) {
+              uint4* p = reinterpret_cast<uint4*>(smem + s * SB + (j < 2 ? j * 8192 : kABytes + (j - 2) * 8192));
+              for (int i = v * 8 + lane; i < nkk * 128; i += 32) p[i] = make_uint4(0u, 0u, 0u, 0u);
             }
+            tc::fence_proxy_async_smem();
+            __syncwarp();
           }
           tc::tc_fence_after();
-          if (lane == 0) {
-            const uint32_t a0 = smem_u32(As), b0 = a0 + kABytes;
-            for (int kk = 0; kk < nkk; ++kk) {
-              const uint64_t da = MODE == 0 ? tc::sdesc(a0 + kk * 32, 16, 1024) : tc::sdesc(a0 + kk * 2048, 8192, 1024);
-              const uint64_t db = (MODE == 0 && !a.b_mn) ? tc::sdesc(b0 + kk * 32, 16, 1024)
-                                                         : tc::sdesc(b0 + kk * 2048, 8192, 1024);
-              tc::mma_bf16(acc, da, db, idesc, (k > c || kk > 0) ? 1u : 0u);
-            }
+          if (elect_one()) {
+            tc::mma_bf16(acc, da, db, idesc, more);
+#pragma unroll
+            for (int kk = 1; kk < kBK / 16; ++kk)
+              if (MODE == 0 || kk < nkk) tc::mma_bf16(acc, da + kk * ka, db + kk * kb_, idesc, 1u);
             tc::mma_commit(empty + s);
           }
-          __syncwarp();
-          ++g;
+          if (++s == stages) { s = 0; ph ^= 1u; }
         }
-        if (lane == 0) tc::mma_commit(tfull + b);     // on an error too: it completes once the issued MMAs have
+        if (elect_one()) tc::mma_commit(tfull + b);    // on an error too: it completes once the issued MMAs have
         last = u;
       }
     }
-    if (!ok && last >= 0 && lane == 0) mbar_drain(tfull + (last & 1), static_cast<uint32_t>(last >> 1) & 1u);
-    __syncwarp();
-  } else {
+    if (!ok && last >= 0) mbar_drain(tfull + (last & 1), static_cast<uint32_t>(last >> 1) & 1u);
+  } else if (warp >= kFirstEpi) {
     const int q = warp & 3;             // TMEM lane quadrant
-    const int col0 = ((warp - 2) >> 2) * CPW;
+    const int col0 = ((warp - kFirstEpi) >> 2) * CPW;
     const int row = q * 32 + lane;      // this thread's row of the tile
     const bool cols = col0 < a.bn;
+    unsigned char* st = scratch + (warp - kFirstEpi) * kStageBytes;
+    const int es = a.out_f32 ? 4 : 2;
     int u = 0;
     bool ok = true;
     for (int t = first; t < total && ok; t += step) {
@@ -427,37 +469,35 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
       }
       if (!ok) break;
       char* out = static_cast<char*>(a.out);
-      const int es = a.out_f32 ? 4 : 2;
       if (MODE == 1) out += static_cast<int64_t>(x.seg) * a.gstride * es;
+      const int nrows = min(32, x.valid - q * 32);             // this warp's rows that exist
       if (S > 1) {
         const int rows = kBM / S;
-        constexpr int P = BNT + 4;      // floats between rows of a partial tile
-        {
-          const uint32_t dst = map_rank(smem_u32(scratch) + static_cast<uint32_t>(((rank * rows + row % rows) * P + col0) * 4),
-                                        static_cast<uint32_t>(row / rows));
-          if (cols) {
+        // partial tiles [sender][row][BNT]; 16-byte chunk j of row r lies at j ^ (r & 7), so that
+        // neither the senders (a row a lane) nor the sums (a chunk a lane) meet bank conflicts
+        if (cols) {
+          const int r = row % rows;
+          const uint32_t to = static_cast<uint32_t>(row / rows);
+          const uint32_t dst = map_rank(smem_u32(scratch) + static_cast<uint32_t>((rank * rows + r) * BNT * 4), to);
+          const uint32_t bar = map_rank(smem_u32(red_full), to);
 #pragma unroll
-            for (int c = 0; c < CPW; c += 4)
-              if (col0 + c < a.bn) st_remote(dst + c * 4, make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]));
-          }
-          __syncwarp();
-          if (lane == 0) {
-            arrive_remote(map_rank(smem_u32(red_full), static_cast<uint32_t>(q * 32 / rows)));
-            if (rows < 32) arrive_remote(map_rank(smem_u32(red_full), static_cast<uint32_t>(q * 32 / rows + 1)));
-          }
-          __syncwarp();
+          for (int c = 0; c < CPW; c += 4)
+            if (col0 + c < a.bn)
+              st_async(dst + (static_cast<uint32_t>(((col0 + c) >> 2) ^ (r & 7)) << 4), bar,
+                       make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]));
         }
         ok = __all_sync(0xffffffffu, mbar_wait_cluster(red_full, 0, err));
         if (!ok) break;
         const float* part = reinterpret_cast<const float*>(scratch);
         const int nq = a.bn / 4;
-        for (int i = static_cast<int>(threadIdx.x) - 64; i < rows * nq; i += 32 * kEpiWarps) {
+        for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstEpi; i < rows * nq; i += 32 * kEpiWarps) {
           // consecutive threads take consecutive columns of a row, or rows of a transposed output
           const int r = a.transposed ? i % rows : i / nq;
           const int c = 4 * (a.transposed ? i / rows : i - r * nq);
-          float4 v = *reinterpret_cast<const float4*>(part + r * P + c);
+          const int at = ((c >> 2) ^ (r & 7)) << 2;
+          float4 v = *reinterpret_cast<const float4*>(part + r * BNT + at);
           for (int p = 1; p < S; ++p) {
-            const float4 w = *reinterpret_cast<const float4*>(part + (p * rows + r) * P + c);
+            const float4 w = *reinterpret_cast<const float4*>(part + (p * rows + r) * BNT + at);
             v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
           }
           v.x *= a.alpha; v.y *= a.alpha; v.z *= a.alpha; v.w *= a.alpha;
@@ -472,85 +512,97 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
             put4(a, out + static_cast<int64_t>(x.m0 + m) * a.ld * es, n, a.ndim - n, v);
           }
         }
-      } else if (a.transposed) {
-        if (cols && row < x.valid) {
+      } else if (!cols || nrows <= 0) {
+        // nothing of this warp's piece exists
+      } else if (MODE == 1 && a.transposed) {
+        if (row < x.valid) {
 #pragma unroll
           for (int c = 0; c < CPW; ++c)
             if (x.n0 + col0 + c < a.ndim)
               put1(a, out, static_cast<int64_t>(x.n0 + col0 + c) * a.ld + x.m0 + row, a.alpha * acc[c]);
         }
-      } else if (cols) {
-        unsigned char* st = scratch + (warp - 2) * 32 * kStagePitch;
-        char* base = out + static_cast<int64_t>(x.m0 + q * 32) * a.ld * es;
-        const int nrows = min(32, x.valid - q * 32);
-        if (!a.out_f32 && !a.accumulate && a.vec) {
-          // 32 bf16 columns at a time: 64 bytes a row, four lanes a row
+      } else if (a.tma_out && (MODE == 1 || nrows == 32)) {
+        // pieces of 128 bytes a row: chunk j of row r lies at j ^ (r & 7), as the tensor map expects
+        const int z = MODE == 1 ? x.seg : 0;
+        if (!a.out_f32) {
 #pragma unroll
-          for (int c0 = 0; c0 < CPW; c0 += 32) {
+          for (int c0 = 0; c0 < CPW; c0 += 64) {
             if (x.n0 + col0 + c0 < a.ndim) {
+              if (lane == 0) store_read_wait();                // the piece before has left the buffer
+              __syncwarp();
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
+              for (int j = 0; j < 8; ++j) {
                 uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  const __nv_bfloat162 b2 = __floats2bfloat162_rn(a.alpha * acc[c0 + 8 * j + 2 * i], a.alpha * acc[c0 + 8 * j + 2 * i + 1]);
+                  const int c = c0 + 8 * j + 2 * i;
+                  const __nv_bfloat162 b2 = __floats2bfloat162_rn(a.alpha * acc[c], a.alpha * acc[c + 1]);
                   w[i] = *reinterpret_cast<const uint32_t*>(&b2);
                 }
-                *reinterpret_cast<uint4*>(st + lane * kStagePitch + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(st + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
               }
+              tc::fence_proxy_async_smem();
               __syncwarp();
-              const int n = x.n0 + col0 + c0 + (lane & 3) * 8;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int r = i * 8 + (lane >> 2);
-                if (r < nrows && n < a.ndim) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(st + r * kStagePitch + (lane & 3) * 16);
-                  __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(base + static_cast<int64_t>(r) * a.ld * 2) + n;
-                  if (n + 8 <= a.ndim) {
-                    *reinterpret_cast<uint4*>(p) = v;
-                  } else {
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                    for (int j = 0; j < a.ndim - n; ++j)
-                      reinterpret_cast<uint16_t*>(p)[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
-                  }
-                }
-              }
-              __syncwarp();
+              if (lane == 0) tma_store_3d(&mapC, st, x.n0 + col0 + c0, x.m0 + q * 32, z);
             }
           }
         } else {
-          // 16 fp32 columns at a time
 #pragma unroll
-          for (int c0 = 0; c0 < CPW; c0 += 16) {
+          for (int c0 = 0; c0 < CPW; c0 += 32) {
             if (x.n0 + col0 + c0 < a.ndim) {
+              if (lane == 0) store_read_wait();
+              __syncwarp();
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float4*>(st + lane * kStagePitch + j * 16) =
+              for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<float4*>(st + lane * 128 + ((j ^ (lane & 7)) << 4)) =
                     make_float4(a.alpha * acc[c0 + 4 * j], a.alpha * acc[c0 + 4 * j + 1], a.alpha * acc[c0 + 4 * j + 2],
                                 a.alpha * acc[c0 + 4 * j + 3]);
+              tc::fence_proxy_async_smem();
               __syncwarp();
-              const int n = x.n0 + col0 + c0 + (lane & 3) * 4;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int r = i * 8 + (lane >> 2);
-                if (r < nrows && n < a.ndim)
-                  put4(a, base + static_cast<int64_t>(r) * a.ld * es, n, a.ndim - n,
-                       *reinterpret_cast<const float4*>(st + r * kStagePitch + (lane & 3) * 16));
-              }
-              __syncwarp();
+              if (lane == 0) tma_store_3d(&mapC, st, x.n0 + col0 + c0, x.m0 + q * 32, z);
             }
+          }
+        }
+      } else {
+        // masked: 16 fp32 columns at a time through the staging, four lanes a row
+        char* base = out + static_cast<int64_t>(x.m0 + q * 32) * a.ld * es;
+        if (lane == 0) store_read_wait();
+        __syncwarp();
+#pragma unroll
+        for (int c0 = 0; c0 < CPW; c0 += 16) {
+          if (x.n0 + col0 + c0 < a.ndim) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(st + lane * kStagePitch + j * 16) =
+                  make_float4(a.alpha * acc[c0 + 4 * j], a.alpha * acc[c0 + 4 * j + 1], a.alpha * acc[c0 + 4 * j + 2],
+                              a.alpha * acc[c0 + 4 * j + 3]);
+            __syncwarp();
+            const int n = x.n0 + col0 + c0 + (lane & 3) * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = i * 8 + (lane >> 2);
+              if (r < nrows && n < a.ndim)
+                put4(a, base + static_cast<int64_t>(r) * a.ld * es, n, a.ndim - n,
+                     *reinterpret_cast<const float4*>(st + r * kStagePitch + (lane & 3) * 16));
+            }
+            __syncwarp();
           }
         }
       }
     }
+    if (lane == 0) store_wait();        // the last pieces are written before the CTA ends
   }
+  __syncwarp();
+  // Split: a CTA's sends all come before its arrival here, and no CTA leaves before every CTA
+  // has arrived, so none is sent to after it left.
+  if (S > 1) cluster_arrive();
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
   }
-  if (S > 1) cluster_sync_all();        // no CTA leaves while a peer may still send to it
+  if (S > 1) cluster_wait();
 }
 
 }  // namespace gr
