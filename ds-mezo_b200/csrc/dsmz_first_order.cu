@@ -172,16 +172,25 @@ int sm_count(int* sms) {
   return e == cudaSuccess ? 0 : cuda_fail("device query", e);
 }
 
+// Shared memory of a launch; sets a.sbuf and a.stages.
 template <int BNT, int MODE>
-int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, int64_t tiles, int sms, const char* what,
-                   cudaStream_t s) {
+size_t grouped_smem(gr::Args& a, int64_t nk) {
   constexpr int SB = gr::kABytes + BNT * gr::kBK * 2;
   constexpr int kSmem = 227 * 1024;
-  const int scratch = a.split > 1 ? gr::kBM * BNT * 4 : gr::kEpiWarps * gr::kStageBytes;
+  // two staging pieces a warp let a store run while the next piece is staged; the widest tile
+  // gives a stage of the ring for them, which pays where a tile has only a few k-steps
+  a.sbuf = BNT < 256 || nk <= 4 ? 2 : 1;
+  const int scratch = a.split > 1 ? gr::split_bytes(a.split, BNT) : gr::kEpiWarps * gr::kStageBytes * a.sbuf;
   const int fixed = 1024 + scratch + (((a.G + 3) * 8 + 15) & ~15) + 64 + 16 * 8;
   a.stages = (kSmem - fixed) / SB;
   if (a.stages > 8) a.stages = 8;
-  const size_t smem = static_cast<size_t>(fixed) + static_cast<size_t>(a.stages) * SB;
+  return static_cast<size_t>(fixed) + static_cast<size_t>(a.stages) * SB;
+}
+
+template <int BNT, int MODE>
+int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, int64_t tiles, int64_t nk,
+                   int sms, const char* what, cudaStream_t s) {
+  const size_t smem = grouped_smem<BNT, MODE>(a, nk);
   auto* kernel = gr::k_grouped<BNT, MODE>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_fail(what, e);
@@ -213,10 +222,10 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
 
 template <int MODE>
 int launch_grouped_bn(int bnt, const gr::Args& a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C,
-                      int64_t tiles, int sms, const char* what, cudaStream_t s) {
-  if (bnt == 64) return launch_grouped<64, MODE>(a, A, B, C, tiles, sms, what, s);
-  if (bnt == 128) return launch_grouped<128, MODE>(a, A, B, C, tiles, sms, what, s);
-  return launch_grouped<256, MODE>(a, A, B, C, tiles, sms, what, s);
+                      int64_t tiles, int64_t nk, int sms, const char* what, cudaStream_t s) {
+  if (bnt == 64) return launch_grouped<64, MODE>(a, A, B, C, tiles, nk, sms, what, s);
+  if (bnt == 128) return launch_grouped<128, MODE>(a, A, B, C, tiles, nk, sms, what, s);
+  return launch_grouped<256, MODE>(a, A, B, C, tiles, nk, sms, what, s);
 }
 
 // Accumulator width for n output columns and `rows` row tiles: 256 columns where that still
@@ -226,12 +235,47 @@ int columns_for(int64_t n, int64_t rows, int sms) {
   if (n <= 128) return 128;
   return rows * ((n + 255) / 256) >= sms ? 256 : 128;
 }
-// CTAs that share a tile's contraction: as many as one wave of the machine holds, while each
-// still has two k-steps.
-int split_for(int bnt, int64_t tiles, int64_t nk, int sms) {
-  int s = 1;
-  while (s < 8 && bnt <= 128 && tiles * 2 * s <= sms && nk / (2 * s) >= 2) s *= 2;
-  return s;
+// Clusters of s CTAs (one CTA an SM) that the current device runs at once. A cluster lies inside
+// one GPC, whose SMs it need not divide: 74, 45, 33, 26, 22, 15 and 15 clusters of 2 to 8 on a
+// chip with 148 SMs.
+int active_clusters(int s) {
+  static thread_local int cached[9] = {0}, cached_dev = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev != cached_dev) {
+    for (int c = 2; c <= 8; ++c) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(static_cast<unsigned>(c * 256));
+      cfg.blockDim = dim3(gr::kThreadsG);
+      cfg.dynamicSmemBytes = 200 * 1024;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = static_cast<unsigned>(c);
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      auto* kernel = gr::k_grouped<128, 0>;
+      int n = 0;
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
+          cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;                                           // not known: no split of this size
+      }
+      cached[c] = n;
+    }
+    cached_dev = dev;
+  }
+  return cached[s];
+}
+
+// CTAs that share a tile's contraction: as many as one wave of clusters allows, while each still
+// has two k-steps. A second wave would double the time (the 70B rank gradient, 36 tiles in
+// clusters of 4: 93 us).
+int split_for(int bnt, int64_t tiles, int64_t nk) {
+  if (bnt > 128) return 1;
+  for (int s = 8; s > 1; --s)
+    if (tiles <= active_clusters(s) && nk / s >= 2) return s;
+  return 1;
 }
 
 bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -324,7 +368,8 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     const int bnt = columns_for(N, rows, sms);
     a.bn = static_cast<int32_t>(N >= bnt ? bnt : (N + 15) / 16 * 16);
     a.ntn = static_cast<int32_t>((N + a.bn - 1) / a.bn);
-    a.split = split_for(bnt, rows * a.ntn, (K + gr::kBK - 1) / gr::kBK, sms);
+    const int64_t nk = (K + gr::kBK - 1) / gr::kBK;
+    a.split = split_for(bnt, rows * a.ntn, nk);
     // short groups: boxes of 32 rows, so that a tile does not fetch 128
     a.arows = M / G >= 96 ? gr::kBM : 32;
     const int64_t tiles = (rows + 2) * a.ntn;                                    // and the rows outside the groups
@@ -342,7 +387,7 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
       const uint64_t sc[2] = {static_cast<uint64_t>(ld_out) * es, static_cast<uint64_t>(ld_out) * es * M};
       a.tma_out = encode_map(&C, out, 3, dc, sc, 128 / es, 32, a.out_f32 != 0);
     }
-    return launch_grouped_bn<0>(bnt, a, A, B, C, tiles, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
+    return launch_grouped_bn<0>(bnt, a, A, B, C, tiles, nk, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -396,7 +441,8 @@ int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, 
     a.ntn = static_cast<int32_t>((narrow + a.bn - 1) / a.bn);
     const int64_t tiles = static_cast<int64_t>(G) * a.mtn * a.ntn;
     if (tiles > (1 << 27)) return fail(DSMZ_ERR_UNSUPPORTED, me + "too many tiles");
-    a.split = split_for(bnt, tiles, (M / G + gr::kBK - 1) / gr::kBK, sms);
+    const int64_t nk = (M / G + gr::kBK - 1) / gr::kBK;
+    a.split = split_for(bnt, tiles, nk);
     CUtensorMap A, B, C{};
     const uint64_t dx[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(M)}, sx[1] = {static_cast<uint64_t>(ld_x) * 2};
     const uint64_t dd[2] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M)}, sd[1] = {static_cast<uint64_t>(ld_dy) * 2};
@@ -407,7 +453,7 @@ int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, 
       const uint64_t sc[2] = {static_cast<uint64_t>(N) * 4, static_cast<uint64_t>(K) * N * 4};
       a.tma_out = encode_map(&C, out, 3, dc, sc, 32, 32, true);
     }
-    return launch_grouped_bn<1>(bnt, a, A, B, C, tiles, sms, "dsmz_grouped_weight_grad", s);
+    return launch_grouped_bn<1>(bnt, a, A, B, C, tiles, nk, sms, "dsmz_grouped_weight_grad", s);
   });
 }
 

@@ -27,8 +27,8 @@
 // the value) do not need it.
 //
 // Few tiles (narrow outputs): a cluster of 2, 4 or 8 CTAs splits the contraction; each CTA
-// sends its partial tile to the CTA that owns the rows (st.async into its shared memory, which
-// counts the bytes on its barrier), and the owner adds the partials in rank order. No atomics: results are the same on every run.
+// copies its partial tile to the CTAs that own the rows (bulk copies through distributed shared
+// memory, counted on the owner's barrier), and the owner adds the partials in rank order. No atomics: results are the same on every run.
 //
 // Every mbarrier wait gives up after ~1 s, sets the error word, and lets each role finish its
 // own copies before the CTA frees its TMEM.
@@ -56,6 +56,9 @@ constexpr int kStagePitch = 80;         // bytes of a staged 64-byte row piece (
 constexpr int kStageBytes = 4096;       // staging of an epilogue warp: 32 rows of 128 bytes
 constexpr int kABytes = kBM * kBK * 2;
 
+// Shared memory for the partial tiles that a CTA of a split receives.
+__host__ __device__ constexpr int split_bytes(int S, int bnt) { return S * ((kBM + S - 1) / S) * bnt * 4; }
+
 struct Args {
   const int32_t* offsets;               // G + 1, device
   int32_t G, mode;
@@ -67,6 +70,7 @@ struct Args {
   int32_t n_inner;                      // MODE 0: concurrent tiles run along the columns, not the rows
   int32_t arows;                        // MODE 0: rows of an A box
   int32_t stages, split;
+  int32_t sbuf;                         // staging pieces of an epilogue warp, 1 or 2
   int32_t chunk;                        // k-steps per accumulator
   void* out;
   int64_t ld, gstride;                  // output pitch; MODE 1: elements between groups
@@ -107,7 +111,10 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* s
                "r"(x), "r"(y), "r"(z), "r"(smem_u32(src))
                : "memory");
 }
-__device__ __forceinline__ void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// At most N of this thread's stores still read shared memory.
+template <int N>
+__device__ __forceinline__ void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
@@ -119,10 +126,11 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
   return r;
 }
-// 16 bytes to another CTA's shared memory, counted on that CTA's barrier when they land.
-__device__ __forceinline__ void st_async(uint32_t addr, uint32_t bar, float4 v) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "f"(v.x),
-               "f"(v.y), "f"(v.z), "f"(v.w), "r"(bar)
+// `bytes` of this CTA's shared memory to another CTA's, counted on that CTA's barrier when they
+// land. (st.async, 16 bytes a lane, took 3.3 us for a 128 x 64 tile, 6 for 128 x 128.)
+__device__ __forceinline__ void copy_to_rank(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "r"(smem_u32(src)), "r"(bytes), "r"(bar)
                : "memory");
 }
 // One lane of a converged warp.
@@ -266,15 +274,10 @@ __device__ __forceinline__ void put4(const Args& a, char* row, int col, int ncol
     }
   }
 }
-// One element of a transposed output.
+// One element of a transposed output (MODE 1: fp32).
 __device__ __forceinline__ void put1(const Args& a, char* base, int64_t i, float v) {
-  if (a.out_f32) {
-    float* p = reinterpret_cast<float*>(base) + i;
-    *p = a.accumulate ? *p + v : v;
-  } else {
-    __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(base) + i;
-    *p = __float2bfloat16_rn(a.accumulate ? __bfloat162float(*p) + v : v);
-  }
+  float* p = reinterpret_cast<float*>(base) + i;
+  *p = a.accumulate ? *p + v : v;
 }
 
 // BNT: columns of the accumulators (64, 128 or 256; a.bn <= BNT). mapC: the output (3-D, boxes
@@ -284,15 +287,16 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
                                                          const __grid_constant__ CUtensorMap mapB,
                                                          const __grid_constant__ CUtensorMap mapC,
                                                          const __grid_constant__ Args a, int* err) {
-  // columns of an epilogue warp: half a tile, or all of a narrow one (whole 128-byte bf16 rows)
-  constexpr int CPW = BNT == 64 ? 64 : BNT / 2;
+  // columns of an epilogue warp: half a tile, or all of a narrow one whose rows may leave as
+  // 128 bytes of bf16
+  constexpr int CPW = BNT == 64 && MODE == 0 ? 64 : BNT / 2;
   constexpr int SB = kABytes + BNT * kBK * 2;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int S = a.split, stages = a.stages;
   unsigned char* scratch = smem + stages * SB;
   // split: partial tiles of the S CTAs for this CTA's rows; else: the epilogue's staging
-  const int scratch_bytes = S > 1 ? kBM * BNT * 4 : kEpiWarps * kStageBytes;
+  const int scratch_bytes = S > 1 ? split_bytes(S, BNT) : kEpiWarps * kStageBytes * a.sbuf;
   int32_t* bnd = reinterpret_cast<int32_t*>(scratch + scratch_bytes);
   int32_t* tile0 = bnd + a.G + 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(
@@ -318,8 +322,10 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     for (int b = 0; b < 2; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, kEpiWarps); }
     mbar_init(red_full, 1);
     mbar_init_fence();
-    // the partial tiles of this CTA's rows: a.bn columns from each of the S CTAs
-    if (S > 1) mbar_expect_tx(red_full, static_cast<uint32_t>(kBM * a.bn * 4));
+    if (S > 1) {                        // the partial tiles of this CTA's rows, from each of the S CTAs
+      const int rows = (kBM + S - 1) / S;
+      mbar_expect_tx(red_full, static_cast<uint32_t>(S * min(rows, kBM - rank * rows) * ((a.bn + CPW - 1) / CPW) * CPW * 4));
+    }
   } else if (warp == 3 && lane == 0) {
     prefetch_map(&mapA);
     prefetch_map(&mapB);
@@ -337,48 +343,54 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
   auto k_end = [&](int nk) { return S == 1 ? nk : nk * (rank + 1) / S; };
 
   if (warp == 0 || warp == 2) {
-    if (lane == 0) {
-      const bool is_a = warp == 0;
-      int s = 0, n = 0;                 // stage, k-steps issued
-      uint32_t ph = 1;                  // parity of the wait for an empty stage (the first round passes)
-      bool ok = true;
-      for (int t = first; t < total && ok; t += step) {
-        const Tile x = tile_of<MODE>(a, bnd, tile0, t);
-        const int nba = MODE == 0 ? (x.valid + a.arows - 1) / a.arows : 2;
-        const uint32_t bytes = !is_a ? (b_mn ? static_cast<uint32_t>(nbox_b * 8192) : static_cast<uint32_t>(a.bn * 128))
-                                     : (MODE == 0 ? static_cast<uint32_t>(nba * a.arows * 128) : 16384u);
-        const int ke = k_end(x.nk);
-        for (int k = k_begin(x.nk); k < ke; ++k) {
-          if (!mbar_wait(empty + s, ph, err)) { ok = false; break; }
-          unsigned char* dst = smem + s * SB + (is_a ? 0 : kABytes);
-          mbar_expect_tx(full + s, bytes);
+    // As the MMA warp below: the whole warp walks the loop, one elected lane issues.
+    const bool is_a = warp == 0;
+    int s = 0, n = 0;                   // stage, k-steps issued
+    uint32_t ph = 1;                    // parity of the wait for an empty stage (the first round passes)
+    bool ok = true;
+    for (int t = first; t < total && ok; t += step) {
+      const Tile y = tile_of<MODE>(a, bnd, tile0, t);
+      const int nk = __shfl_sync(0xffffffffu, y.nk, 0), m0 = __shfl_sync(0xffffffffu, y.m0, 0);
+      const int n0 = __shfl_sync(0xffffffffu, y.n0, 0), seg = __shfl_sync(0xffffffffu, y.seg, 0);
+      const int r0 = __shfl_sync(0xffffffffu, y.r0, 0), valid = __shfl_sync(0xffffffffu, y.valid, 0);
+      const int nba = MODE == 0 ? (valid + a.arows - 1) / a.arows : 2;
+      const uint32_t bytes = !is_a ? (b_mn ? static_cast<uint32_t>(nbox_b * 8192) : static_cast<uint32_t>(a.bn * 128))
+                                   : (MODE == 0 ? static_cast<uint32_t>(nba * a.arows * 128) : 16384u);
+      const int ke = k_end(nk);
+      for (int k = k_begin(nk); k < ke; ++k) {
+        ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ph, err));
+        if (!ok) break;
+        unsigned char* dst = smem + s * SB + (is_a ? 0 : kABytes);
+        uint64_t* bar = full + s;
+        if (elect_one()) {
+          mbar_expect_tx(bar, bytes);
           if (MODE == 0) {
             if (is_a) {
-              for (int i = 0; i < nba; ++i)
-                tma_load_2d(dst + i * a.arows * 128, &mapA, k * kBK, x.m0 + i * a.arows, full + s);
+              tma_load_2d(dst, &mapA, k * kBK, m0, bar);
+              for (int i = 1; i < nba; ++i) tma_load_2d(dst + i * a.arows * 128, &mapA, k * kBK, m0 + i * a.arows, bar);
             } else if (b_mn) {
-              for (int j = 0; j < nbox_b; ++j) tma_load_3d(dst + j * 8192, &mapB, x.n0 + 64 * j, k * kBK, x.seg - 1, full + s);
+              for (int j = 0; j < nbox_b; ++j) tma_load_3d(dst + j * 8192, &mapB, n0 + 64 * j, k * kBK, seg - 1, bar);
             } else {
-              tma_load_3d(dst, &mapB, k * kBK, x.n0, x.seg - 1, full + s);
+              tma_load_3d(dst, &mapB, k * kBK, n0, seg - 1, bar);
             }
           } else {
-            const int r = x.r0 + k * kBK;
+            const int r = r0 + k * kBK;
             if (is_a) {
-              tma_load_2d(dst, &mapA, x.m0, r, full + s);
-              tma_load_2d(dst + 8192, &mapA, x.m0 + 64, r, full + s);
+              tma_load_2d(dst, &mapA, m0, r, bar);
+              tma_load_2d(dst + 8192, &mapA, m0 + 64, r, bar);
             } else {
-              for (int j = 0; j < nbox_b; ++j) tma_load_2d(dst + j * 8192, &mapB, x.n0 + 64 * j, r, full + s);
+              for (int j = 0; j < nbox_b; ++j) tma_load_2d(dst + j * 8192, &mapB, n0 + 64 * j, r, bar);
             }
           }
-          ++n;
-          if (++s == stages) { s = 0; ph ^= 1u; }
         }
+        ++n;
+        if (++s == stages) { s = 0; ph ^= 1u; }
       }
-      // on an error: let the loads already issued land before the CTA can exit
-      if (!ok)
-        for (int i = (n > stages ? n - stages : 0); i < n; ++i)
-          mbar_drain(full + (i % stages), static_cast<uint32_t>(i / stages) & 1u);
     }
+    // on an error: let the loads already issued land before the CTA can exit
+    if (!ok)
+      for (int i = (n > stages ? n - stages : 0); i < n; ++i)
+        mbar_drain(full + (i % stages), static_cast<uint32_t>(i / stages) & 1u);
   } else if (warp == 1) {
     // The whole warp walks the loop, with every branch on a vote or a broadcast, so that stages
     // and descriptors stay in uniform registers; one elected lane issues.
@@ -438,7 +450,8 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     const int col0 = ((warp - kFirstEpi) >> 2) * CPW;
     const int row = q * 32 + lane;      // this thread's row of the tile
     const bool cols = col0 < a.bn;
-    unsigned char* st = scratch + (warp - kFirstEpi) * kStageBytes;
+    unsigned char* st = scratch + (warp - kFirstEpi) * a.sbuf * kStageBytes;
+    int flip = 0;                       // staging piece in use
     const int es = a.out_f32 ? 4 : 2;
     int u = 0;
     bool ok = true;
@@ -472,37 +485,47 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
       if (MODE == 1) out += static_cast<int64_t>(x.seg) * a.gstride * es;
       const int nrows = min(32, x.valid - q * 32);             // this warp's rows that exist
       if (S > 1) {
-        const int rows = kBM / S;
-        // partial tiles [sender][row][BNT]; 16-byte chunk j of row r lies at j ^ (r & 7), so that
-        // neither the senders (a row a lane) nor the sums (a chunk a lane) meet bank conflicts
+        // Partial tiles [sender][column half][row][CPW]; 16-byte chunk j of row r lies at j ^ (r & 7),
+        // so that neither writing a row a lane nor summing a chunk a lane meets bank conflicts.
+        // Each warp stages its piece where the ring was (every load of this CTA has landed and
+        // every MMA is done) and copies the rows of each owner as one block.
+        const int rows = (kBM + S - 1) / S, half = col0 / CPW;
+        constexpr int RB = CPW * 4, H = BNT / CPW;       // bytes of a staged row, column halves
         if (cols) {
-          const int r = row % rows;
-          const uint32_t to = static_cast<uint32_t>(row / rows);
-          const uint32_t dst = map_rank(smem_u32(scratch) + static_cast<uint32_t>((rank * rows + r) * BNT * 4), to);
-          const uint32_t bar = map_rank(smem_u32(red_full), to);
+          unsigned char* mine = smem + ((warp - kFirstEpi) >> 2) * (kBM * RB) + row * RB;
 #pragma unroll
           for (int c = 0; c < CPW; c += 4)
-            if (col0 + c < a.bn)
-              st_async(dst + (static_cast<uint32_t>(((col0 + c) >> 2) ^ (r & 7)) << 4), bar,
-                       make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]));
+            *reinterpret_cast<float4*>(mine + (((c >> 2) ^ (row & 7)) << 4)) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+          tc::fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (cols && lane == 0) {
+          int r = q * 32;
+          while (r < q * 32 + 32) {
+            const int to = r / rows, upto = min(min(q * 32 + 32, (to + 1) * rows), kBM);
+            const uint32_t dst = smem_u32(scratch) + static_cast<uint32_t>(((rank * H + half) * rows + r - to * rows) * RB);
+            copy_to_rank(map_rank(dst, static_cast<uint32_t>(to)), smem + half * (kBM * RB) + r * RB,
+                         static_cast<uint32_t>((upto - r) * RB), map_rank(smem_u32(red_full), static_cast<uint32_t>(to)));
+            r = upto;
+          }
         }
         ok = __all_sync(0xffffffffu, mbar_wait_cluster(red_full, 0, err));
         if (!ok) break;
-        const float* part = reinterpret_cast<const float*>(scratch);
-        const int nq = a.bn / 4;
-        for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstEpi; i < rows * nq; i += 32 * kEpiWarps) {
+        const int first_row = rank * rows, nr = min(rows, kBM - first_row);     // the rows this CTA owns
+        constexpr int NQ = BNT / 4;
+        for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstEpi; i < rows * NQ; i += 32 * kEpiWarps) {
           // consecutive threads take consecutive columns of a row, or rows of a transposed output
-          const int r = a.transposed ? i % rows : i / nq;
-          const int c = 4 * (a.transposed ? i / rows : i - r * nq);
-          const int at = ((c >> 2) ^ (r & 7)) << 2;
-          float4 v = *reinterpret_cast<const float4*>(part + r * BNT + at);
+          const int r = a.transposed ? i % rows : i / NQ;
+          const int c = 4 * (a.transposed ? i / rows : i % NQ);
+          const int m = first_row + r, n = x.n0 + c;
+          if (r >= nr || m >= x.valid || c >= a.bn || n >= a.ndim) continue;
+          const unsigned char* part = scratch + ((c / CPW) * rows + r) * RB + ((((c % CPW) >> 2) ^ (m & 7)) << 4);
+          float4 v = *reinterpret_cast<const float4*>(part);
           for (int p = 1; p < S; ++p) {
-            const float4 w = *reinterpret_cast<const float4*>(part + (p * rows + r) * BNT + at);
+            const float4 w = *reinterpret_cast<const float4*>(part + p * H * rows * RB);
             v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
           }
           v.x *= a.alpha; v.y *= a.alpha; v.z *= a.alpha; v.w *= a.alpha;
-          const int m = rank * rows + r, n = x.n0 + c;
-          if (m >= x.valid || n >= a.ndim) continue;
           if (a.transposed) {
             const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -515,21 +538,51 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
       } else if (!cols || nrows <= 0) {
         // nothing of this warp's piece exists
       } else if (MODE == 1 && a.transposed) {
+        // a lane a feature: each column's 32 values are contiguous
         if (row < x.valid) {
+          float* p = reinterpret_cast<float*>(out) + static_cast<int64_t>(x.n0 + col0) * a.ld + x.m0 + row;
+          const int nc = min(CPW, a.ndim - x.n0 - col0);
 #pragma unroll
-          for (int c = 0; c < CPW; ++c)
-            if (x.n0 + col0 + c < a.ndim)
-              put1(a, out, static_cast<int64_t>(x.n0 + col0 + c) * a.ld + x.m0 + row, a.alpha * acc[c]);
+          for (int c = 0; c < CPW; ++c) {
+            if (c < nc) *p = a.accumulate ? *p + a.alpha * acc[c] : a.alpha * acc[c];
+            p += a.ld;
+          }
         }
-      } else if (a.tma_out && (MODE == 1 || nrows == 32)) {
-        // pieces of 128 bytes a row: chunk j of row r lies at j ^ (r & 7), as the tensor map expects
-        const int z = MODE == 1 ? x.seg : 0;
+      } else if (a.vec && !a.accumulate && a.ndim * es % 16 == 0) {
+        // pieces of 32 rows x 128 bytes; chunk j of row r lies at j ^ (r & 7), as the tensor map
+        // expects. A whole piece leaves by TMA; of a group's last rows eight lanes store each row.
+        const bool whole = a.tma_out && (MODE == 1 || nrows == 32);
+        char* base = out + (static_cast<int64_t>(x.m0 + q * 32) * a.ld + x.n0 + col0) * es;
+        auto piece = [&](int c0) {                        // the columns from c0 on are staged: send them
+          if (whole) {
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tma_store_3d(&mapC, st + flip, x.n0 + col0 + c0, x.m0 + q * 32, MODE == 1 ? x.seg : 0);
+          } else {
+            if (lane == 0) store_commit();                // an empty group: pieces and groups stay in step
+            __syncwarp();
+            const int j = lane & 7, left = (a.ndim - x.n0 - col0 - c0) * es - 16 * j;
+            char* p = base + c0 * es + 16 * j + static_cast<int64_t>(lane >> 3) * a.ld * es;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3);
+              const uint4 v = *reinterpret_cast<const uint4*>(st + flip + r * 128 + ((j ^ (r & 7)) << 4));
+              if (r < nrows && left > 0) *reinterpret_cast<uint4*>(p) = v;
+              p += 4 * a.ld * es;
+            }
+          }
+        };
+        auto ready = [&]() -> unsigned char* {             // a piece of staging whose last store has read it
+          flip = a.sbuf == 2 ? flip ^ kStageBytes : 0;
+          if (lane == 0) { if (a.sbuf == 2) store_read_wait<1>(); else store_read_wait<0>(); }
+          __syncwarp();
+          return st + flip + lane * 128;
+        };
         if (!a.out_f32) {
 #pragma unroll
           for (int c0 = 0; c0 < CPW; c0 += 64) {
             if (x.n0 + col0 + c0 < a.ndim) {
-              if (lane == 0) store_read_wait();                // the piece before has left the buffer
-              __syncwarp();
+              unsigned char* mine = ready();
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 uint32_t w[4];
@@ -539,34 +592,29 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
                   const __nv_bfloat162 b2 = __floats2bfloat162_rn(a.alpha * acc[c], a.alpha * acc[c + 1]);
                   w[i] = *reinterpret_cast<const uint32_t*>(&b2);
                 }
-                *reinterpret_cast<uint4*>(st + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(mine + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
               }
-              tc::fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) tma_store_3d(&mapC, st, x.n0 + col0 + c0, x.m0 + q * 32, z);
+              piece(c0);
             }
           }
         } else {
 #pragma unroll
           for (int c0 = 0; c0 < CPW; c0 += 32) {
             if (x.n0 + col0 + c0 < a.ndim) {
-              if (lane == 0) store_read_wait();
-              __syncwarp();
+              unsigned char* mine = ready();
 #pragma unroll
               for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<float4*>(st + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                *reinterpret_cast<float4*>(mine + ((j ^ (lane & 7)) << 4)) =
                     make_float4(a.alpha * acc[c0 + 4 * j], a.alpha * acc[c0 + 4 * j + 1], a.alpha * acc[c0 + 4 * j + 2],
                                 a.alpha * acc[c0 + 4 * j + 3]);
-              tc::fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) tma_store_3d(&mapC, st, x.n0 + col0 + c0, x.m0 + q * 32, z);
+              piece(c0);
             }
           }
         }
       } else {
-        // masked: 16 fp32 columns at a time through the staging, four lanes a row
+        // odd pitches and accumulation: 16 fp32 columns at a time through the staging, four lanes a row
         char* base = out + static_cast<int64_t>(x.m0 + q * 32) * a.ld * es;
-        if (lane == 0) store_read_wait();
+        if (lane == 0) store_read_wait<0>();
         __syncwarp();
 #pragma unroll
         for (int c0 = 0; c0 < CPW; c0 += 16) {
