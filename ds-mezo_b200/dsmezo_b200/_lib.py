@@ -9,6 +9,8 @@ import ctypes
 import os
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
+import torch
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libdsmezo.so")
 
@@ -196,6 +198,28 @@ def check(status: int, what: str) -> None:
     if status != 0:
         msg = lib().dsmz_last_error()
         raise DsmzError(f"{what} failed (status {status}): {msg.decode() if msg else ''}")
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def current_stream(index: int) -> int:
+    """The current stream of CUDA device `index`, as the C entry points take it."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def launch(what: str, device, fn, *args) -> None:
+    """fn(*args, stream) on the device's current stream, with that device current; raises on an
+    error status. The device is switched only where another is current: the switch costs a few
+    microseconds, as much as a small kernel."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, current_stream(index))
+    if rc != 0:
+        check(rc, what)
 
 
 def schedule(name_or_coeffs) -> NSSchedule:

@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._lib import DSMZ_BF16, DSMZ_F32, GROUPED_ACCUMULATE, GROUPED_ZERO_REST, MAX_GROUPS, check, lib
+from ._lib import DSMZ_BF16, DSMZ_F32, GROUPED_ACCUMULATE, GROUPED_ZERO_REST, MAX_GROUPS, launch, lib
 
 __all__ = ["grouped_matmul", "grouped_weight_grad", "adapter_forward", "adapter_backward", "device_error"]
 
@@ -27,22 +27,25 @@ def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError(f"{what}: CUDA tensors only (no CPU fallback)")
     if t.dim() != 2 or t.dtype != torch.bfloat16:
         raise ValueError(f"{what}: operands are 2-D bfloat16 tensors")
-    if t.shape[1] < 1:
-        raise ValueError(f"{what}: an operand has no columns")
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
-        return t
     width = t.shape[1]
+    if width < 1:
+        raise ValueError(f"{what}: an operand has no columns")
+    pitch, unit = t.stride()
+    if unit == 1 and pitch % 8 == 0 and pitch >= width and t.data_ptr() % 16 == 0:
+        return t
     return t.new_empty(t.shape[0], (width + 7) // 8 * 8)[:, :width].copy_(t)
 
 
 def _weights(w: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     """(tensor, group stride, row pitch, whether N is the contiguous dimension) of w: G x K x N."""
     G, K, N = w.shape
-    for nc, inner, outer in ((0, 1, 2), (1, 2, 1)):
-        if w.stride(inner) == 1 and w.stride(outer) % 8 == 0 and w.stride(outer) >= w.shape[inner] and \
-                (G == 1 or (w.stride(0) % 8 == 0 and w.stride(0) > 0)) and w.data_ptr() % 16 == 0:
-            return w, w.stride(0), w.stride(outer), nc
-    nc = 0 if w.stride(1) < w.stride(2) else 1                     # keep the faster dimension
+    gs, sk, sn = w.stride()
+    if (G == 1 or (gs % 8 == 0 and gs > 0)) and w.data_ptr() % 16 == 0:
+        if sk == 1 and sn % 8 == 0 and sn >= K:
+            return w, gs, sn, 0
+        if sn == 1 and sk % 8 == 0 and sk >= N:
+            return w, gs, sk, 1
+    nc = 0 if sk < sn else 1                                       # keep the faster dimension
     inner = K if nc == 0 else N
     pad = (inner + 7) // 8 * 8
     c = w.new_empty(G, N if nc == 0 else K, pad)[:, :, :inner]
@@ -92,11 +95,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, row_offsets: torch.Tensor, 
     if M == 0:
         return out
     w, gs, ld, nc = _weights(w, me)
-    with torch.cuda.device(x.device):
-        check(lib().dsmz_grouped_matmul(x.data_ptr(), M, K, x.stride(0) if M > 1 else (K + 7) // 8 * 8, w.data_ptr(), G, N, gs, ld,
-                                        nc, row_offsets.data_ptr(), _DT[out.dtype], out.data_ptr(),
-                                        out.stride(0) if M > 1 else N, float(alpha), flags,
-                                        torch.cuda.current_stream(x.device).cuda_stream), me)
+    launch(me, x.device, lib().dsmz_grouped_matmul, x.data_ptr(), M, K, x.stride(0) if M > 1 else (K + 7) // 8 * 8,
+           w.data_ptr(), G, N, gs, ld, nc, row_offsets.data_ptr(), _DT[out.dtype], out.data_ptr(),
+           out.stride(0) if M > 1 else N, float(alpha), flags)
     return out
 
 
@@ -120,11 +121,9 @@ def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, row_offsets: torch.Te
         out = torch.empty(G, K, N, dtype=torch.float32, device=x.device)
     elif tuple(out.shape) != (G, K, N) or out.dtype != torch.float32 or out.device != x.device or not out.is_contiguous():
         raise ValueError(f"{me}: out must be a contiguous G x K x N float32 tensor on the operands' device")
-    with torch.cuda.device(x.device):
-        check(lib().dsmz_grouped_weight_grad(x.data_ptr(), M, K, x.stride(0) if M > 1 else (K + 7) // 8 * 8, dy.data_ptr(), N,
-                                             dy.stride(0) if M > 1 else (N + 7) // 8 * 8, G, row_offsets.data_ptr(), out.data_ptr(),
-                                             float(alpha), GROUPED_ACCUMULATE if accumulate else 0,
-                                             torch.cuda.current_stream(x.device).cuda_stream), me)
+    launch(me, x.device, lib().dsmz_grouped_weight_grad, x.data_ptr(), M, K, x.stride(0) if M > 1 else (K + 7) // 8 * 8,
+           dy.data_ptr(), N, dy.stride(0) if M > 1 else (N + 7) // 8 * 8, G, row_offsets.data_ptr(), out.data_ptr(),
+           float(alpha), GROUPED_ACCUMULATE if accumulate else 0)
     return out
 
 

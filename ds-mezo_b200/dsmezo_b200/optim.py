@@ -17,7 +17,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import ADAMW_BLOCK, DSMZ_BF16, DSMZ_F32, AdamWDesc, AdamWTensor, check, lib
+from ._lib import ADAMW_BLOCK, DSMZ_BF16, DSMZ_F32, AdamWDesc, AdamWTensor, lib
 
 __all__ = ["AdamW", "AdamWState"]
 
@@ -180,23 +180,21 @@ class AdamW:
             self.grads = None                    # a later step() must be given its own again
         elif self.grads is None:
             raise ValueError("AdamW: no gradients bound; give them to step()")
-        with torch.cuda.device(self.device):
-            d = self._desc
-            if self.step_counter is None and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdamW: a captured step would repeat one step number at every replay; "
-                                   "construct with capturable=True")
-            d.lr_device = self._scalar(lr, "lr") if isinstance(lr, torch.Tensor) else None
-            d.lr = self.lr if lr is None or d.lr_device else float(lr)
-            d.grad_scale = self._scalar(grad_scale, "grad_scale")
-            d.step = self.step_count + 1
-            d.step_counter = None if self.step_counter is None else self.step_counter.data_ptr()
-            ws, nbytes = None, 0
-            if d.step_counter or d.lr_device:
-                ws = torch.empty(_lib.ADAMW_WORKSPACE_BYTES, dtype=torch.uint8, device=self.device)
-                nbytes = ws.numel()
-            check(lib().dsmz_adamw_step(ctypes.byref(d), self._table, len(self.params),
-                                        None if ws is None else ws.data_ptr(), nbytes,
-                                        torch.cuda.current_stream(self.device).cuda_stream), "adamw_step")
+        d = self._desc
+        if self.step_counter is None and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a captured step would repeat one step number at every replay; "
+                               "construct with capturable=True")
+        d.lr_device = self._scalar(lr, "lr") if isinstance(lr, torch.Tensor) else None
+        d.lr = self.lr if lr is None or d.lr_device else float(lr)
+        d.grad_scale = self._scalar(grad_scale, "grad_scale")
+        d.step = self.step_count + 1
+        d.step_counter = None if self.step_counter is None else self.step_counter.data_ptr()
+        ws, nbytes = None, 0
+        if d.step_counter or d.lr_device:
+            ws = torch.empty(_lib.ADAMW_WORKSPACE_BYTES, dtype=torch.uint8, device=self.device)
+            nbytes = ws.numel()
+        _lib.launch("adamw_step", self.device, lib().dsmz_adamw_step, ctypes.byref(d), self._table, len(self.params),
+                    None if ws is None else ws.data_ptr(), nbytes)
         if self.step_counter is None:
             self.step_count += 1
 
@@ -214,6 +212,4 @@ class AdamW:
         table = type(self._table).from_buffer_copy(self._table)
         for e, a, v in zip(table, m_out, v_out):
             e.param, e.shadow = a.data_ptr(), v.data_ptr()
-        with torch.cuda.device(self.device):
-            check(lib().dsmz_adamw_state_values(table, n, torch.cuda.current_stream(self.device).cuda_stream),
-                  "adamw_state_values")
+        _lib.launch("adamw_state_values", self.device, lib().dsmz_adamw_state_values, table, n)

@@ -15,7 +15,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-from ._lib import check, lib
+from ._lib import check, launch, lib
 
 SCORE_LOGITS_F32, SCORE_LOGITS_BF16, SCORE_LOGPROBS_F32 = 0, 1, 2
 
@@ -100,14 +100,13 @@ def contrastive_loss_grad(logits: torch.Tensor, seq_tokens: Sequence[int], advan
         start[i + 1] = start[i] + int(k)
     adv = (ctypes.c_double * max(n, 1))(*[float(a) for a in advantages])
     L = lib()
-    with torch.cuda.device(logits.device):
-        wsb = int(L.dsmz_contrastive_loss_grad_workspace_bytes(ntok))
-        ws = torch.empty(wsb, dtype=torch.uint8, device=logits.device)
-        loss = torch.empty(1, dtype=torch.float32, device=logits.device)
-        check(L.dsmz_contrastive_loss_grad(
-            SCORE_LOGITS_F32 if logits.dtype == torch.float32 else SCORE_LOGITS_BF16, logits.data_ptr(), V, ld,
-            tgt.data_ptr(), ntok, start, adv, n, float(grad_scale), loss.data_ptr(), out.data_ptr(), ld_out,
-            ws.data_ptr(), wsb, torch.cuda.current_stream(logits.device).cuda_stream), "contrastive_loss_grad")
+    wsb = int(L.dsmz_contrastive_loss_grad_workspace_bytes(ntok))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=logits.device)
+    loss = torch.empty(1, dtype=torch.float32, device=logits.device)
+    launch("contrastive_loss_grad", logits.device, L.dsmz_contrastive_loss_grad,
+           SCORE_LOGITS_F32 if logits.dtype == torch.float32 else SCORE_LOGITS_BF16, logits.data_ptr(), V, ld,
+           tgt.data_ptr(), ntok, start, adv, n, float(grad_scale), loss.data_ptr(), out.data_ptr(), ld_out,
+           ws.data_ptr(), wsb)
     return loss, out
 
 
