@@ -151,18 +151,31 @@ int adamw_run(const dsmz_adamw_desc& d, const dsmz_adamw_tensor* tensors, int32_
 // Error word of the grouped products' bounded waits, one per device.
 __device__ int g_grouped_err;
 
-// Tensor map of rank 2 or 3 (inner dimension contiguous, byte strides of the others), 128-byte
-// swizzle, zero fill outside; bf16, or fp32.
+// Tensor map of rank 2 to 4 (inner dimension contiguous, byte strides of the others, boxes of up
+// to three dimensions), 128-byte swizzle, zero fill outside; bf16, or fp32.
 bool encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
-                uint32_t box0, uint32_t box1, bool f32 = false) {
+                uint32_t box0, uint32_t box1, bool f32 = false, uint32_t box2 = 1) {
   auto fn = encode_fn();
   if (!fn) return false;
-  cuuint64_t d[3] = {dims[0], dims[1], rank == 3 ? dims[2] : 1}, st[2] = {strides[0], rank == 3 ? strides[1] : 0};
-  cuuint32_t box[3] = {box0, box1, 1}, es[3] = {1, 1, 1};
+  cuuint64_t d[4] = {1, 1, 1, 1}, st[3] = {0, 0, 0};
+  for (int i = 0; i < rank; ++i) d[i] = dims[i];
+  for (int i = 0; i + 1 < rank; ++i) st[i] = strides[i];
+  cuuint32_t box[4] = {box0, box1, box2, 1}, es[4] = {1, 1, 1, 1};
   return fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank),
             const_cast<void*>(base), d, st, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// `rows` rows of `width` bf16 (byte pitch), to be read in boxes of 64 rows x `cols` columns with the
+// column as the MMA's major dimension: slabs of 64 columns (64, row, slab) where the width is a
+// whole number of them, so that a box is one copy; else boxes of 64 columns.
+bool encode_width(CUtensorMap* m, int32_t* slabs, const void* base, int64_t width, int64_t rows, int64_t pitch, int cols) {
+  *slabs = width % 64 == 0;
+  const uint64_t d[3] = {*slabs ? 64u : static_cast<uint64_t>(width), static_cast<uint64_t>(rows), static_cast<uint64_t>(width / 64)};
+  const uint64_t st[2] = {static_cast<uint64_t>(pitch) * 2, 128};
+  return *slabs ? encode_map(m, base, 3, d, st, 64, 64, false, static_cast<uint32_t>((cols + 63) / 64))
+                : encode_map(m, base, 2, d, st, 64, 64);
 }
 
 int sm_count(int* sms) {
@@ -192,17 +205,19 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
                    int sms, const char* what, cudaStream_t s) {
   const size_t smem = grouped_smem<BNT, MODE>(a, nk);
   auto* kernel = gr::k_grouped<BNT, MODE>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e != cudaSuccess) return cuda_fail(what, e);
+  // per thread and device: the shared memory limit and the error word's address
   static thread_local int* err = nullptr;
   static thread_local int err_dev = -1;
   int dev = 0;
-  e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && (dev != err_dev || !err)) {
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev != err_dev) {
     void* p = nullptr;
-    e = cudaGetSymbolAddress(&p, g_grouped_err);
-    err = static_cast<int*>(p);
-    err_dev = dev;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e == cudaSuccess) e = cudaGetSymbolAddress(&p, g_grouped_err);
+    if (e == cudaSuccess) {
+      err = static_cast<int*>(p);
+      err_dev = dev;
+    }
   }
   if (e != cudaSuccess) return cuda_fail(what, e);
   cudaLaunchConfig_t cfg{};
@@ -376,11 +391,15 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     if (tiles > (1 << 27)) return fail(DSMZ_ERR_UNSUPPORTED, me + "too many tiles");
     CUtensorMap A, B, C{};
     const uint64_t da[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(M)}, sa[1] = {static_cast<uint64_t>(ld_x) * 2};
-    const uint64_t db[3] = {static_cast<uint64_t>(wi), static_cast<uint64_t>(wo), static_cast<uint64_t>(G)};
-    const uint64_t sb[2] = {static_cast<uint64_t>(w_ld) * 2,
-                            static_cast<uint64_t>(G > 1 ? w_group_stride : (w_ld * wo + 7) / 8 * 8) * 2};
+    const uint64_t pitch = static_cast<uint64_t>(w_ld) * 2;
+    const uint64_t group = static_cast<uint64_t>(G > 1 ? w_group_stride : (w_ld * wo + 7) / 8 * 8) * 2;
+    const uint64_t db[3] = {static_cast<uint64_t>(wi), static_cast<uint64_t>(wo), static_cast<uint64_t>(G)}, sb[2] = {pitch, group};
+    const uint64_t ds[4] = {64, static_cast<uint64_t>(wo), static_cast<uint64_t>(wi / 64), static_cast<uint64_t>(G)};
+    const uint64_t ss[3] = {pitch, 128, group};
+    a.b_slabs = w_n_contiguous && N % 64 == 0;
     if (!encode_map(&A, x, 2, da, sa, gr::kBK, static_cast<uint32_t>(a.arows)) ||
-        !encode_map(&B, w, 3, db, sb, 64, w_n_contiguous ? 64 : static_cast<uint32_t>(a.bn)))
+        !(a.b_slabs ? encode_map(&B, w, 4, ds, ss, 64, 64, false, static_cast<uint32_t>((a.bn + 63) / 64))
+                    : encode_map(&B, w, 3, db, sb, 64, w_n_contiguous ? 64 : static_cast<uint32_t>(a.bn))))
       return fail(DSMZ_ERR_CUDA, me + "the driver refused a tensor map");
     if (a.vec && !a.accumulate && a.split == 1) {
       const uint64_t dc[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M), 1};
@@ -444,9 +463,8 @@ int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, 
     const int64_t nk = (M / G + gr::kBK - 1) / gr::kBK;
     a.split = split_for(bnt, tiles, nk);
     CUtensorMap A, B, C{};
-    const uint64_t dx[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(M)}, sx[1] = {static_cast<uint64_t>(ld_x) * 2};
-    const uint64_t dd[2] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M)}, sd[1] = {static_cast<uint64_t>(ld_dy) * 2};
-    if (!encode_map(xw ? &A : &B, x, 2, dx, sx, 64, 64) || !encode_map(xw ? &B : &A, dy, 2, dd, sd, 64, 64))
+    if (!encode_width(&A, &a.a_slabs, xw ? x : dy, wide, M, xw ? ld_x : ld_dy, gr::kBM) ||
+        !encode_width(&B, &a.b_slabs, xw ? dy : x, narrow, M, xw ? ld_dy : ld_x, a.bn))
       return fail(DSMZ_ERR_CUDA, me + "the driver refused a tensor map");
     if (a.vec && !a.accumulate && !a.transposed && a.split == 1) {
       const uint64_t dc[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(K), static_cast<uint64_t>(G)};

@@ -67,6 +67,8 @@ struct Args {
   int32_t bn;                           // MMA N (multiple of 16) = columns of a tile
   int32_t ntn, mtn;                     // column tiles; MODE 1: feature tiles
   int32_t b_mn;                         // MODE 0: W is contiguous along N
+  int32_t a_slabs, b_slabs;             // an operand read along its rows' width is mapped as slabs of 64
+                                        // columns (slab, row, 64) and comes in one box
   int32_t n_inner;                      // MODE 0: concurrent tiles run along the columns, not the rows
   int32_t arows;                        // MODE 0: rows of an A box
   int32_t stages, split;
@@ -80,24 +82,30 @@ struct Args {
   float alpha;
 };
 
-// 32 lanes x 32 consecutive fp32 columns of TMEM.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 lanes x 32 consecutive fp32 columns of TMEM into v[0..31]; complete after tmem_wait().
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Waits for the thread's TMEM loads (their registers pass through an empty volatile asm after it,
+// so that no use of them moves before the wait).
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// Box {inner, rows, 1} of a 3-D tensor map (inner, row, group) into this CTA's shared memory.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+// Box of a 3-D tensor map into this CTA's shared memory.
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
@@ -209,39 +217,55 @@ struct Tile {
   int nk;                               // k-steps of the whole contraction
 };
 
-template <int MODE>
-__device__ __forceinline__ Tile tile_of(const Args& a, const int32_t* bnd, const int32_t* tile0, int t) {
-  Tile x;
-  if (MODE == 0) {
-    int lo = 0, hi = a.G + 1;           // the last segment whose first tile is at or before t
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (tile0[mid] * a.ntn <= t) lo = mid; else hi = mid - 1;
-    }
-    const int nm = tile0[lo + 1] - tile0[lo];
-    const int local = t - tile0[lo] * a.ntn;
-    int nt, mt;
-    if (a.n_inner) { mt = local / a.ntn; nt = local - mt * a.ntn; } else { nt = local / nm; mt = local - nt * nm; }
-    x.seg = lo;
-    x.m0 = bnd[lo] + mt * kBM;
-    x.n0 = nt * a.bn;
-    x.valid = min(kBM, bnd[lo + 1] - x.m0);
-    x.r0 = x.cnt = 0;
-    x.nk = (lo >= 1 && lo <= a.G) ? (a.kdim + kBK - 1) / kBK : 0;
-  } else {
-    const int per = a.mtn * a.ntn;
-    x.seg = t / per;
-    const int local = t - x.seg * per;
-    const int nt = local / a.mtn;
-    x.m0 = (local - nt * a.mtn) * kBM;
-    x.n0 = nt * a.bn;
-    x.valid = min(kBM, a.mdim - x.m0);
-    x.r0 = bnd[x.seg + 1];
-    x.cnt = bnd[x.seg + 2] - x.r0;
-    x.nk = (x.cnt + kBK - 1) / kBK;
-  }
-  return x;
+// i / d for 0 <= i < 2^27 and d >= 1, with inv = 1 / d rounded: the estimate is off by one at most.
+__device__ __forceinline__ int fast_div(int i, int d, float inv) {
+  int q = static_cast<int>(static_cast<float>(i) * inv);
+  if (static_cast<float>(i) >= 16777216.f) q = i / d;          // beyond fp32's integers
+  q += (i - q * d >= d) ? 1 : 0;
+  q -= (i - q * d < 0) ? 1 : 0;
+  return q;
 }
+
+// Walks a CTA's tiles t, t + step, ... in ascending order.
+template <int MODE>
+struct Cursor {
+  int lo;                               // MODE 0: segment of the last tile found
+  float inv_ntn, inv_mtn, inv_per;
+  __device__ __forceinline__ Cursor(const Args& a) : lo(0) {
+    inv_ntn = 1.f / static_cast<float>(a.ntn);
+    if (MODE == 1) {
+      inv_mtn = 1.f / static_cast<float>(a.mtn);
+      inv_per = 1.f / (static_cast<float>(a.mtn) * static_cast<float>(a.ntn));
+    }
+  }
+  __device__ __forceinline__ Tile at(const Args& a, const int32_t* bnd, const int32_t* tile0, int t) {
+    Tile x;
+    if (MODE == 0) {
+      while (tile0[lo + 1] * a.ntn <= t) ++lo;         // t is below the total: stops at a segment with tiles
+      const int t0 = tile0[lo], nm = tile0[lo + 1] - t0, local = t - t0 * a.ntn;
+      int nt, mt;
+      if (a.n_inner) { mt = fast_div(local, a.ntn, inv_ntn); nt = local - mt * a.ntn; } else { nt = local / nm; mt = local - nt * nm; }
+      x.seg = lo;
+      x.m0 = bnd[lo] + mt * kBM;
+      x.n0 = nt * a.bn;
+      x.valid = min(kBM, bnd[lo + 1] - x.m0);
+      x.r0 = x.cnt = 0;
+      x.nk = (lo >= 1 && lo <= a.G) ? (a.kdim + kBK - 1) / kBK : 0;
+    } else {
+      const int per = a.mtn * a.ntn;
+      x.seg = fast_div(t, per, inv_per);
+      const int local = t - x.seg * per;
+      const int nt = fast_div(local, a.mtn, inv_mtn);
+      x.m0 = (local - nt * a.mtn) * kBM;
+      x.n0 = nt * a.bn;
+      x.valid = min(kBM, a.mdim - x.m0);
+      x.r0 = bnd[x.seg + 1];
+      x.cnt = bnd[x.seg + 2] - x.r0;
+      x.nk = (x.cnt + kBK - 1) / kBK;
+    }
+    return x;
+  }
+};
 
 // Four consecutive output columns: (old +) alpha v, rounded once.
 __device__ __forceinline__ void put4(const Args& a, char* row, int col, int ncols, float4 v) {
@@ -348,8 +372,9 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     int s = 0, n = 0;                   // stage, k-steps issued
     uint32_t ph = 1;                    // parity of the wait for an empty stage (the first round passes)
     bool ok = true;
+    Cursor<MODE> cur(a);
     for (int t = first; t < total && ok; t += step) {
-      const Tile y = tile_of<MODE>(a, bnd, tile0, t);
+      const Tile y = cur.at(a, bnd, tile0, t);
       const int nk = __shfl_sync(0xffffffffu, y.nk, 0), m0 = __shfl_sync(0xffffffffu, y.m0, 0);
       const int n0 = __shfl_sync(0xffffffffu, y.n0, 0), seg = __shfl_sync(0xffffffffu, y.seg, 0);
       const int r0 = __shfl_sync(0xffffffffu, y.r0, 0), valid = __shfl_sync(0xffffffffu, y.valid, 0);
@@ -369,15 +394,22 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
               tma_load_2d(dst, &mapA, k * kBK, m0, bar);
               for (int i = 1; i < nba; ++i) tma_load_2d(dst + i * a.arows * 128, &mapA, k * kBK, m0 + i * a.arows, bar);
             } else if (b_mn) {
-              for (int j = 0; j < nbox_b; ++j) tma_load_3d(dst + j * 8192, &mapB, n0 + 64 * j, k * kBK, seg - 1, bar);
+              if (a.b_slabs) tma_load_4d(dst, &mapB, 0, k * kBK, n0 >> 6, seg - 1, bar);
+              else for (int j = 0; j < nbox_b; ++j) tma_load_3d(dst + j * 8192, &mapB, n0 + 64 * j, k * kBK, seg - 1, bar);
             } else {
               tma_load_3d(dst, &mapB, k * kBK, n0, seg - 1, bar);
             }
           } else {
             const int r = r0 + k * kBK;
             if (is_a) {
-              tma_load_2d(dst, &mapA, m0, r, bar);
-              tma_load_2d(dst + 8192, &mapA, m0 + 64, r, bar);
+              if (a.a_slabs) {
+                tma_load_3d(dst, &mapA, 0, r, m0 >> 6, bar);
+              } else {
+                tma_load_2d(dst, &mapA, m0, r, bar);
+                tma_load_2d(dst + 8192, &mapA, m0 + 64, r, bar);
+              }
+            } else if (a.b_slabs) {
+              tma_load_3d(dst, &mapB, 0, r, n0 >> 6, bar);
             } else {
               for (int j = 0; j < nbox_b; ++j) tma_load_2d(dst + j * 8192, &mapB, n0 + 64 * j, r, bar);
             }
@@ -402,8 +434,9 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     int s = 0, u = 0, last = -1;        // stage, accumulators begun, the last one committed
     uint32_t ph = 0;
     bool ok = true;
+    Cursor<MODE> cur(a);
     for (int t = first; t < total && ok; t += step) {
-      const Tile x = tile_of<MODE>(a, bnd, tile0, t);
+      const Tile x = cur.at(a, bnd, tile0, t);
       const int nk = __shfl_sync(0xffffffffu, x.nk, 0), cnt = __shfl_sync(0xffffffffu, x.cnt, 0);
       const int kb = k_begin(nk), ke = k_end(nk);
       for (int c = kb; c < ke && ok; c += a.chunk, ++u) {
@@ -455,12 +488,15 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     const int es = a.out_f32 ? 4 : 2;
     int u = 0;
     bool ok = true;
+    Cursor<MODE> cur(a);
     for (int t = first; t < total && ok; t += step) {
-      const Tile x = tile_of<MODE>(a, bnd, tile0, t);
+      const Tile x = cur.at(a, bnd, tile0, t);
       const int kb = k_begin(x.nk), ke = k_end(x.nk);
       float acc[CPW];
+      if (kb >= ke) {
 #pragma unroll
-      for (int c = 0; c < CPW; ++c) acc[c] = 0.f;
+        for (int c = 0; c < CPW; ++c) acc[c] = 0.f;
+      }
       for (int c = kb; c < ke; c += a.chunk, ++u) {
         const int b = u & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(tfull + b, static_cast<uint32_t>(u >> 1) & 1u, err));
@@ -468,12 +504,22 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
         tc::tc_fence_after();
         const uint32_t src = tmem + static_cast<uint32_t>(b * BNT + col0) + (static_cast<uint32_t>(q * 32) << 16);
         if (cols) {
+          if (c == kb) {                // the first accumulator as it is: all loads, then one wait
+            uint32_t v[CPW];
 #pragma unroll
-          for (int c0 = 0; c0 < CPW; c0 += 32) {
-            float v[32];
-            tmem_ld32(src + c0, v);
+            for (int c0 = 0; c0 < CPW; c0 += 32) tmem_ld32(src + c0, v + c0);
+            tmem_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c0 + i] += v[i];
+            for (int i = 0; i < CPW; ++i) { asm volatile("" : "+r"(v[i])); acc[i] = __uint_as_float(v[i]); }
+          } else {
+#pragma unroll
+            for (int c0 = 0; c0 < CPW; c0 += 32) {
+              uint32_t v[32];
+              tmem_ld32(src + c0, v);
+              tmem_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) { asm volatile("" : "+r"(v[i])); acc[c0 + i] += __uint_as_float(v[i]); }
+            }
           }
         }
         tc::tc_fence_before();
