@@ -147,9 +147,27 @@ int adamw_run(const dsmz_adamw_desc& d, const dsmz_adamw_tensor* tensors, int32_
       [&](const aw::Args<CAP>& a, int grid) { launch_adamw<CAP>(a, grid, d.param_dtype, d.grad_dtype, d.state_bits, s); });
 }
 
+// Error word of the bounded waits, one per device.
+__device__ int g_wait_err;
+
+int wait_err(int** p) {
+  static thread_local int* addr = nullptr;
+  static thread_local int addr_dev = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev != addr_dev) {
+    void* q = nullptr;
+    e = cudaGetSymbolAddress(&q, g_wait_err);
+    if (e == cudaSuccess) {
+      addr = static_cast<int*>(q);
+      addr_dev = dev;
+    }
+  }
+  *p = addr;
+  return e == cudaSuccess ? 0 : cuda_fail("error word", e);
+}
+
 // ------------------------------------------------------------------ products grouped by adapter copy
-// Error word of the grouped products' bounded waits, one per device.
-__device__ int g_grouped_err;
 
 // Tensor map of rank 2 to 4 (inner dimension contiguous, byte strides of the others, boxes of up
 // to three dimensions), 128-byte swizzle, zero fill outside; bf16, or fp32.
@@ -205,19 +223,15 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
                    int sms, const char* what, cudaStream_t s) {
   const size_t smem = grouped_smem<BNT, MODE>(a, nk);
   auto* kernel = gr::k_grouped<BNT, MODE>;
-  // per thread and device: the shared memory limit and the error word's address
-  static thread_local int* err = nullptr;
-  static thread_local int err_dev = -1;
+  int* err = nullptr;
+  int rc = wait_err(&err);
+  if (rc) return rc;
+  static thread_local int set_dev = -1;                  // the device whose shared memory limit is raised
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && dev != err_dev) {
-    void* p = nullptr;
+  if (e == cudaSuccess && dev != set_dev) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-    if (e == cudaSuccess) e = cudaGetSymbolAddress(&p, g_grouped_err);
-    if (e == cudaSuccess) {
-      err = static_cast<int*>(p);
-      err_dev = dev;
-    }
+    if (e == cudaSuccess) set_dev = dev;
   }
   if (e != cudaSuccess) return cuda_fail(what, e);
   cudaLaunchConfig_t cfg{};
@@ -475,14 +489,14 @@ int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, 
   });
 }
 
-int32_t dsmz_grouped_device_error(dsmz_stream_t stream) {
+int32_t dsmz_first_order_device_error(dsmz_stream_t stream) {
   int v = -1, zero = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cudaMemcpyFromSymbolAsync(&v, g_grouped_err, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+  if (cudaMemcpyFromSymbolAsync(&v, g_wait_err, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
       cudaStreamSynchronize(s) != cudaSuccess)
     return -1;
   if (v != 0) {
-    cudaMemcpyToSymbolAsync(g_grouped_err, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
+    cudaMemcpyToSymbolAsync(g_wait_err, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
     cudaStreamSynchronize(s);
   }
   return v;

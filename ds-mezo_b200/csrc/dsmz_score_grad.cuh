@@ -7,9 +7,11 @@
 // over the slice keeps a running maximum and sum of exponentials a thread; the CTAs exchange
 // (max, sum) through distributed shared memory; pass two reads the slice again, from L2 (a cluster's barrier empties L1), and writes the
 // gradient. HBM sees each logit once in and each gradient once out, which is the floor: 190 us
-// for 2048 rows of 152064 bf16 logits, of which this takes 273 (0.70). The unit that makes
-// exponentials and packs bf16 pairs is 61% busy (2.5 operations a logit), the rest is the
-// latency of a slice's two passes.
+// for 2048 rows of 152064 bf16 logits, of which this takes 260 (0.73). The unit that makes
+// exponentials and packs bf16 pairs is busy two thirds of the time (2.5 operations a logit),
+// the rest is the latency between a slice's two passes. A variant that streamed whole rows
+// through a shared-memory ring, one CTA a row, took 244 us there but 119 against 113 for 2048 rows
+// of 65536; it did not stay.
 // Rows need not be aligned: a slice has a scalar head up to the first 16-byte boundary,
 // 16-byte accesses, and a scalar tail. The target's logit is read before the exchange, so
 // the gradient may overwrite the logits.
@@ -32,7 +34,8 @@ namespace sg {
 
 constexpr int kMaxSeqs = 128;
 // Largest slice of a row. 2048 rows of 152064 bf16 logits (304 KB) took 311, 297, 273 and 345 us
-// with 1, 2, 4 and 8 CTAs of 256 threads a row (293, 279, 361 and 515 us with 512 threads):
+// with 1, 2, 4 and 8 CTAs of 256 threads a row (293, 279, 361 and 515 us with 512 threads),
+// before the packed arithmetic below:
 // more CTAs cut the tail of the last wave, and past slices of 76 KB their barriers cost more.
 constexpr int kSliceBytes = 80 * 1024;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -116,9 +119,50 @@ template <> struct Vec<__nv_bfloat16> {
   __device__ static void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 };
 
+// Two fp32 in one register pair: the packed instructions halve the issue slots of everything but
+// the exponentials and the maximum (273 -> 260 us, with registers for a fifth CTA an SM).
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void split(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 c;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
+  return c;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 c;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
+  return c;
+}
+__device__ __forceinline__ F2 exp2_of(F2 a) {
+  float x, y;
+  a.split(x, y);
+  return F2(ex2(x), ex2(y));
+}
+// One 16-byte vector as pairs.
+__device__ __forceinline__ void load_pairs(const float* p, F2 (&x)[2], float& top) {
+  const float4 u = *reinterpret_cast<const float4*>(p);
+  top = fmaxf(top, fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w)));
+  x[0] = F2(u.x, u.y);
+  x[1] = F2(u.z, u.w);
+}
+__device__ __forceinline__ void load_pairs(const __nv_bfloat16* p, F2 (&x)[4], float& top) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float a = __uint_as_float(w[q] << 16), b = __uint_as_float(w[q] & 0xFFFF0000u);
+    top = fmaxf(top, fmaxf(a, b));
+    x[q] = F2(a, b);
+  }
+}
+
 // grid: ntok * cluster size; row = blockIdx.x / cluster size.
 template <typename T>
-__global__ void __launch_bounds__(256) k_loss_grad(const T* logits, int64_t ld, int64_t V,
+__global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t ld, int64_t V,
                                                    const int32_t* __restrict__ targets, Seqs seqs, double grad_scale,
                                                    T* grad, int64_t ld_grad, double* __restrict__ term) {
   constexpr int N = Vec<T>::N;
@@ -154,21 +198,20 @@ __global__ void __launch_bounds__(256) k_loss_grad(const T* logits, int64_t ld, 
   // UN vectors a thread: one maximum and one rescaling of the running sum for all of them
   auto block = [&](auto un, int i) {
     constexpr int UN = decltype(un)::value;
-    float y[UN][N];
-#pragma unroll
-    for (int u = 0; u < UN; ++u) Vec<T>::load(xv + static_cast<int64_t>(i + u * nt) * N, y[u]);
+    F2 y[UN][N / 2];
     float t = m;
 #pragma unroll
-    for (int u = 0; u < UN; ++u)
-#pragma unroll
-      for (int k = 0; k < N; ++k) t = fmaxf(t, y[u][k]);
+    for (int u = 0; u < UN; ++u) load_pairs(xv + static_cast<int64_t>(i + u * nt) * N, y[u], t);
     const float b = t == -INFINITY ? 0.f : t;         // -inf logits alone: every exponential is 0
-    float a[2] = {0.f, 0.f};
+    const F2 nb(-b, -b), le(kLog2e, kLog2e);
+    F2 acc(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
-      for (int k = 0; k < N; ++k) a[k & 1] += exp_of(y[u][k] - b);
-    s = s * exp_of(m - b) + (a[0] + a[1]);
+      for (int k = 0; k < N / 2; ++k) acc = acc + exp2_of((y[u][k] + nb) * le);
+    float a0, a1;
+    acc.split(a0, a1);
+    s = s * exp_of(m - b) + (a0 + a1);
     m = t;
   };
   int i = tid;
@@ -212,25 +255,24 @@ __global__ void __launch_bounds__(256) k_loss_grad(const T* logits, int64_t ld, 
   auto value = [&](float y) { return wf * (exp_of(y - m) * inv); };
   T* gv = g + v0;
   if (same) {
-    i = tid;
-    for (; i + 3 * nt < nv; i += 4 * nt) {
-      float y[4][N];
+    auto pass = [&](auto un, int i) {
+      constexpr int UN = decltype(un)::value;
+      F2 y[UN][N / 2];
+      float unused = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) Vec<T>::load(xv + static_cast<int64_t>(i + u * nt) * N, y[u]);
+      for (int u = 0; u < UN; ++u) load_pairs(xv + static_cast<int64_t>(i + u * nt) * N, y[u], unused);
+      const F2 nm(-m, -m), le(kLog2e, kLog2e), ww(wf * inv, wf * inv);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < UN; ++u) {
+        float z[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) y[u][k] = value(y[u][k]);
-        Vec<T>::store(gv + static_cast<int64_t>(i + u * nt) * N, y[u]);
+        for (int k = 0; k < N / 2; ++k) (exp2_of((y[u][k] + nm) * le) * ww).split(z[2 * k], z[2 * k + 1]);
+        Vec<T>::store(gv + static_cast<int64_t>(i + u * nt) * N, z);
       }
-    }
-    for (; i < nv; i += nt) {
-      float y[N];
-      Vec<T>::load(xv + static_cast<int64_t>(i) * N, y);
-#pragma unroll
-      for (int k = 0; k < N; ++k) y[k] = value(y[k]);
-      Vec<T>::store(gv + static_cast<int64_t>(i) * N, y);
-    }
+    };
+    i = tid;
+    for (; i + 3 * nt < nv; i += 4 * nt) pass(std::integral_constant<int, 4>{}, i);
+    for (; i < nv; i += nt) pass(std::integral_constant<int, 1>{}, i);
   } else {
     for (i = tid; i < nv; i += nt) {
       float y[N];

@@ -157,4 +157,4 @@ def device_error(device=None) -> int:
     """Reads and clears the device's error word of the grouped products (synchronises the
     current stream): nonzero when a kernel's barrier wait ran out of time."""
     with torch.cuda.device(device):
-        return int(lib().dsmz_grouped_device_error(torch.cuda.current_stream().cuda_stream))
+        return int(lib().dsmz_first_order_device_error(torch.cuda.current_stream().cuda_stream))

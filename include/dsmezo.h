@@ -394,10 +394,10 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
 int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, const void* dy, int64_t N, int64_t ld_dy,
                              int32_t G, const int32_t* row_offsets, float* out, float alpha, uint32_t flags,
                              dsmz_stream_t stream);
-/* Reads and clears the current device's error word of the grouped products (synchronises the
+/* Reads and clears the current device's error word of the first-order kernels (synchronises the
  * stream): 1 when a kernel gave up on a barrier wait after its time limit, -1 when the word
  * could not be read. */
-int32_t dsmz_grouped_device_error(dsmz_stream_t stream);
+int32_t dsmz_first_order_device_error(dsmz_stream_t stream);
 
 /* The contrastive scoring loss (dsmz_contrastive_loss) with its gradient in the logits:
  *   loss[0] (device F32; the terms and their sum are fp64) = sum_i a_i mean_{t in i} nll_t

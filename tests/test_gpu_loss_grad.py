@@ -183,9 +183,42 @@ def test_offsets_past_32_bits(S):
     x = base.repeat(n // 50, 1)
     t = t50.repeat(n // 50)
     lens, adv = [n], [float(n)]
-    S.contrastive_loss_grad(x, lens, adv, t, out=x)
-    _, want = S.contrastive_loss_grad(base, [50], [50.0], t50)
-    assert torch.equal(x[-50:], want) and torch.equal(x[:50], want) and torch.equal(x[14100:14150], want)
+    loss, _ = S.contrastive_loss_grad(x, lens, adv, t, out=x)
+    for a in (0, 14100, n - 50):
+        check(base, [50], [50.0], t50, loss / (n / 50), x[a:a + 50])
+    assert torch.equal(x[:50], x[-50:])
+
+
+@pytest.mark.parametrize("dt,V", [(torch.bfloat16, 40000), (torch.bfloat16, 32771), (torch.float32, 20001), (torch.float32, 65536)])
+def test_many_long_rows(S, dt, V):
+    # two waves of rows past 64 KB, ragged last slices, in place too
+    n, pitch = 330, (-V) % 8 + 8
+    x, t = rows(n, V, dt, 31, pitch=pitch)
+    t[5], t[6], t[7] = V - 1, 0, V // 8 * 8 - 1
+    lens, adv = [100, 1, 229], [1.0, -2.0, 0.5]
+    loss, grad = S.contrastive_loss_grad(x, lens, adv, t)
+    check(x, lens, adv, t, loss, grad)
+    again = S.contrastive_loss_grad(x, lens, adv, t)
+    assert torch.equal(again[0], loss) and torch.equal(again[1], grad)
+    old = x.clone()
+    x[300, 17:] = float("-inf")
+    x[301] = float("-inf")
+    x[302, 5] = float("nan")
+    x[303] = torch.finfo(dt).min
+    t[300], t[304] = 3, V
+    bad = S.contrastive_loss_grad(x, lens, adv, t)
+    assert torch.isnan(bad[0]).all() and torch.isnan(bad[1][[301, 302, 304]]).all()
+    assert torch.isfinite(bad[1][:301]).all() and torch.isfinite(bad[1][303]).all()
+    t[300], t[304] = 1, 1
+    keep = torch.ones(n, dtype=torch.bool, device=DEV)
+    keep[301:303] = False
+    for i in (300, 303):
+        one = S.contrastive_loss_grad(x[i:i + 1], [1], [0.5 / 229], t[i:i + 1])[1]
+        check(x[i:i + 1], [1], [0.5 / 229], t[i:i + 1], S.contrastive_loss_grad(x[i:i + 1], [1], [0.5 / 229], t[i:i + 1])[0], one)
+    x.copy_(old)
+    buf = x.clone(memory_format=torch.preserve_format)
+    loss2, out = S.contrastive_loss_grad(buf, lens, adv, t, out=buf)
+    check(x, lens, adv, t, loss2, out)
 
 
 def test_refusals(S):
