@@ -27,7 +27,7 @@ from typing import List, Optional, Sequence
 
 import torch
 
-from . import _lib
+from . import _lib, grouped
 from ._lib import DSMZ_BF16, DSMZ_F32, BasisSpec, ModuleSpec, PlanDesc, check, lib
 
 FLT_MIN = float(torch.finfo(torch.float32).tiny)
@@ -237,6 +237,59 @@ class AdapterSet:
     def V(self, b):
         s = self.bases[b]
         return self.V_arena[self.offV[b]:self.offV[b] + s.D * self.basis_width].view(s.D, self.basis_width)
+
+    # ------------------------------------------------------------------ products through the adapters
+    def grad_arena(self) -> torch.Tensor:
+        """A zeroed fp32 gradient arena laid out as the master factors (A(i, g) and B(i, g) view
+        it), for ``delta_backward`` and ``AdamW.for_adapters``."""
+        return torch.zeros(self.numel, dtype=torch.float32, device=self.device)
+
+    def _copies(self, i: int, which: str):
+        """(A, B) of module i: copies x d_out x r and copies x r x d_in views of the bf16 arenas."""
+        if self.copy_dtype != torch.bfloat16:
+            raise ValueError("products through the adapters take bfloat16 copies (copy_dtype=torch.bfloat16)")
+        arena = {"shadow": self.shadow, "pos": self.pos, "neg": self.neg}.get(which)
+        if arena is None:
+            raise ValueError("which must be 'shadow', 'pos' or 'neg'")
+        m, r = self.modules[i], self.rank
+        n = 1 if which == "shadow" else self.directions
+        a = arena.as_strided((n, m.d_out, r), (self.capacity, r, 1), arena.storage_offset() + self.offA[i])
+        b = arena.as_strided((n, r, m.d_in), (self.capacity, m.d_in, 1), arena.storage_offset() + self.offB[i])
+        return a, b
+
+    def _rows(self, x: torch.Tensor, row_offsets: Optional[torch.Tensor], n: int) -> torch.Tensor:
+        if row_offsets is not None:
+            return row_offsets
+        if n != 1:
+            raise ValueError(f"{n} copies need row_offsets (the first row of each copy's rows, and the end)")
+        rows = x.shape[0]
+        return torch.arange(0, 2 * max(rows, 1), max(rows, 1), dtype=torch.int32, device=x.device) if rows else \
+            torch.zeros(2, dtype=torch.int32, device=x.device)
+
+    def delta(self, i: int, x: torch.Tensor, which: str = "shadow", row_offsets: Optional[torch.Tensor] = None, *,
+              out: Optional[torch.Tensor] = None, alpha: float = 1.0, accumulate: bool = False):
+        """The share of module i's adapters in its output: (y, t), y[row] = alpha * (x[row] B^T) A^T
+        with the row's own copy, t = x B^T.
+
+        x: rows x d_in, bf16. which: 'shadow' (the factors as last updated) or 'pos' / 'neg',
+        whose ``directions`` copies each own the rows [row_offsets[k], row_offsets[k + 1]) (int32
+        on the device; may be left out for a single copy). out, accumulate: add to the base
+        module's output in place. Runs on the current stream; see ``grouped.adapter_forward``."""
+        A, B = self._copies(i, which)
+        return grouped.adapter_forward(x, A, B, self._rows(x, row_offsets, A.shape[0]), out=out, alpha=alpha,
+                                       accumulate=accumulate)
+
+    def delta_backward(self, i: int, dy: torch.Tensor, x: torch.Tensor, t: torch.Tensor, grad: torch.Tensor, *,
+                       alpha: float = 1.0, accumulate: bool = False, need_dx: bool = True) -> Optional[torch.Tensor]:
+        """Gradients of ``delta(i, x, 'shadow')``: writes (accumulate: adds) those of A and B into
+        module i's part of the gradient arena and returns the one in x (None without need_dx)."""
+        A, B = self._copies(i, "shadow")
+        if grad.dtype != torch.float32 or grad.dim() != 1 or grad.numel() < self.numel or not grad.is_contiguous():
+            raise ValueError("delta_backward: grad is a gradient arena (grad_arena())")
+        dx, _, _ = grouped.adapter_backward(dy, x, t, A, B, self._rows(x, None, 1), alpha=alpha,
+                                            dA=self.A(i, grad).unsqueeze(0), dB=self.B(i, grad).unsqueeze(0),
+                                            accumulate=accumulate, need_dx=need_dx)
+        return dx
 
     # ------------------------------------------------------------------ plan
     def _build_plan(self, rng_offset_before: int):
