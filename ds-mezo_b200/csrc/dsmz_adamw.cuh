@@ -15,13 +15,13 @@
 // those of 64-bit arithmetic: a warp forms its block in fp32 with a bound on every rounding
 // made, decides the elements that lie within that bound of a border (one block in thirty has
 // one) in fp64, and takes the scales from the one or two elements that can be the largest,
-// formed again in fp64. The 161.5 M elements of a 7B set (bf16 gradients and shadow, 16 bytes
-// an element, 394 us at the measured copy rate) took 1634 us with everything in fp64, 1376 in
-// fp32 with blocks near a border done again whole, 634 with single elements done again, no
-// conversions, and a path without bounds for whole blocks. What bounds it is instruction
-// issue (83%): some 60 instructions an element.
-// A block with a NaN or an infinity gets
-// a scale that makes every element of the block NaN: the whole block, not one element.
+// formed again in fp64. A 7B set (161.5 M elements; bf16 gradients and shadow, 16 bytes an
+// element, 394 us at the measured copy rate) took 1634 us with everything in fp64, 1376 in
+// fp32 with blocks near a border done again whole, 723 with single elements done again, no
+// conversions and a path without bounds for whole blocks, 590 with packed arithmetic. What
+// bounds it is instruction issue and latency: 84 instructions an element, 32 warps an SM.
+// A block with a NaN or an infinity gets a scale that makes every element of the block NaN: the
+// whole block, not one element.
 //
 // One CTA takes a tile of one tensor, a warp one block of 256: its lanes own elements
 // 4 l .. 4 l + 3 and 128 + 4 l .. + 3, so that every access of a warp is contiguous. The pass
@@ -32,6 +32,7 @@
 #include <stdint.h>
 
 #include "dsmezo.h"
+#include "dsmz_pairs.cuh"
 
 namespace dsmz {
 namespace aw {
@@ -171,9 +172,6 @@ __device__ __forceinline__ uint32_t pack4(const uint32_t (&c)[4]) {
 // 2^23 + byte k of u, without the conversion unit.
 __device__ __forceinline__ float byte_float(uint32_t u, int k) {
   return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440u + static_cast<uint32_t>(k)));
-}
-__device__ __forceinline__ float floor_small(float x) {     // 0 <= x < 2^22
-  return __fadd_rd(x, 8388608.f) - 8388608.f;
 }
 constexpr float kU = 0x1p-24f;   // half a step of fp32: one rounding
 
@@ -336,27 +334,42 @@ __device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, 
         for (int k = 0; k < 4; ++k) g[h][k] *= gs;
     }
     const float o1 = a.fo1, o2 = a.fo2, cm = ms * a.fb1, cv = (vs * vs) * a.fb2;
-    float m[2][4], v[2][4];
-    uint32_t mtb = 0, vtb = 0, gtb = 0, pos[2] = {0, 0};
+    F2 m2[2][2], v2[2][2];                             // the new m and v, two elements a pair
+    uint32_t mtb = 0, vtb = 0;
+    float gt = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float qm = byte_float(mq[h], k) - 8388736.f, qv = byte_float(vq[h], k) - 8388608.f;
-        const float q2 = qv * qv;
-        // |error| of the mean: at most 3 kU of the old term, 3 kU of the new, kU of the sum
-        float mm = fmaf(g[h][k], o1, (qm * fabsf(qm)) * cm);
-        float vv = fmaf(g[h][k] * g[h][k], o2, (q2 * q2) * cv);           // 6 kU
-        if (!FULL && k >= nv[h]) mm = vv = 0.f;        // past the tensor: a NaN scale must not count there
-        m[h][k] = mm;
-        v[h][k] = vv;
-        pos[h] |= (fabsf(g[h][k]) + qv > 0.f) ? 1u << (8 * k) : 0u;
-        mtb = max(mtb, __float_as_uint(fabsf(mm)));    // as integers: a NaN wins
-        vtb = max(vtb, __float_as_uint(vv));
-        gtb = max(gtb, __float_as_uint(fabsf(g[h][k])));
+      for (int j = 0; j < 2; ++j) {
+        const int k = 2 * j;
+        const F2 gg(g[h][k], g[h][k + 1]);
+        float q0, q1;
+        const F2 qm = F2(byte_float(mq[h], k), byte_float(mq[h], k + 1)) + F2(-8388736.f);
+        qm.split(q0, q1);
+        // error of the mean: at most 3 kU of the old term, 3 kU of the new, kU of the sum
+        F2 mm = fma2(gg, F2(o1), (qm * F2(fabsf(q0), fabsf(q1))) * F2(cm));
+        const F2 qv = F2(byte_float(vq[h], k), byte_float(vq[h], k + 1)) + F2(-8388608.f);
+        const F2 q2 = qv * qv;
+        F2 vv = fma2(gg * gg, F2(o2), (q2 * q2) * F2(cv));                // 6 kU
+        float a0, a1, b0, b1;
+        mm.split(a0, a1);
+        vv.split(b0, b1);
+        if (!FULL) {                                   // past the tensor: a NaN scale must not count there
+          if (k >= nv[h]) a0 = b0 = 0.f;
+          if (k + 1 >= nv[h]) a1 = b1 = 0.f;
+          mm = F2(a0, a1);
+          vv = F2(b0, b1);
+        }
+        m2[h][j] = mm;
+        v2[h][j] = vv;
+        mtb = max(max(mtb, __float_as_uint(fabsf(a0))), __float_as_uint(fabsf(a1)));   // as integers: a NaN wins
+        vtb = max(max(vtb, __float_as_uint(b0)), __float_as_uint(b1));
+        gt = fmaxf(fmaxf(gt, fabsf(g[h][k])), fabsf(g[h][k + 1]));
         // the update itself with the one-instruction root and reciprocal (2 kU each): its error
         // is far below that of the 8-bit states it is made from
-        p[h][k] = fmaf(-c.step, mm * rcp_ftz(fmaf(sqrt_ftz(vv), c.inv_root, a.eps)), p[h][k] * c.decay);
+        float d0, d1;
+        fma2(F2(sqrt_ftz(b0), sqrt_ftz(b1)), F2(c.inv_root), F2(a.eps)).split(d0, d1);
+        fma2(F2(-c.step), mm * F2(rcp_ftz(d0), rcp_ftz(d1)), F2(p[h][k], p[h][k + 1]) * F2(c.decay)).split(p[h][k], p[h][k + 1]);
       }
       store4<P>(t.p, i[h], nv[h], vec, p[h]);
       if (sizeof(P) == 4 && t.shadow) store4<__nv_bfloat16>(t.shadow, i[h], nv[h], vec, p[h]);
@@ -364,43 +377,83 @@ __device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, 
     const float mt = __uint_as_float(__reduce_max_sync(0xffffffffu, mtb));
     const float vt = __uint_as_float(__reduce_max_sync(0xffffffffu, vtb));
     // no |old term| + |new term| of the block is above et
-    const float et = 1.0001f * fmaf(__uint_as_float(__reduce_max_sync(0xffffffffu, gtb)), o1, 16129.f * cm);
+    gt = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(gt)));
+    const float et = 1.0001f * fmaf(gt, o1, 16129.f * cm);
     // fp32 carries the block where its largest values are well inside the range and the means
     // do not cancel throughout; an all-zero block is exact
     const bool mok = (mt > 0x1p-90f && mt < 0x1p100f && et <= 32.f * mt) || et == 0.f;
     const bool vok = (vt > 0x1p-70f && vt < 0x1p100f && (vs == 0.f || vs > 0x1p-60f)) ||
-                     (vt == 0.f && !__any_sync(0xffffffffu, (pos[0] | pos[1]) != 0));
-    uint32_t near = 0;             // elements next to a border: bits 0-7 for m, 8-15 for v
+                     (vt == 0.f && gt == 0.f && !__any_sync(0xffffffffu, (vq[0] | vq[1]) != 0));
     const float im = mt > 0.f ? 16129.f * rcp_ftz(mt) : 0.f, iv = vt > 0.f ? 4228250625.f * rcp_ftz(vt) : 0.f;
     const float ir = sqrt_ftz(iv);
     // error of y = |m| im: at most 4 kU et im from m, and relative 4 kU et / mt from the top, 3 kU
     // from the quotient, 1 from the product and 2 of second order
     const float e0 = 4.f * kU * im * et, ey = kU * (4.f * et * rcp_ftz(mt) + 6.f);
+    // y = (127 sqrt(|m| / top))^2 of a pair lies next to the borders b^2, b = floor(sqrt(y)) + 1/2,
+    // which split the codes b - 1/2 and b + 1/2; returns b, y - b^2 and the error of that
+    auto mean_border = [&](F2 m, F2& b, F2& d, F2& tol) {
+      float a0, a1, y0, y1;
+      m.split(a0, a1);
+      const F2 y = F2(fabsf(a0), fabsf(a1)) * F2(im);
+      y.split(y0, y1);
+      b = add_down(F2(sqrt_ftz(y0), sqrt_ftz(y1)), F2(8388608.f)) + F2(-8388607.5f);
+      float c0, c1;
+      b.split(c0, c1);
+      d = fma2(F2(-c0, -c1), b, y);                                       // b^2 is exact
+      tol = fma2(F2(ey), y, F2(e0));
+    };
+    // likewise b^4 and z = (255 sqrt(sqrt(v) / top))^4: relative 6 kU for v, 6 for the top, 4 for
+    // the quotient and its product, 2 for the border
+    auto root_border = [&](F2 v, F2& b, F2& d, F2& tol) {
+      float a0, a1, x0, x1;
+      v.split(a0, a1);
+      (F2(sqrt_ftz(a0), sqrt_ftz(a1)) * F2(ir)).split(x0, x1);
+      b = add_down(F2(sqrt_ftz(x0), sqrt_ftz(x1)), F2(8388608.f)) + F2(-8388607.5f);
+      const F2 r2 = b * b;
+      float s0, s1;
+      r2.split(s0, s1);
+      d = fma2(F2(-s0, -s1), r2, v * F2(iv));
+      tol = (r2 * F2(20.f * kU)) * r2;
+    };
+    bool near = false;             // an element of this lane lies next to a border
     uint32_t um[2], uv[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t qm[4], qv[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // y = (127 sqrt(|m| / top))^2 lies next to the border b^2, b = floor(sqrt(y)) + 1/2, which
-        // splits the codes b - 1/2 and b + 1/2
-        const float y = fabsf(m[h][k]) * im;
-        const float b = floor_small(sqrt_ftz(y)) + 0.5f;
-        const float d = y - b * b;                                        // b^2 is exact
-        if (fabsf(d) <= fmaf(ey, y, e0)) near |= 1u << (4 * h + k);
+      for (int j = 0; j < 2; ++j) {
+        F2 b, d, tol;
+        float b0, b1, d0, d1, t0, t1, s0, s1;
+        mean_border(m2[h][j], b, d, tol);
+        d.split(d0, d1);
+        tol.split(t0, t1);
+        m2[h][j].split(s0, s1);
+        near |= fabsf(d0) <= t0;
+        near |= fabsf(d1) <= t1;
+        (b + F2(copysignf(0.5f, d0), copysignf(0.5f, d1))).split(b0, b1);
         // the low byte of 1.5 2^23 + q is q's two's complement
-        qm[k] = __float_as_uint(copysignf(b + copysignf(0.5f, d), m[h][k]) + 12582912.f);
-        // likewise b^4 and z = (255 sqrt(sqrt(v) / top))^4: relative 6 kU for v, 6 for the top, 4
-        // for the quotient and its product, 2 for the border
-        const float z = v[h][k] * iv;
-        const float r = floor_small(sqrt_ftz(sqrt_ftz(v[h][k]) * ir)) + 0.5f;
-        const float r4 = (r * r) * (r * r);
-        const float f = z - r4;
-        if (fabsf(f) <= 20.f * kU * r4) near |= 256u << (4 * h + k);
-        qv[k] = __float_as_uint(r + copysignf(0.5f, f) + 8388608.f);
+        (F2(copysignf(b0, s0), copysignf(b1, s1)) + F2(12582912.f)).split(b0, b1);
+        qm[2 * j] = __float_as_uint(b0);
+        qm[2 * j + 1] = __float_as_uint(b1);
+        root_border(v2[h][j], b, d, tol);
+        d.split(d0, d1);
+        tol.split(t0, t1);
+        near |= fabsf(d0) <= t0;
+        near |= fabsf(d1) <= t1;
+        (b + F2(copysignf(0.5f, d0), copysignf(0.5f, d1)) + F2(8388608.f)).split(b0, b1);
+        qv[2 * j] = __float_as_uint(b0);
+        qv[2 * j + 1] = __float_as_uint(b1);
       }
       um[h] = pack4(qm);
-      uv[h] = __vmaxu4(pack4(qv), pos[h]);                                // a positive v keeps a code
+      uv[h] = pack4(qv);
+      if (((uv[h] - 0x01010101u) & ~uv[h] & 0x80808080u) != 0) {          // a code 0: a positive v keeps 1
+        float raw[4];                                    // the gradient before a scale that may underflow
+        load4<G>(t.g, i[h], nv[h], vec, raw);
+        const bool live = !a.grad_scale || *a.grad_scale != 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if ((uv[h] >> (8 * k) & 0xFFu) == 0 && ((raw[k] != 0.f && live) || (vq[h] >> (8 * k) & 0xFFu) != 0)) uv[h] |= 1u << (8 * k);
+      }
     }
     float msn = 0.f, vsn = 0.f;
     if (!(mok && vok)) {
@@ -442,12 +495,28 @@ __device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, 
         r1 = fma(fma(-r1, r1, top64), half, r1);
       }
       vsn = __shfl_sync(0xffffffffu, static_cast<float>(r1 * (1.0 / 65025.0)), 8);
-      if (__any_sync(0xffffffffu, near != 0)) {
+      if (__any_sync(0xffffffffu, near)) {
         // codes of the elements next to a border (a block in thirty has one) from fp64
         const double mt64 = __shfl_sync(0xffffffffu, top64, 0), vt64 = __shfl_sync(0xffffffffu, top64, 8);
-        while (near != 0) {
-          const int e = __ffs(static_cast<int>(near)) - 1, k = e & 3;
-          near &= near - 1;
+        uint32_t which = 0;                              // bits 0-7 for m, 8-15 for v
+        if (near) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            F2 b, d, tol;
+            float d0, d1, t0, t1;
+            mean_border(m2[e >> 1][e & 1], b, d, tol);
+            d.split(d0, d1);
+            tol.split(t0, t1);
+            which |= (fabsf(d0) <= t0 ? 1u << (2 * e) : 0u) | (fabsf(d1) <= t1 ? 2u << (2 * e) : 0u);
+            root_border(v2[e >> 1][e & 1], b, d, tol);
+            d.split(d0, d1);
+            tol.split(t0, t1);
+            which |= (fabsf(d0) <= t0 ? 256u << (2 * e) : 0u) | (fabsf(d1) <= t1 ? 512u << (2 * e) : 0u);
+          }
+        }
+        while (which != 0) {
+          const int e = __ffs(static_cast<int>(which)) - 1, k = e & 3;
+          which &= which - 1;
           const int64_t at = base + 128 * ((e >> 2) & 1) + 4 * lane + k;
           uint32_t q, clear = ~(0xFFu << (8 * k));
           if (e < 8) {
@@ -475,18 +544,17 @@ __device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, 
   }
 }
 
+// 8-bit states: four CTAs an SM (64 registers) took 628 us for a 7B set, three 739, five 840.
 template <int CAP, typename P, typename G, int BITS>
-__global__ void __launch_bounds__(kThreadsAW) k_adamw(const __grid_constant__ Args<CAP> a) {
+__global__ void __launch_bounds__(kThreadsAW, BITS == 8 ? 4 : 1) k_adamw(const __grid_constant__ Args<CAP> a) {
   const int ti = tensor_of(a, static_cast<int>(blockIdx.x));
   const Tensor& t = a.t[ti];
   const int lane = threadIdx.x & 31;
   const bool vec = a.vec[ti] != 0;
-  int64_t base = (static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.tile0[ti]) * a.tiles) * kTile +
-                 (threadIdx.x >> 5) * kBlock;
-  for (int j = 0; j < a.tiles && base < t.n; ++j, base += kTile) {     // uniform in the warp
-    if (vec && base + kBlock <= t.n) step_block<CAP, P, G, BITS, true>(a, t, base, lane, true);
-    else step_block<CAP, P, G, BITS, false>(a, t, base, lane, vec);
-  }
+  const int64_t base = static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.tile0[ti]) * kTile + (threadIdx.x >> 5) * kBlock;
+  if (base >= t.n) return;                         // the whole warp: no element of this block exists
+  if (vec && base + kBlock <= t.n) step_block<CAP, P, G, BITS, true>(a, t, base, lane, true);
+  else step_block<CAP, P, G, BITS, false>(a, t, base, lane, vec);
 }
 
 // The fp32 values that 8-bit codes stand for.

@@ -40,7 +40,8 @@ bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 constexpr int kSmall = 8, kLarge = 256;
 // Reading states back takes four tiles a CTA where that still fills the machine four times over
 // (289 -> 267 us for a 7B set: a tile is short against finding its tensor in the arguments).
-// The step does not: a second tile's loads would wait for the first (8-bit 634 -> 784 us).
+// The step does not: a second tile's loads would wait for the first (8-bit 634 -> 784 us; with
+// them issued ahead and three CTAs an SM for the registers, 688).
 constexpr int64_t kManyTiles = 148 * 4 * 4;
 
 template <int CAP>

@@ -27,6 +27,7 @@
 
 #include <type_traits>
 
+#include "dsmz_pairs.cuh"
 #include "dsmz_ptx.cuh"
 
 namespace dsmz {
@@ -119,24 +120,6 @@ template <> struct Vec<__nv_bfloat16> {
   __device__ static void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 };
 
-// Two fp32 in one register pair: the packed instructions halve the issue slots of everything but
-// the exponentials and the maximum (273 -> 260 us, with registers for a fifth CTA an SM).
-struct F2 {
-  uint64_t v;
-  __device__ __forceinline__ F2() {}
-  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ void split(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-  F2 c;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
-  return c;
-}
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-  F2 c;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v));
-  return c;
-}
 __device__ __forceinline__ F2 exp2_of(F2 a) {
   float x, y;
   a.split(x, y);
@@ -160,6 +143,7 @@ __device__ __forceinline__ void load_pairs(const __nv_bfloat16* p, F2 (&x)[4], f
   }
 }
 
+// The packed instructions (273 -> 260 us) leave registers for a fifth CTA an SM.
 // grid: ntok * cluster size; row = blockIdx.x / cluster size.
 template <typename T>
 __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t ld, int64_t V,
