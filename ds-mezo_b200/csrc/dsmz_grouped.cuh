@@ -119,10 +119,8 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* s
                "r"(x), "r"(y), "r"(z), "r"(smem_u32(src))
                : "memory");
 }
-__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// At most N of this thread's stores still read shared memory.
-template <int N>
-__device__ __forceinline__ void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+// No store of this thread reads shared memory any more.
+__device__ __forceinline__ void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
@@ -180,13 +178,16 @@ __device__ __forceinline__ void scan_groups(const int32_t* off, int G, int M, bo
   int carry = 0;
   for (int i0 = 0; i0 <= G; i0 += 32) {
     const int i = i0 + lane;
-    int v = i <= G ? min(max(off[i], 0), M) : 0;
+    int v = i <= G ? min(max(off[i], 0), M) : M;
+    const int before = __shfl_up_sync(0xffffffffu, v, 1);
+    if (!__all_sync(0xffffffffu, v >= (lane == 0 ? carry : before))) {       // not ascending
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v = max(v, u);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v = max(v, u);
+      }
+      v = max(v, carry);
     }
-    v = max(v, carry);
     if (i <= G) bnd[i + 1] = v;
     carry = __shfl_sync(0xffffffffu, v, 31);
   }
@@ -484,7 +485,6 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     const int row = q * 32 + lane;      // this thread's row of the tile
     const bool cols = col0 < a.bn;
     unsigned char* st = scratch + (warp - kFirstEpi) * a.sbuf * kStageBytes;
-    int flip = 0;                       // staging piece in use
     const int es = a.out_f32 ? 4 : 2;
     int u = 0;
     bool ok = true;
@@ -530,6 +530,10 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
       char* out = static_cast<char*>(a.out);
       if (MODE == 1) out += static_cast<int64_t>(x.seg) * a.gstride * es;
       const int nrows = min(32, x.valid - q * 32);             // this warp's rows that exist
+      if (a.alpha != 1.f) {
+#pragma unroll
+        for (int c = 0; c < CPW; ++c) acc[c] *= a.alpha;
+      }
       if (S > 1) {
         // Partial tiles [sender][column half][row][CPW]; 16-byte chunk j of row r lies at j ^ (r & 7),
         // so that neither writing a row a lane nor summing a chunk a lane meets bank conflicts.
@@ -571,7 +575,6 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
             const float4 w = *reinterpret_cast<const float4*>(part + p * H * rows * RB);
             v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
           }
-          v.x *= a.alpha; v.y *= a.alpha; v.z *= a.alpha; v.w *= a.alpha;
           if (a.transposed) {
             const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -590,77 +593,80 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
           const int nc = min(CPW, a.ndim - x.n0 - col0);
 #pragma unroll
           for (int c = 0; c < CPW; ++c) {
-            if (c < nc) *p = a.accumulate ? *p + a.alpha * acc[c] : a.alpha * acc[c];
+            if (c < nc) *p = a.accumulate ? *p + acc[c] : acc[c];
             p += a.ld;
           }
         }
       } else if (a.vec && !a.accumulate && a.ndim * es % 16 == 0) {
-        // pieces of 32 rows x 128 bytes; chunk j of row r lies at j ^ (r & 7), as the tensor map
-        // expects. A whole piece leaves by TMA; of a group's last rows eight lanes store each row.
+        // Pieces of 32 rows x 128 bytes; chunk j of row r lies at j ^ (r & 7), as the tensor map
+        // expects. a.sbuf of them are staged, fenced and sent together. A whole piece leaves by
+        // TMA; of a group's last rows eight lanes store each row.
         const bool whole = a.tma_out && (MODE == 1 || nrows == 32);
         char* base = out + (static_cast<int64_t>(x.m0 + q * 32) * a.ld + x.n0 + col0) * es;
-        auto piece = [&](int c0) {                        // the columns from c0 on are staged: send them
+        unsigned char* mine = st + lane * 128;
+        const int per = a.out_f32 ? 32 : 64;              // columns of a piece
+        auto send = [&](int p0, int p1) {                 // pieces [p0, p1) are staged: send them
           if (whole) {
             tc::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) tma_store_3d(&mapC, st + flip, x.n0 + col0 + c0, x.m0 + q * 32, MODE == 1 ? x.seg : 0);
+            if (lane == 0) {
+              for (int p = p0; p < p1; ++p)
+                tma_store_3d(&mapC, st + (p - p0) * kStageBytes, x.n0 + col0 + p * per, x.m0 + q * 32, MODE == 1 ? x.seg : 0);
+            }
           } else {
-            if (lane == 0) store_commit();                // an empty group: pieces and groups stay in step
             __syncwarp();
-            const int j = lane & 7, left = (a.ndim - x.n0 - col0 - c0) * es - 16 * j;
-            char* p = base + c0 * es + 16 * j + static_cast<int64_t>(lane >> 3) * a.ld * es;
+            const int j = lane & 7;
+            for (int p = p0; p < p1; ++p) {
+              const int left = (a.ndim - x.n0 - col0 - p * per) * es - 16 * j;
+              char* o = base + p * 128 + 16 * j + static_cast<int64_t>(lane >> 3) * a.ld * es;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 4 * i + (lane >> 3);
-              const uint4 v = *reinterpret_cast<const uint4*>(st + flip + r * 128 + ((j ^ (r & 7)) << 4));
-              if (r < nrows && left > 0) *reinterpret_cast<uint4*>(p) = v;
-              p += 4 * a.ld * es;
+              for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                const uint4 v = *reinterpret_cast<const uint4*>(st + (p - p0) * kStageBytes + r * 128 + ((j ^ (r & 7)) << 4));
+                if (r < nrows && left > 0) *reinterpret_cast<uint4*>(o) = v;
+                o += 4 * a.ld * es;
+              }
             }
           }
         };
-        auto ready = [&]() -> unsigned char* {             // a piece of staging whose last store has read it
-          flip = a.sbuf == 2 ? flip ^ kStageBytes : 0;
-          if (lane == 0) { if (a.sbuf == 2) store_read_wait<1>(); else store_read_wait<0>(); }
-          __syncwarp();
-          return st + flip + lane * 128;
-        };
-        if (!a.out_f32) {
+        const int np = min(CPW / per, (a.ndim - x.n0 - col0 + per - 1) / per);       // pieces with columns
+        int from = 0;                                     // first piece of the batch
 #pragma unroll
-          for (int c0 = 0; c0 < CPW; c0 += 64) {
-            if (x.n0 + col0 + c0 < a.ndim) {
-              unsigned char* mine = ready();
+        for (int p = 0; p < CPW / 32; ++p) {              // bf16 has half as many
+          if (p < np) {
+            if (p == from) {                              // the stores before have read the staging
+              if (lane == 0) store_read_wait();
+              __syncwarp();
+            }
+            unsigned char* to = mine + (p - from) * kStageBytes;
+            if (a.out_f32) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<float4*>(to + ((j ^ (lane & 7)) << 4)) =
+                    make_float4(acc[32 * p + 4 * j], acc[32 * p + 4 * j + 1], acc[32 * p + 4 * j + 2], acc[32 * p + 4 * j + 3]);
+            } else if (64 * p < CPW) {
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  const int c = c0 + 8 * j + 2 * i;
-                  const __nv_bfloat162 b2 = __floats2bfloat162_rn(a.alpha * acc[c], a.alpha * acc[c + 1]);
+                  const int c = (64 * p + 8 * j + 2 * i) % CPW;            // p < CPW / 64 here
+                  const __nv_bfloat162 b2 = __floats2bfloat162_rn(acc[c], acc[c + 1]);
                   w[i] = *reinterpret_cast<const uint32_t*>(&b2);
                 }
-                *reinterpret_cast<uint4*>(mine + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(to + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
               }
-              piece(c0);
             }
-          }
-        } else {
-#pragma unroll
-          for (int c0 = 0; c0 < CPW; c0 += 32) {
-            if (x.n0 + col0 + c0 < a.ndim) {
-              unsigned char* mine = ready();
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<float4*>(mine + ((j ^ (lane & 7)) << 4)) =
-                    make_float4(a.alpha * acc[c0 + 4 * j], a.alpha * acc[c0 + 4 * j + 1], a.alpha * acc[c0 + 4 * j + 2],
-                                a.alpha * acc[c0 + 4 * j + 3]);
-              piece(c0);
+            if (p + 1 - from == a.sbuf || p + 1 == np) {
+              send(from, p + 1);
+              from = p + 1;
             }
           }
         }
       } else {
         // odd pitches and accumulation: 16 fp32 columns at a time through the staging, four lanes a row
         char* base = out + static_cast<int64_t>(x.m0 + q * 32) * a.ld * es;
-        if (lane == 0) store_read_wait<0>();
+        if (lane == 0) store_read_wait();
         __syncwarp();
 #pragma unroll
         for (int c0 = 0; c0 < CPW; c0 += 16) {
@@ -668,8 +674,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               *reinterpret_cast<float4*>(st + lane * kStagePitch + j * 16) =
-                  make_float4(a.alpha * acc[c0 + 4 * j], a.alpha * acc[c0 + 4 * j + 1], a.alpha * acc[c0 + 4 * j + 2],
-                              a.alpha * acc[c0 + 4 * j + 3]);
+                  make_float4(acc[c0 + 4 * j], acc[c0 + 4 * j + 1], acc[c0 + 4 * j + 2], acc[c0 + 4 * j + 3]);
             __syncwarp();
             const int n = x.n0 + col0 + c0 + (lane & 3) * 4;
 #pragma unroll
