@@ -18,7 +18,7 @@
 // formed again in fp64. A 7B set (161.5 M elements; bf16 gradients and shadow, 16 bytes an
 // element, 394 us at the measured copy rate) took 1634 us with everything in fp64, 1376 in
 // fp32 with blocks near a border done again whole, 723 with single elements done again, no
-// conversions and a path without bounds for whole blocks, 590 with packed arithmetic. What
+// conversions and a path without bounds for whole blocks, 608 with packed arithmetic. What
 // bounds it is instruction issue and latency: 84 instructions an element, 32 warps an SM.
 // A block with a NaN or an infinity gets a scale that makes every element of the block NaN: the
 // whole block, not one element.
@@ -462,8 +462,8 @@ __device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, 
       // The scales come from the largest values in fp64. Lanes whose largest could be it in spite
       // of the roundings (nearly always one): their eight elements are formed again, side by side
       // on eight lanes, lanes 0-7 for m and 8-15 for v.
-      uint32_t cand_m = __ballot_sync(0xffffffffu, __uint_as_float(mtb) >= mt - 8.f * kU * et);
-      uint32_t cand_v = __ballot_sync(0xffffffffu, __uint_as_float(vtb) >= vt * (1.f - 16.f * kU));
+      uint32_t cand_m = __ballot_sync(0xffffffffu, mt > 0.f && __uint_as_float(mtb) >= mt - 8.f * kU * et);
+      uint32_t cand_v = __ballot_sync(0xffffffffu, vt > 0.f && __uint_as_float(vtb) >= vt * (1.f - 16.f * kU));
       const double gs64 = a.grad_scale ? static_cast<double>(*a.grad_scale) : 1.0;
       auto grad_at = [&](int64_t at) {
         return sizeof(G) == 4 ? reinterpret_cast<const float*>(t.g)[at]
@@ -476,15 +476,30 @@ __device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, 
         return root64(reinterpret_cast<const uint8_t*>(t.v)[at], vs, grad_at(at), gs64, a.b2, a.omb2);
       };
       double top64 = 0.0;
-      while ((cand_m | cand_v) != 0) {
-        const int src = __ffs(static_cast<int>((lane & 8) ? cand_v : cand_m)) - 1;
-        const int64_t at = base + 128 * ((lane >> 2) & 1) + 4 * src + (lane & 3);
-        if (src >= 0 && lane < 16 && (FULL || at < t.n)) top64 = fmax(top64, (lane & 8) ? v64_at(at) : fabs(m64_at(at)));
-        cand_m &= cand_m - 1;
-        cand_v &= cand_v - 1;
-      }
+      if (__popc(cand_m) + __popc(cand_v) <= 8) {
+        while ((cand_m | cand_v) != 0) {
+          const int src = __ffs(static_cast<int>((lane & 8) ? cand_v : cand_m)) - 1;
+          const int64_t at = base + 128 * ((lane >> 2) & 1) + 4 * src + (lane & 3);
+          if (src >= 0 && lane < 16 && (FULL || at < t.n)) top64 = fmax(top64, (lane & 8) ? v64_at(at) : fabs(m64_at(at)));
+          cand_m &= cand_m - 1;
+          cand_v &= cand_v - 1;
+        }
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) top64 = fmax(top64, __shfl_xor_sync(0xffffffffu, top64, o));
+        for (int o = 4; o > 0; o >>= 1) top64 = fmax(top64, __shfl_xor_sync(0xffffffffu, top64, o));
+      } else {                                           // many equal values: every element again
+        double m64 = 0.0, v64 = 0.0;
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const int64_t at = base + 128 * (e >> 2) + 4 * lane + (e & 3);
+          if (FULL || at < t.n) {
+            m64 = fmax(m64, fabs(m64_at(at)));
+            v64 = fmax(v64, v64_at(at));
+          }
+        }
+        m64 = warp_top(m64);
+        v64 = warp_top(v64);
+        top64 = (lane & 8) ? v64 : m64;
+      }
       msn = static_cast<float>(top64 * (1.0 / 16129.0));                  // lanes 0-7
       // lanes 8-15: two Newton steps take the fp32 root (2^-23) to fp64's last bits
       const float r0 = sqrt_ftz(static_cast<float>(top64));

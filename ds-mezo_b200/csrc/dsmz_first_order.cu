@@ -152,19 +152,9 @@ int adamw_run(const dsmz_adamw_desc& d, const dsmz_adamw_tensor* tensors, int32_
 __device__ int g_wait_err;
 
 int wait_err(int** p) {
-  static thread_local int* addr = nullptr;
-  static thread_local int addr_dev = -1;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && dev != addr_dev) {
-    void* q = nullptr;
-    e = cudaGetSymbolAddress(&q, g_wait_err);
-    if (e == cudaSuccess) {
-      addr = static_cast<int*>(q);
-      addr_dev = dev;
-    }
-  }
-  *p = addr;
+  void* q = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&q, g_wait_err);
+  *p = static_cast<int*>(q);
   return e == cudaSuccess ? 0 : cuda_fail("error word", e);
 }
 

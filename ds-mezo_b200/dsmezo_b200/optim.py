@@ -119,6 +119,7 @@ class AdamW:
                 e.shadow = sh.data_ptr()
         self._desc = AdamWDesc(param_dtype=_DT[p0.dtype], state_bits=self.state_bits, beta1=b1, beta2=b2,
                                eps=self.eps, weight_decay=self.weight_decay)
+        self._pointers = [p.data_ptr() for p in self.params]
         self.step_count = int(step)              # steps taken (host count; not moved when capturable)
         self.step_counter = torch.full((1,), int(step), dtype=torch.int64, device=self.device) if capturable else None
         self.grads = None
@@ -180,6 +181,8 @@ class AdamW:
             self.grads = None                    # a later step() must be given its own again
         elif self.grads is None:
             raise ValueError("AdamW: no gradients bound; give them to step()")
+        if [p.data_ptr() for p in self.params] != self._pointers:
+            raise RuntimeError("AdamW: a parameter's memory has been replaced since it was bound")
         d = self._desc
         if self.step_counter is None and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: a captured step would repeat one step number at every replay; "

@@ -207,6 +207,27 @@ def test_8_bit_states_over_the_whole_range(O):
     assert bool(((s.v_scale.double().cpu() - sv).abs() <= 2 * U * sv + 1e-45).all())
 
 
+@pytest.mark.parametrize("n", [256, 1000])
+def test_blocks_of_equal_values(O, n):
+    # every element can be the largest: constant and alternating gradients over several steps
+    for g in (torch.full((n,), 0.37, device=DEV), 0.01 * (1.0 - 2.0 * (torch.arange(n, device=DEV) % 2))):
+        p = torch.randn(n, generator=torch.Generator(device=DEV).manual_seed(n), device=DEV)
+        opt = O.AdamW([p], LR, (B1, B2), EPS, WD, grads=[g], state_bits=8)
+        for t in range(1, 5):
+            p0, (m, v) = p.clone(), decode(opt.states[0], n)
+            opt.step()
+            check_step(p0, g, m, v, t, p, opt.states[0])
+
+
+def test_replaced_parameter_is_refused(O):
+    p, g = torch.zeros(8, device=DEV), torch.ones(8, device=DEV)
+    opt = O.AdamW([p], grads=[g])
+    opt.step()
+    p.data = torch.zeros(8, device=DEV)
+    with pytest.raises(RuntimeError, match="replaced"):
+        opt.step()
+
+
 def test_state_values(O):
     for n in (1, 256, 1000):
         p, g, s = make(n, torch.float32, torch.float32, 8, n, O)

@@ -174,6 +174,21 @@ def test_weight_gradients(Gr, M, G, K, N):
         check_grad(x, dy, edges, acc, old, 0.25)
 
 
+@pytest.mark.parametrize("tiles", [1, 12, 16, 20, 24, 30, 36, 50, 76, 150])
+@pytest.mark.parametrize("N", [48, 128])
+def test_every_way_to_split(Gr, tiles, N):
+    # clusters of 8 down to 2 and none: as many row (or feature) tiles as each can hold, the last
+    # one ragged, and contractions that do not divide
+    M, K = 128 * tiles - 37, 64 * 17 + 8
+    x, w = rnd((M, K), 41), rnd((1, K, N), 42, K ** -0.5)
+    for dt in (torch.bfloat16, torch.float32):
+        check_product(x, w, [0, M], Gr.grouped_matmul(x, w, offs([0, M]), out_dtype=dt))
+    wide, rows = 128 * tiles - 24, 1100
+    a, b = rnd((rows, wide), 43), rnd((rows, N), 44)
+    for u, v in ((a, b), (b, a)):
+        check_grad(u, v, [0, rows], Gr.grouped_weight_grad(u, v, offs([0, rows])))
+
+
 def test_no_rows(Gr):
     w = rnd((3, 16, 24), 22)
     assert Gr.grouped_matmul(rnd((0, 16), 1), w, offs([0, 0, 0, 0])).shape == (0, 24)
