@@ -230,12 +230,14 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
   cfg.blockDim = dim3(gr::kThreadsG);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = static_cast<unsigned>(a.split);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = static_cast<unsigned>(a.split);
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  cfg.numAttrs = a.split > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, kernel, A, B, C, a, err);
   return e == cudaSuccess ? DSMZ_OK : cuda_fail(what, e);
 }
@@ -332,9 +334,12 @@ int loss_grad(const void* logits, int64_t V, int64_t ld, const int32_t* targets,
   e = cudaLaunchKernelEx(&cfg, sg::k_loss_grad<T>, static_cast<const T*>(logits), ld, V, targets, q, grad_scale,
                          static_cast<T*>(grad), ld_grad, term);
   if (e != cudaSuccess) return cuda_fail("dsmz_contrastive_loss_grad: rows", e);
-  sg::k_loss_sum<<<1, 256, 0, s>>>(term, ntok, loss);
-  DSMZ_LAUNCHED("dsmz_contrastive_loss_grad: sum");
-  return DSMZ_OK;
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(256);
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  e = cudaLaunchKernelEx(&cfg, sg::k_loss_sum, static_cast<const double*>(term), ntok, loss);
+  return e == cudaSuccess ? DSMZ_OK : cuda_fail("dsmz_contrastive_loss_grad: sum", e);
 }
 
 }  // namespace

@@ -346,7 +346,9 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
   const int rank = S > 1 ? static_cast<int>(blockIdx.x) % S : 0;
   const int first = static_cast<int>(blockIdx.x) / S, step = static_cast<int>(gridDim.x) / S;
 
+  launch_dependents();
   if (warp == 2) {
+    grid_dependency_wait();
     scan_groups(a.offsets, a.G, static_cast<int>(a.M), a.zero_rest != 0, bnd, tile0, lane);
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
@@ -367,6 +369,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     if (a.tma_out) prefetch_map(&mapC);
   }
   __syncwarp();
+  grid_dependency_wait();               // nothing above reads or writes global memory but the scan, after its own
   tc::tc_fence_before();
   if (S > 1) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
   tc::tc_fence_after();

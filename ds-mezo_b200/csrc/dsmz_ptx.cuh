@@ -173,6 +173,13 @@ __device__ __forceinline__ bool spin_geq(const int* p, int target, int* err) {
   }
 }
 
+// Programmatic dependent launch. A kernel launched with the attribute may start while the one
+// before it in the stream still runs: grid_dependency_wait() returns once that kernel has
+// completed and its writes are visible (at once without the attribute), and must come before
+// any access to global memory. launch_dependents() lets the next kernel start its own prologue.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Barrier over the `n` threads of the consumer warps (id 1; warp-multiple n).
 __device__ __forceinline__ void named_sync(int id, int n) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");

@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
   constexpr int N = Vec<T>::N;
   __shared__ float2 red[8];
   __shared__ float2 part[8];                          // (max, sum) of every CTA of the cluster
+  launch_dependents();                                // the sum's launch overlaps the rows
   const int tid = threadIdx.x, nt = blockDim.x;
   const uint32_t C = cluster_size(), rank = cluster_rank();
   const int64_t row = blockIdx.x / C;
@@ -279,6 +280,7 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
 __global__ void __launch_bounds__(256) k_loss_sum(const double* __restrict__ term, int64_t ntok, float* loss) {
   __shared__ double part[256];
   const int tid = threadIdx.x;
+  grid_dependency_wait();
   const int64_t per = (ntok + 255) / 256;
   double a = 0.0;
   for (int64_t i = tid * per; i < min(ntok, (tid + 1) * per); ++i) a += term[i];
