@@ -195,13 +195,13 @@ int sm_count(int* sms) {
 }
 
 // Shared memory of a launch; sets a.sbuf and a.stages.
-template <int BNT, int MODE>
+template <int BNT, int MODE, bool PAIR>
 size_t grouped_smem(gr::Args& a, int64_t nk) {
-  constexpr int SB = gr::kABytes + BNT * gr::kBK * 2;
+  constexpr int SB = gr::kABytes + (PAIR ? BNT / 2 : BNT) * gr::kBK * 2;
   constexpr int kSmem = 227 * 1024;
   // two staging pieces a warp let a store run while the next piece is staged; the widest tile
   // gives a stage of the ring for them, which pays where a tile has only a few k-steps
-  a.sbuf = BNT < 256 || nk <= 4 ? 2 : 1;
+  a.sbuf = BNT < 256 || PAIR || nk <= 4 ? 2 : 1;
   const int scratch = a.split > 1 ? gr::split_bytes(a.split, BNT) : gr::kEpiWarps * gr::kStageBytes * a.sbuf;
   const int fixed = 1024 + scratch + (((a.G + 3) * 8 + 15) & ~15) + 64 + 16 * 8;
   a.stages = (kSmem - fixed) / SB;
@@ -209,11 +209,11 @@ size_t grouped_smem(gr::Args& a, int64_t nk) {
   return static_cast<size_t>(fixed) + static_cast<size_t>(a.stages) * SB;
 }
 
-template <int BNT, int MODE>
+template <int BNT, int MODE, bool PAIR = false>
 int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, int64_t tiles, int64_t nk,
                    int sms, const char* what, cudaStream_t s) {
-  const size_t smem = grouped_smem<BNT, MODE>(a, nk);
-  auto* kernel = gr::k_grouped<BNT, MODE>;
+  const size_t smem = grouped_smem<BNT, MODE, PAIR>(a, nk);
+  auto* kernel = gr::k_grouped<BNT, MODE, PAIR>;
   int* err = nullptr;
   int rc = wait_err(&err);
   if (rc) return rc;
@@ -226,7 +226,10 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
   }
   if (e != cudaSuccess) return cuda_fail(what, e);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.split > 1 ? tiles * a.split : (tiles < sms ? tiles : sms)));
+  const int cluster = PAIR ? 2 : a.split;
+  const int64_t wave = sms / 2;                          // pairs: one a TPC
+  cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * (tiles < wave ? tiles : wave)
+                                                : (a.split > 1 ? tiles * a.split : (tiles < sms ? tiles : sms))));
   cfg.blockDim = dim3(gr::kThreadsG);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -234,10 +237,10 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = static_cast<unsigned>(a.split);
+  at[1].val.clusterDim.x = static_cast<unsigned>(cluster);
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = a.split > 1 ? 2 : 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, kernel, A, B, C, a, err);
   return e == cudaSuccess ? DSMZ_OK : cuda_fail(what, e);
 }
@@ -276,7 +279,7 @@ int active_clusters(int s) {
       at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
       cfg.attrs = at;
       cfg.numAttrs = 1;
-      auto* kernel = gr::k_grouped<128, 0>;
+      auto* kernel = gr::k_grouped<128, 0, false>;
       int n = 0;
       if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
           cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
@@ -395,9 +398,15 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     a.ntn = static_cast<int32_t>((N + a.bn - 1) / a.bn);
     const int64_t nk = (K + gr::kBK - 1) / gr::kBK;
     a.split = split_for(bnt, rows * a.ntn, nk);
+    // Pairs of CTAs where the products, not the output, take a tile's time and the groups are long
+    // enough for 256-row tiles. 8192 x 3584 x 18944 in 8 ragged groups (9% of the tiles' rows are
+    // empty, 5% with 128-row tiles): 826 us with pairs and 856 without in a short run, 1014 and
+    // 1078 under the power cap.
+    const bool pair = bnt == 256 && N >= 256 && K >= 512 && M / G >= 512 && rows / 2 * a.ntn >= sms / 2;
     // short groups: boxes of 32 rows, so that a tile does not fetch 128
     a.arows = M / G >= 96 ? gr::kBM : 32;
     const int64_t tiles = (rows + 2) * a.ntn;                                    // and the rows outside the groups
+    const uint32_t bcols = static_cast<uint32_t>(pair ? a.bn / 2 : a.bn);        // columns of a CTA's box of W
     if (tiles > (1 << 27)) return fail(DSMZ_ERR_UNSUPPORTED, me + "too many tiles");
     CUtensorMap A, B, C{};
     const uint64_t da[2] = {static_cast<uint64_t>(K), static_cast<uint64_t>(M)}, sa[1] = {static_cast<uint64_t>(ld_x) * 2};
@@ -408,14 +417,15 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     const uint64_t ss[3] = {pitch, 128, group};
     a.b_slabs = w_n_contiguous && N % 64 == 0;
     if (!encode_map(&A, x, 2, da, sa, gr::kBK, static_cast<uint32_t>(a.arows)) ||
-        !(a.b_slabs ? encode_map(&B, w, 4, ds, ss, 64, 64, false, static_cast<uint32_t>((a.bn + 63) / 64))
-                    : encode_map(&B, w, 3, db, sb, 64, w_n_contiguous ? 64 : static_cast<uint32_t>(a.bn))))
+        !(a.b_slabs ? encode_map(&B, w, 4, ds, ss, 64, 64, false, (bcols + 63) / 64)
+                    : encode_map(&B, w, 3, db, sb, 64, w_n_contiguous ? 64 : bcols)))
       return fail(DSMZ_ERR_CUDA, me + "the driver refused a tensor map");
     if (a.vec && !a.accumulate && a.split == 1) {
       const uint64_t dc[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M), 1};
       const uint64_t sc[2] = {static_cast<uint64_t>(ld_out) * es, static_cast<uint64_t>(ld_out) * es * M};
       a.tma_out = encode_map(&C, out, 3, dc, sc, 128 / es, 32, a.out_f32 != 0);
     }
+    if (pair) return launch_grouped<256, 0, true>(a, A, B, C, tiles, nk, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
     return launch_grouped_bn<0>(bnt, a, A, B, C, tiles, nk, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
   });
 }

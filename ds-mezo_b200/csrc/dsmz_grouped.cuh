@@ -31,7 +31,8 @@
 // results are the same on every run.
 //
 // What bounds it, on one B200 (floors at the measured copy and bf16 rates):
-//   8192 x 3584 x 18944, 8 groups     848 us of 664 (802 at the sustained rate): the power cap
+//   8192 x 3584 x 18944, 8 groups     826 us of 664 (1014 of 802 sustained): the power cap and
+//                                     the empty rows of ragged last tiles
 //   4001 x 64 x 18944, 32 ragged      56 us of 36: the epilogue of half-filled last tiles, 5 us
 //                                     until the first tile is stored
 //   4133 x 28672 x 128, 4 groups      54 us of 40: 36 tiles in clusters of 3 leave 40 SMs idle,
@@ -155,6 +156,32 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
   return p != 0;
 }
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// TMA loads into this CTA's shared memory that complete on a barrier of the pair's leader (a
+// shared::cluster address); no multicast.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(m), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
 // Bounded wait with cluster-scope acquire (arrivals come from other CTAs).
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
   const uint64_t t0 = gtimer();
@@ -182,7 +209,8 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
 
 // Row boundaries bnd[0..G+2] = 0, the offsets (clamped to [0, M], running maximum), M; segment
 // s = rows [bnd[s], bnd[s+1]): 1..G are the groups, 0 and G+1 the rows outside them. tile0[s] =
-// 128-row tiles before segment s (0 and G+1 have none unless they are zeroed). One warp.
+// tiles of bm rows before segment s (0 and G+1 have none unless they are zeroed). One warp.
+template <int BM>
 __device__ __forceinline__ void scan_groups(const int32_t* off, int G, int M, bool rest, int32_t* bnd, int32_t* tile0,
                                             int lane) {
   int carry = 0;
@@ -207,7 +235,7 @@ __device__ __forceinline__ void scan_groups(const int32_t* off, int G, int M, bo
   for (int s0 = 0; s0 < G + 2; s0 += 32) {
     const int s = s0 + lane;
     int n = 0;
-    if (s < G + 2 && (rest || (s >= 1 && s <= G))) n = (bnd[s + 1] - bnd[s] + kBM - 1) / kBM;
+    if (s < G + 2 && (rest || (s >= 1 && s <= G))) n = (bnd[s + 1] - bnd[s] + BM - 1) / BM;
     int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -237,8 +265,8 @@ __device__ __forceinline__ int fast_div(int i, int d, float inv) {
   return q;
 }
 
-// Walks a CTA's tiles t, t + step, ... in ascending order.
-template <int MODE>
+// Walks a CTA's tiles t, t + step, ... in ascending order; BM rows a tile (MODE 0).
+template <int MODE, int BM>
 struct Cursor {
   int lo;                               // MODE 0: segment of the last tile found
   float inv_ntn, inv_mtn, inv_per;
@@ -257,9 +285,9 @@ struct Cursor {
       int nt, mt;
       if (a.n_inner) { mt = fast_div(local, a.ntn, inv_ntn); nt = local - mt * a.ntn; } else { nt = local / nm; mt = local - nt * nm; }
       x.seg = lo;
-      x.m0 = bnd[lo] + mt * kBM;
+      x.m0 = bnd[lo] + mt * BM;
       x.n0 = nt * a.bn;
-      x.valid = min(kBM, bnd[lo + 1] - x.m0);
+      x.valid = min(BM, bnd[lo + 1] - x.m0);
       x.r0 = x.cnt = 0;
       x.nk = (lo >= 1 && lo <= a.G) ? (a.kdim + kBK - 1) / kBK : 0;
     } else {
@@ -317,7 +345,11 @@ __device__ __forceinline__ void put1(const Args& a, char* base, int64_t i, float
 
 // BNT: columns of the accumulators (64, 128 or 256; a.bn <= BNT). mapC: the output (3-D, boxes
 // of 32 rows x 128 bytes) where a.tma_out.
-template <int BNT, int MODE>
+// PAIR (MODE 0, BNT 256): a cluster of two CTAs computes 256 x 256 tiles with cta_group::2 MMAs.
+// Each loads its 128 rows of A and 128 of B's rows, so a k-step costs 32 KB a CTA instead of 48;
+// the CTA of rank 0 (the leader) waits for both CTAs' loads on its barriers and issues, each CTA's
+// epilogue drains its own half.
+template <int BNT, int MODE, bool PAIR>
 __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant__ CUtensorMap mapA,
                                                          const __grid_constant__ CUtensorMap mapB,
                                                          const __grid_constant__ CUtensorMap mapC,
@@ -325,7 +357,8 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
   // columns of an epilogue warp: half a tile, or all of a narrow one whose rows may leave as
   // 128 bytes of bf16
   constexpr int CPW = BNT == 64 && MODE == 0 ? 64 : BNT / 2;
-  constexpr int SB = kABytes + BNT * kBK * 2;
+  constexpr int SB = kABytes + (PAIR ? BNT / 2 : BNT) * kBK * 2;
+  constexpr int BM = PAIR ? 2 * kBM : kBM;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int S = a.split, stages = a.stages;
@@ -343,20 +376,27 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_full + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kCols = 2 * BNT;        // TMEM columns: two accumulators
-  const int rank = S > 1 ? static_cast<int>(blockIdx.x) % S : 0;
-  const int first = static_cast<int>(blockIdx.x) / S, step = static_cast<int>(gridDim.x) / S;
+  const int rank = PAIR ? static_cast<int>(blockIdx.x) & 1 : (S > 1 ? static_cast<int>(blockIdx.x) % S : 0);
+  const int C = PAIR ? 2 : S;           // CTAs of a cluster
+  const int first = static_cast<int>(blockIdx.x) / C, step = static_cast<int>(gridDim.x) / C;
 
   launch_dependents();
   if (warp == 2) {
     grid_dependency_wait();
-    scan_groups(a.offsets, a.G, static_cast<int>(a.M), a.zero_rest != 0, bnd, tile0, lane);
+    scan_groups<BM>(a.offsets, a.G, static_cast<int>(a.M), a.zero_rest != 0, bnd, tile0, lane);
   } else if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   } else if (warp == 0 && lane == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(full + s, 2); mbar_init(empty + s, 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, kEpiWarps); }
+    for (int b = 0; b < 2; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, (PAIR ? 2 : 1) * kEpiWarps); }
     mbar_init(red_full, 1);
     mbar_init_fence();
     if (S > 1) {                        // the partial tiles of this CTA's rows, from each of the S CTAs
@@ -371,12 +411,13 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
   __syncwarp();
   grid_dependency_wait();               // nothing above reads or writes global memory but the scan, after its own
   tc::tc_fence_before();
-  if (S > 1) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
+  if (C > 1) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int total = MODE == 0 ? tile0[a.G + 2] * a.ntn : a.G * a.mtn * a.ntn;
   const bool b_mn = MODE == 1 || a.b_mn != 0;
-  const int nbox_b = b_mn ? (a.bn + 63) / 64 : 1;
+  const int bnc = PAIR ? a.bn / 2 : a.bn;                     // columns of B that this CTA loads
+  const int nbox_b = b_mn ? (bnc + 63) / 64 : 1;
   auto k_begin = [&](int nk) { return S == 1 ? 0 : nk * rank / S; };
   auto k_end = [&](int nk) { return S == 1 ? nk : nk * (rank + 1) / S; };
 
@@ -386,22 +427,41 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     int s = 0, n = 0;                   // stage, k-steps issued
     uint32_t ph = 1;                    // parity of the wait for an empty stage (the first round passes)
     bool ok = true;
-    Cursor<MODE> cur(a);
+    Cursor<MODE, BM> cur(a);
     for (int t = first; t < total && ok; t += step) {
       const Tile y = cur.at(a, bnd, tile0, t);
       const int nk = __shfl_sync(0xffffffffu, y.nk, 0), m0 = __shfl_sync(0xffffffffu, y.m0, 0);
       const int n0 = __shfl_sync(0xffffffffu, y.n0, 0), seg = __shfl_sync(0xffffffffu, y.seg, 0);
       const int r0 = __shfl_sync(0xffffffffu, y.r0, 0), valid = __shfl_sync(0xffffffffu, y.valid, 0);
-      const int nba = MODE == 0 ? (valid + a.arows - 1) / a.arows : 2;
-      const uint32_t bytes = !is_a ? (b_mn ? static_cast<uint32_t>(nbox_b * 8192) : static_cast<uint32_t>(a.bn * 128))
-                                   : (MODE == 0 ? static_cast<uint32_t>(nba * a.arows * 128) : 16384u);
+      // rows of A that this CTA loads, in boxes of arows, and those of the pair's other CTA
+      const int rows_a = PAIR ? min(max(valid - kBM * rank, 0), kBM) : valid;
+      const int rows_p = PAIR ? min(max(valid - kBM * (1 - rank), 0), kBM) : 0;
+      const int nba = MODE == 0 ? (rows_a + a.arows - 1) / a.arows : 2;
+      const int nbp = PAIR ? (rows_p + a.arows - 1) / a.arows : 0;
+      // bytes that complete on the barrier: both CTAs' where a pair shares the leader's
+      const uint32_t bytes = !is_a ? (b_mn ? static_cast<uint32_t>(nbox_b * 8192) : static_cast<uint32_t>(bnc * 128)) * (PAIR ? 2u : 1u)
+                                   : (MODE == 0 ? static_cast<uint32_t>((nba + nbp) * a.arows * 128) : 16384u);
       const int ke = k_end(nk);
       for (int k = k_begin(nk); k < ke; ++k) {
         ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ph, err));
         if (!ok) break;
         unsigned char* dst = smem + s * SB + (is_a ? 0 : kABytes);
         uint64_t* bar = full + s;
-        if (elect_one()) {
+        if (PAIR) {
+          if (elect_one()) {
+            if (rank == 0) mbar_expect_tx(bar, bytes);
+            const uint32_t lead = map_rank(smem_u32(bar), 0);
+            if (is_a) {
+              for (int i = 0; i < nba; ++i)
+                tma_load_2d_pair(dst + i * a.arows * 128, &mapA, k * kBK, m0 + kBM * rank + i * a.arows, lead);
+            } else if (b_mn) {
+              if (a.b_slabs) tma_load_4d_pair(dst, &mapB, 0, k * kBK, (n0 + bnc * rank) >> 6, seg - 1, lead);
+              else for (int j = 0; j < nbox_b; ++j) tma_load_3d_pair(dst + j * 8192, &mapB, n0 + bnc * rank + 64 * j, k * kBK, seg - 1, lead);
+            } else {
+              tma_load_3d_pair(dst, &mapB, k * kBK, n0 + bnc * rank, seg - 1, lead);
+            }
+          }
+        } else if (elect_one()) {
           mbar_expect_tx(bar, bytes);
           if (MODE == 0) {
             if (is_a) {
@@ -433,14 +493,17 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
         if (++s == stages) { s = 0; ph ^= 1u; }
       }
     }
-    // on an error: let the loads already issued land before the CTA can exit
-    if (!ok)
+    // on an error: let the loads already issued land before the CTA can exit (a pair's complete on
+    // the leader, and neither CTA leaves before the other)
+    if (!ok && rank * (PAIR ? 1 : 0) == 0)
       for (int i = (n > stages ? n - stages : 0); i < n; ++i)
         mbar_drain(full + (i % stages), static_cast<uint32_t>(i / stages) & 1u);
+  } else if (warp == 1 && PAIR && rank != 0) {
+    // the leader issues for both
   } else if (warp == 1) {
     // The whole warp walks the loop, with every branch on a vote or a broadcast, so that stages
     // and descriptors stay in uniform registers; one elected lane issues.
-    const uint32_t idesc = tc::idesc_bf16(a.bn, MODE, b_mn ? 1 : 0);
+    const uint32_t idesc = PAIR ? tc::idesc_bf16_pair(a.bn, b_mn ? 1 : 0) : tc::idesc_bf16(a.bn, MODE, b_mn ? 1 : 0);
     // descriptors of stage 0; addresses advance in units of 16 bytes
     const uint64_t a0 = MODE == 0 ? tc::sdesc(smem_u32(smem), 16, 1024) : tc::sdesc(smem_u32(smem), 8192, 1024);
     const uint64_t b0 = b_mn ? tc::sdesc(smem_u32(smem) + kABytes, 8192, 1024) : tc::sdesc(smem_u32(smem) + kABytes, 16, 1024);
@@ -448,14 +511,17 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     int s = 0, u = 0, last = -1;        // stage, accumulators begun, the last one committed
     uint32_t ph = 0;
     bool ok = true;
-    Cursor<MODE> cur(a);
+    Cursor<MODE, BM> cur(a);
     for (int t = first; t < total && ok; t += step) {
       const Tile x = cur.at(a, bnd, tile0, t);
       const int nk = __shfl_sync(0xffffffffu, x.nk, 0), cnt = __shfl_sync(0xffffffffu, x.cnt, 0);
       const int kb = k_begin(nk), ke = k_end(nk);
       for (int c = kb; c < ke && ok; c += a.chunk, ++u) {
         const int b = u & 1;
-        if (u >= 2) ok = __all_sync(0xffffffffu, mbar_wait(tempty + b, static_cast<uint32_t>((u >> 1) - 1) & 1u, err));
+        if (u >= 2) {
+          const uint32_t par = static_cast<uint32_t>((u >> 1) - 1) & 1u;
+          ok = __all_sync(0xffffffffu, PAIR ? mbar_wait_cluster(tempty + b, par, err) : mbar_wait(tempty + b, par, err));
+        }
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t acc = tmem + static_cast<uint32_t>(b * BNT);
@@ -478,7 +544,14 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
             __syncwarp();
           }
           tc::tc_fence_after();
-          if (elect_one()) {
+          if (PAIR) {
+            if (elect_one()) {
+              tc::mma_bf16_pair(acc, da, db, idesc, more);
+#pragma unroll
+              for (int kk = 1; kk < kBK / 16; ++kk) tc::mma_bf16_pair(acc, da + kk * ka, db + kk * kb_, idesc, 1u);
+              tc::mma_commit_pair(empty + s);
+            }
+          } else if (elect_one()) {
             tc::mma_bf16(acc, da, db, idesc, more);
 #pragma unroll
             for (int kk = 1; kk < kBK / 16; ++kk)
@@ -487,7 +560,9 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
           }
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
-        if (elect_one()) tc::mma_commit(tfull + b);    // on an error too: it completes once the issued MMAs have
+        if (elect_one()) {                             // on an error too: it completes once the issued MMAs have
+          if (PAIR) tc::mma_commit_pair(tfull + b); else tc::mma_commit(tfull + b);
+        }
         last = u;
       }
     }
@@ -501,9 +576,13 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     const int es = a.out_f32 ? 4 : 2;
     int u = 0;
     bool ok = true;
-    Cursor<MODE> cur(a);
+    Cursor<MODE, BM> cur(a);
     for (int t = first; t < total && ok; t += step) {
-      const Tile x = cur.at(a, bnd, tile0, t);
+      Tile x = cur.at(a, bnd, tile0, t);
+      if (PAIR) {                       // this CTA's half of the rows
+        x.m0 += kBM * rank;
+        x.valid = min(max(x.valid - kBM * rank, 0), kBM);
+      }
       const int kb = k_begin(x.nk), ke = k_end(x.nk);
       float acc[CPW];
       if (kb >= ke) {
@@ -537,7 +616,9 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
         }
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty + b);
+        if (lane == 0) {
+          if (PAIR) arrive_remote(map_rank(smem_u32(tempty + b), 0)); else mbar_arrive(tempty + b);
+        }
       }
       if (!ok) break;
       char* out = static_cast<char*>(a.out);
@@ -705,16 +786,19 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     if (lane == 0) store_wait();        // the last pieces are written before the CTA ends
   }
   __syncwarp();
-  // Split: a CTA's sends all come before its arrival here, and no CTA leaves before every CTA
-  // has arrived, so none is sent to after it left.
-  if (S > 1) cluster_arrive();
+  // A CTA's sends, MMAs and arrivals at others all come before its arrival here, and no CTA leaves
+  // before every CTA of the cluster has arrived, so none is reached after it left.
+  if (C > 1) cluster_arrive();
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc::tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+    if (!PAIR) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
   }
-  if (S > 1) cluster_wait();
+  if (C > 1) cluster_wait();
+  __syncwarp();
+  if (PAIR && warp == 1)                // once both CTAs are done with the pair's accumulators
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
 }
 
 }  // namespace gr

@@ -35,6 +35,28 @@ __device__ __forceinline__ void mma_bf16(uint32_t tmem_d, uint64_t a, uint64_t b
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
+// The same for a pair of CTAs (cta_group::2): M = 256, of which each CTA's shared memory holds 128
+// rows of A and half of B's N rows, and each CTA's TMEM receives its 128 rows of D.
+__host__ __device__ constexpr uint32_t idesc_bf16_pair(int n, int b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn_major) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(2 * kBM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_bf16_pair(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
+          tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Arrives on the barrier at this shared-memory offset of both CTAs of a pair once the MMAs that
+// this thread issued are done.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
 // Instruction descriptor, kind::tf32: tf32 A and B (32-bit operands whose low 13 mantissa
 // bits the tensor core does not use), fp32 accumulator, M = 128, N = n, both K-major.
 __host__ __device__ constexpr uint32_t idesc_tf32(int n) {

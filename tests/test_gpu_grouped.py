@@ -189,6 +189,23 @@ def test_every_way_to_split(Gr, tiles, N):
         check_grad(u, v, [0, rows], Gr.grouped_weight_grad(u, v, offs([0, rows])))
 
 
+@pytest.mark.parametrize("major", ["k", "n"])
+@pytest.mark.parametrize("M,G,K,N", [(4096, 2, 512, 2560), (5000, 7, 776, 3000), (9000, 3, 1024, 1096), (2600, 4, 520, 8968)])
+def test_wide_products(Gr, M, G, K, N, major):
+    # long groups and wide outputs: pairs of CTAs on 256-row tiles, ragged in every dimension
+    x = rnd((M, K), 45)
+    w = rnd((G, N, K), 46, K ** -0.5).transpose(1, 2) if major == "k" else rnd((G, K, N), 46, K ** -0.5)
+    for kind in ("even", "ragged", "empty"):
+        edges = split(M, G, kind, before=3, after=130)
+        for dt in (torch.bfloat16, torch.float32):
+            check_product(x, w, edges, Gr.grouped_matmul(x, w, offs(edges), out_dtype=dt))
+    out = rnd((M, N), 47, dt=torch.float32)
+    old = out.clone()
+    Gr.grouped_matmul(x, w, offs(edges), out=out, alpha=0.5, accumulate=True)
+    check_product(x, w, edges, out, old, 0.5, True)
+    assert torch.equal(Gr.grouped_matmul(x, w, offs(edges)), Gr.grouped_matmul(x, w, offs(edges)))
+
+
 def test_no_rows(Gr):
     w = rnd((3, 16, 24), 22)
     assert Gr.grouped_matmul(rnd((0, 16), 1), w, offs([0, 0, 0, 0])).shape == (0, 24)
