@@ -24,8 +24,9 @@
 // whole block, not one element.
 //
 // One CTA takes a tile of one tensor, a warp one block of 256: its lanes own elements
-// 4 l .. 4 l + 3 and 128 + 4 l .. + 3, so that every access of a warp is contiguous. The pass
-// is bound by HBM: 28 to 30 bytes an element with fp32 states, 12 to 18 with 8-bit ones.
+// 4 l .. 4 l + 3 and 128 + 4 l .. + 3, so that every access of a warp is contiguous. With fp32
+// states (28 to 30 bytes an element) HBM bounds the pass: 731 us for the same 7B set, 739 at
+// the measured copy rate.
 #pragma once
 
 #include <cuda_bf16.h>

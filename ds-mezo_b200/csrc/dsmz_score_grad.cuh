@@ -5,13 +5,15 @@
 //
 // A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary. Pass one
 // over the slice keeps a running maximum and sum of exponentials a thread; the CTAs exchange
-// (max, sum) through distributed shared memory; pass two reads the slice again, from L2 (a cluster's barrier empties L1), and writes the
-// gradient. HBM sees each logit once in and each gradient once out, which is the floor: 190 us
-// for 2048 rows of 152064 bf16 logits, of which this takes 260 (0.73). The unit that makes
-// exponentials and packs bf16 pairs is busy two thirds of the time (2.5 operations a logit),
-// the rest is the latency between a slice's two passes. A variant that streamed whole rows
-// through a shared-memory ring, one CTA a row, took 244 us there but 119 against 113 for 2048 rows
-// of 65536; it did not stay.
+// (max, sum) through distributed shared memory; pass two reads the slice again, from L2 (a
+// cluster's barrier empties L1), and writes the gradient. HBM sees each logit once in and each
+// gradient once out, which is the floor: 190 us for 2048 rows of 152064 bf16 logits, of which
+// this takes 260 (0.73). The unit that makes exponentials and packs bf16 pairs is busy two
+// thirds of the time (2.5 operations a logit), the rest is the latency between a slice's two
+// passes. A variant that streamed whole rows through a shared-memory ring, one CTA a row, took
+// 244 us there but 119 against 113 for 2048 rows of 65536; it did not stay. A short call (8
+// rows of 32000) is the launches' latency: 10 us on the device with the sum's kernel launched
+// beside the rows'.
 // Rows need not be aligned: a slice has a scalar head up to the first 16-byte boundary,
 // 16-byte accesses, and a scalar tail. The target's logit is read before the exchange, so
 // the gradient may overwrite the logits.
@@ -36,8 +38,8 @@ namespace sg {
 constexpr int kMaxSeqs = 128;
 // Largest slice of a row. 2048 rows of 152064 bf16 logits (304 KB) took 311, 297, 273 and 345 us
 // with 1, 2, 4 and 8 CTAs of 256 threads a row (293, 279, 361 and 515 us with 512 threads),
-// before the packed arithmetic below:
-// more CTAs cut the tail of the last wave, and past slices of 76 KB their barriers cost more.
+// before the packed arithmetic below: more CTAs cut the tail of the last wave, and below
+// slices of 76 KB their barriers cost more.
 constexpr int kSliceBytes = 80 * 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -14,6 +14,7 @@ import ctypes
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -24,10 +25,11 @@ __all__ = ["AdamW", "AdamWState"]
 _DT = {torch.float32: DSMZ_F32, torch.bfloat16: DSMZ_BF16}
 
 
-@dataclass
+@dataclass(frozen=True)
 class AdamWState:
     """Mean and second moment of one parameter: fp32 tensors of its size, or int8 / uint8 codes
-    with one fp32 scale for every 256 elements (m = sign q^2 scale, sqrt(v) = q^2 scale)."""
+    with one fp32 scale for every 256 elements (m = sign q^2 scale, sqrt(v) = q^2 scale). The
+    tensors stay: a saved state is copied into them."""
     m: torch.Tensor
     v: torch.Tensor
     m_scale: Optional[torch.Tensor] = None
@@ -63,13 +65,17 @@ class AdamW:
     be None). step: steps already taken. capturable: keep the step count in a device counter,
     which a captured ``step`` advances at every replay; without it the count is the host's,
     and capturing a step is refused, since its replays would repeat one step number.
+
+    The tensors are bound once (``params``, ``states``, ``shadows``, ``grads`` and
+    ``step_counter`` are read-only; what they hold may be written). ``lr``, ``betas``, ``eps``,
+    ``weight_decay`` and ``step_count`` may be set between steps.
     """
 
     def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, grads: Optional[Sequence[torch.Tensor]] = None,
                  states: Optional[Sequence[AdamWState]] = None, state_bits: int = 32,
                  shadows: Optional[Sequence[Optional[torch.Tensor]]] = None, step: int = 0, capturable: bool = False):
-        self.params = list(params)
+        self._params = tuple(params)
         if not self.params:
             raise ValueError("AdamW: no parameters")
         p0 = self.params[0]
@@ -89,7 +95,7 @@ class AdamW:
         self._numels = [p.numel() for p in self.params]
         self.device, self.lr, self.betas = p0.device, float(lr), (b1, b2)
         self.eps, self.weight_decay = float(eps), float(weight_decay)
-        self.states = [AdamWState.zeros(p, state_bits) for p in self.params] if states is None else list(states)
+        self._states = tuple(AdamWState.zeros(p, state_bits) for p in self.params) if states is None else tuple(states)
         if len(self.states) != n:
             raise ValueError("AdamW: one state a parameter")
         self.state_bits = self.states[0].bits
@@ -97,7 +103,7 @@ class AdamW:
             raise ValueError("AdamW: 8-bit states need eps >= 1e-12")
         for p, s in zip(self.params, self.states):
             self._check_state(p, s)
-        self.shadows = [None] * n if shadows is None else list(shadows)
+        self._shadows = (None,) * n if shadows is None else tuple(shadows)
         if len(self.shadows) != n:
             raise ValueError("AdamW: one shadow (or None) a parameter")
         for p, s in zip(self.params, self.shadows):
@@ -117,15 +123,21 @@ class AdamW:
                 e.m_scale, e.v_scale = s.m_scale.data_ptr(), s.v_scale.data_ptr()
             if sh is not None:
                 e.shadow = sh.data_ptr()
-        self._desc = AdamWDesc(param_dtype=_DT[p0.dtype], state_bits=self.state_bits, beta1=b1, beta2=b2,
-                               eps=self.eps, weight_decay=self.weight_decay)
+        self._desc = AdamWDesc(param_dtype=_DT[p0.dtype], state_bits=self.state_bits)
         self._pointers = [p.data_ptr() for p in self.params]
         self.step_count = int(step)              # steps taken (host count; not moved when capturable)
-        self.step_counter = torch.full((1,), int(step), dtype=torch.int64, device=self.device) if capturable else None
-        self.grads = None
+        self._counter = torch.full((1,), int(step), dtype=torch.int64, device=self.device) if capturable else None
+        self._grads = None
         if grads is not None:
             self._bind(grads)
-            self.grads = list(grads)
+            self._grads = tuple(grads)
+
+    # The C table holds their addresses, so what they refer to is not exchanged.
+    params = property(lambda self: self._params)
+    states = property(lambda self: self._states)
+    shadows = property(lambda self: self._shadows)
+    grads = property(lambda self: self._grads)
+    step_counter = property(lambda self: self._counter)
 
     @classmethod
     def for_adapters(cls, adapter_set, grad: torch.Tensor, **kw) -> "AdamW":
@@ -153,7 +165,7 @@ class AdamW:
         if len(grads) != len(self.params):
             raise ValueError("AdamW: one gradient a parameter")
         dt = grads[0].dtype
-        for e, p, g in zip(self._table, self.params, grads):
+        for p, g in zip(self._params, grads):
             if g.dtype != dt or dt not in _DT or g.numel() != p.numel() or g.device != p.device or not g.is_contiguous():
                 raise ValueError("AdamW: gradients must be contiguous, all float32 or all bfloat16, of their "
                                  "parameters' sizes and device")
@@ -161,6 +173,7 @@ class AdamW:
             k = bisect.bisect_left(self._starts, hi)       # the last written range that starts before g ends
             if lo < hi and k > 0 and self._written[k - 1][1] > lo:
                 raise ValueError("AdamW: a gradient overlaps a parameter, state or shadow")
+        for e, g in zip(self._table, grads):               # only once all are good: a refused call changes nothing
             e.grad = g.data_ptr()
         self._desc.grad_dtype = _DT[dt]
 
@@ -178,41 +191,46 @@ class AdamW:
         multiplies every gradient (a clipping or loss-scale factor)."""
         if grads is not None:
             self._bind(grads)
-            self.grads = None                    # a later step() must be given its own again
-        elif self.grads is None:
+            self._grads = None                   # a later step() must be given its own again
+        elif self._grads is None:
             raise ValueError("AdamW: no gradients bound; give them to step()")
-        if [p.data_ptr() for p in self.params] != self._pointers:
+        if [p.data_ptr() for p in self._params] != self._pointers:
             raise RuntimeError("AdamW: a parameter's memory has been replaced since it was bound")
         d = self._desc
-        if self.step_counter is None and torch.cuda.is_current_stream_capturing():
+        if self._counter is None and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: a captured step would repeat one step number at every replay; "
                                "construct with capturable=True")
         d.lr_device = self._scalar(lr, "lr") if isinstance(lr, torch.Tensor) else None
         d.lr = self.lr if lr is None or d.lr_device else float(lr)
         d.grad_scale = self._scalar(grad_scale, "grad_scale")
+        d.beta1, d.beta2 = self.betas
+        d.eps, d.weight_decay = self.eps, self.weight_decay
         d.step = self.step_count + 1
-        d.step_counter = None if self.step_counter is None else self.step_counter.data_ptr()
+        d.step_counter = None if self._counter is None else self._counter.data_ptr()
         ws, nbytes = None, 0
         if d.step_counter or d.lr_device:
             ws = torch.empty(_lib.ADAMW_WORKSPACE_BYTES, dtype=torch.uint8, device=self.device)
             nbytes = ws.numel()
         _lib.launch("adamw_step", self.device, lib().dsmz_adamw_step, ctypes.byref(d), self._table, len(self.params),
                     None if ws is None else ws.data_ptr(), nbytes)
-        if self.step_counter is None:
+        if self._counter is None:
             self.step_count += 1
 
     def state_values(self, m_out: Sequence[torch.Tensor], v_out: Sequence[torch.Tensor]) -> None:
-        """Writes the fp32 values of 8-bit states (a checkpoint in plain fp32, a diagnostic)."""
+        """Writes the fp32 values of 8-bit states (a checkpoint in plain fp32, a diagnostic) to
+        tensors apart from the optimizer's own."""
         if self.state_bits != 8:
             raise ValueError("AdamW: fp32 states are their own values")
         n = len(self.params)
         if len(m_out) != n or len(v_out) != n:
             raise ValueError("AdamW: one output a parameter")
+        index = self.device.index
         for outs in (m_out, v_out):
             if [t.numel() for t in outs] != self._numels or any(
-                    t.dtype != torch.float32 or t.device != self.device or not t.is_contiguous() for t in outs):
+                    t.dtype != torch.float32 or t.get_device() != index or not t.is_contiguous() for t in outs):
                 raise ValueError("AdamW: state values go to contiguous float32 tensors of the parameters' sizes")
         table = type(self._table).from_buffer_copy(self._table)
-        for e, a, v in zip(table, m_out, v_out):
-            e.param, e.shadow = a.data_ptr(), v.data_ptr()
+        words = np.frombuffer(table, dtype=np.int64).reshape(n, -1)       # rows of 64-bit words: no loop over tensors
+        words[:, AdamWTensor.param.offset // 8] = [t.data_ptr() for t in m_out]
+        words[:, AdamWTensor.shadow.offset // 8] = [t.data_ptr() for t in v_out]
         _lib.launch("adamw_state_values", self.device, lib().dsmz_adamw_state_values, table, n)

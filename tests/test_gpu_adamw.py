@@ -328,3 +328,33 @@ def test_refusals(O):
     with pytest.raises(ValueError):
         O.AdamW([p], state_bits=8).state_values([f(9)], [f()])
     assert math.isfinite(float(p.sum()))
+
+
+def test_refused_gradients_leave_the_bound_ones(O):
+    runs = []
+    for refuse in (True, False):
+        made = [make(n, torch.float32, torch.float32, 32, 40 + n, O) for n in (300, 41)]
+        opt = O.AdamW([p for p, _, _ in made], states=[s for _, _, s in made], grads=[g for _, g, _ in made])
+        if refuse:
+            with pytest.raises(ValueError, match="sizes"):
+                opt.step([torch.ones(300, device=DEV), torch.ones(40, device=DEV)])
+            assert opt.step_count == 0
+        opt.step()
+        runs.append([p.clone() for p, _, _ in made])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_bound_tensors_stay_and_settings_may_change(O):
+    p, g, s = make(515, torch.float32, torch.float32, 8, 5, O)
+    opt = O.AdamW([p], LR, (B1, B2), EPS, WD, states=[s], grads=[g])
+    for name in ("params", "states", "shadows", "grads", "step_counter"):
+        with pytest.raises(AttributeError):
+            setattr(opt, name, [p])
+    with pytest.raises(AttributeError):
+        opt.states[0].m = torch.zeros_like(s.m)
+    q, h, r = make(515, torch.float32, torch.float32, 8, 5, O)
+    other = O.AdamW([q], states=[r], grads=[h])            # constructed with the defaults, then set
+    other.lr, other.betas, other.eps, other.weight_decay = LR, (B1, B2), EPS, WD
+    opt.step()
+    other.step()
+    assert torch.equal(p, q) and torch.equal(s.m, r.m) and torch.equal(s.v_scale, r.v_scale)
