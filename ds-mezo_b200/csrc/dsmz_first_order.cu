@@ -209,11 +209,11 @@ size_t grouped_smem(gr::Args& a, int64_t nk) {
   return static_cast<size_t>(fixed) + static_cast<size_t>(a.stages) * SB;
 }
 
-template <int BNT, int MODE, bool PAIR = false>
+template <int BNT, int MODE, bool PAIR, bool F32>
 int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, int64_t tiles, int64_t nk,
                    int sms, const char* what, cudaStream_t s) {
   const size_t smem = grouped_smem<BNT, MODE, PAIR>(a, nk);
-  auto* kernel = gr::k_grouped<BNT, MODE, PAIR>;
+  auto* kernel = gr::k_grouped<BNT, MODE, PAIR, F32>;
   int* err = nullptr;
   int rc = wait_err(&err);
   if (rc) return rc;
@@ -245,12 +245,12 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
   return e == cudaSuccess ? DSMZ_OK : cuda_fail(what, e);
 }
 
-template <int MODE>
+template <int MODE, bool F32>
 int launch_grouped_bn(int bnt, const gr::Args& a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C,
                       int64_t tiles, int64_t nk, int sms, const char* what, cudaStream_t s) {
-  if (bnt == 64) return launch_grouped<64, MODE>(a, A, B, C, tiles, nk, sms, what, s);
-  if (bnt == 128) return launch_grouped<128, MODE>(a, A, B, C, tiles, nk, sms, what, s);
-  return launch_grouped<256, MODE>(a, A, B, C, tiles, nk, sms, what, s);
+  if (bnt == 64) return launch_grouped<64, MODE, false, F32>(a, A, B, C, tiles, nk, sms, what, s);
+  if (bnt == 128) return launch_grouped<128, MODE, false, F32>(a, A, B, C, tiles, nk, sms, what, s);
+  return launch_grouped<256, MODE, false, F32>(a, A, B, C, tiles, nk, sms, what, s);
 }
 
 // Accumulator width for n output columns and `rows` row tiles: 256 columns where that still
@@ -279,7 +279,7 @@ int active_clusters(int s) {
       at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
       cfg.attrs = at;
       cfg.numAttrs = 1;
-      auto* kernel = gr::k_grouped<128, 0, false>;
+      auto* kernel = gr::k_grouped<128, 0, false, false>;
       int n = 0;
       if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
           cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
@@ -425,8 +425,13 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
       const uint64_t sc[2] = {static_cast<uint64_t>(ld_out) * es, static_cast<uint64_t>(ld_out) * es * M};
       a.tma_out = encode_map(&C, out, 3, dc, sc, 128 / es, 32, a.out_f32 != 0);
     }
-    if (pair) return launch_grouped<256, 0, true>(a, A, B, C, tiles, nk, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
-    return launch_grouped_bn<0>(bnt, a, A, B, C, tiles, nk, sms, "dsmz_grouped_matmul", static_cast<cudaStream_t>(stream));
+    const char* what = "dsmz_grouped_matmul";
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a.out_f32)
+      return pair ? launch_grouped<256, 0, true, true>(a, A, B, C, tiles, nk, sms, what, s)
+                  : launch_grouped_bn<0, true>(bnt, a, A, B, C, tiles, nk, sms, what, s);
+    return pair ? launch_grouped<256, 0, true, false>(a, A, B, C, tiles, nk, sms, what, s)
+                : launch_grouped_bn<0, false>(bnt, a, A, B, C, tiles, nk, sms, what, s);
   });
 }
 
@@ -491,7 +496,7 @@ int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, 
       const uint64_t sc[2] = {static_cast<uint64_t>(N) * 4, static_cast<uint64_t>(K) * N * 4};
       a.tma_out = encode_map(&C, out, 3, dc, sc, 32, 32, true);
     }
-    return launch_grouped_bn<1>(bnt, a, A, B, C, tiles, nk, sms, "dsmz_grouped_weight_grad", s);
+    return launch_grouped_bn<1, true>(bnt, a, A, B, C, tiles, nk, sms, "dsmz_grouped_weight_grad", s);
   });
 }
 

@@ -33,7 +33,7 @@
 // What bounds it, on one B200 (floors at the measured copy and bf16 rates):
 //   8192 x 3584 x 18944, 8 groups     826 us of 664 (1014 of 802 sustained): the power cap and
 //                                     the empty rows of ragged last tiles
-//   4001 x 64 x 18944, 32 ragged      56 us of 36: the epilogue of half-filled last tiles, 5 us
+//   4001 x 64 x 18944, 32 ragged      48 us of 36: the epilogue of half-filled last tiles, 5 us
 //                                     until the first tile is stored
 //   4133 x 28672 x 128, 4 groups      54 us of 40: 36 tiles in clusters of 3 leave 40 SMs idle,
 //                                     5 us for the sum of the partial tiles
@@ -105,6 +105,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
         "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
 // Waits for the thread's TMEM loads (their registers pass through an empty volatile asm after it,
 // so that no use of them moves before the wait).
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -132,6 +140,9 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* s
 }
 // No store of this thread reads shared memory any more.
 __device__ __forceinline__ void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// At most the latest group of stores does.
+__device__ __forceinline__ void store_read_wait_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
@@ -343,13 +354,53 @@ __device__ __forceinline__ void put1(const Args& a, char* base, int64_t i, float
   *p = a.accumulate ? *p + v : v;
 }
 
+// The first nrows rows of a staged piece (32 rows of 128 bytes, chunk j of row r at j ^ (r & 7)), of
+// which `bytes` exist: eight lanes a row. All loads first: one by one with the stores they made the
+// case of 127-row groups below 61 us instead of 56.
+__device__ __forceinline__ void store_rows(char* out, int64_t pitch, const unsigned char* piece, int nrows, int bytes, int lane) {
+  const int j = lane & 7;
+  char* o = out + 16 * j + static_cast<int64_t>(lane >> 3) * pitch;
+  uint4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3);
+    v[i] = *reinterpret_cast<const uint4*>(piece + r * 128 + ((j ^ (r & 7)) << 4));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (4 * i + (lane >> 3) < nrows && 16 * j < bytes) *reinterpret_cast<uint4*>(o) = v[i];
+    o += 4 * pitch;
+  }
+}
+
+// 16 fp32 columns (from column c of the warp's, of which `left` exist) of 32 rows, a row a lane, through
+// the staging to the output, four lanes a row.
+__device__ __forceinline__ void put16(const Args& a, char* out, unsigned char* st, const uint32_t* v, int c, int left, int nrows,
+                                      int lane) {
+  if (c >= left) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(st + lane * kStagePitch + j * 16) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
+  const int n = c + (lane & 3) * 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    if (r < nrows && n < left)
+      put4(a, out + static_cast<int64_t>(r) * a.ld * (a.out_f32 ? 4 : 2), n, left - n,
+           *reinterpret_cast<const float4*>(st + r * kStagePitch + (lane & 3) * 16));
+  }
+  __syncwarp();
+}
+
 // BNT: columns of the accumulators (64, 128 or 256; a.bn <= BNT). mapC: the output (3-D, boxes
 // of 32 rows x 128 bytes) where a.tma_out.
+// F32: the type of the output (MODE 1: fp32).
 // PAIR (MODE 0, BNT 256): a cluster of two CTAs computes 256 x 256 tiles with cta_group::2 MMAs.
 // Each loads its 128 rows of A and 128 of B's rows, so a k-step costs 32 KB a CTA instead of 48;
 // the CTA of rank 0 (the leader) waits for both CTAs' loads on its barriers and issues, each CTA's
 // epilogue drains its own half.
-template <int BNT, int MODE, bool PAIR>
+template <int BNT, int MODE, bool PAIR, bool F32>
 __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant__ CUtensorMap mapA,
                                                          const __grid_constant__ CUtensorMap mapB,
                                                          const __grid_constant__ CUtensorMap mapC,
@@ -361,7 +412,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
   constexpr int BM = PAIR ? 2 * kBM : kBM;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int S = a.split, stages = a.stages;
+  const int S = BNT == 256 ? 1 : a.split, stages = a.stages;          // the widest tiles are never split
   unsigned char* scratch = smem + stages * SB;
   // split: partial tiles of the S CTAs for this CTA's rows; else: the epilogue's staging
   const int scratch_bytes = S > 1 ? split_bytes(S, BNT) : kEpiWarps * kStageBytes * a.sbuf;
@@ -574,7 +625,17 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     const bool cols = col0 < a.bn;
     unsigned char* st = scratch + (warp - kFirstEpi) * a.sbuf * kStageBytes;
     const int es = a.out_f32 ? 4 : 2;
-    int u = 0;
+    const float alpha = a.alpha;
+    const bool rows16 = a.vec && !a.accumulate && a.ndim % (16 / es) == 0;         // rows of whole 16-byte chunks
+    // This warp has read accumulator b.
+    auto release = [&](int b) {
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) arrive_remote(map_rank(smem_u32(tempty + b), 0)); else mbar_arrive(tempty + b);
+      }
+    };
+    int u = 0, slot = 0;
     bool ok = true;
     Cursor<MODE, BM> cur(a);
     for (int t = first; t < total && ok; t += step) {
@@ -584,6 +645,77 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
         x.valid = min(max(x.valid - kBM * rank, 0), kBM);
       }
       const int kb = k_begin(x.nk), ke = k_end(x.nk);
+      const int nrows = min(32, x.valid - q * 32);             // this warp's rows that exist
+      if (!F32 && S == 1) {
+        // One accumulator a tile: it goes from TMEM to the output in pieces of 32 rows x 64 columns,
+        // so that few registers are live. All of a warp's columns at once needed more than 168;
+        // the spilled ones go to L2, since shared memory takes nearly all of L1 (4064 x 64 x 18944
+        // in 32 groups of 127 rows: 61 us, 47 so).
+        const bool some = x.nk > 0;                            // else the rows outside the groups: zeros
+        const int b = u & 1;
+        if (some) {
+          ok = __all_sync(0xffffffffu, mbar_wait(tfull + b, static_cast<uint32_t>(u >> 1) & 1u, err));
+          if (!ok) break;
+          tc::tc_fence_after();
+        }
+        const int left = a.ndim - x.n0 - col0;                 // columns from this warp's first
+        const int np = cols && nrows > 0 ? min(CPW / 64, (left + 63) / 64) : 0;
+        const uint32_t src = tmem + static_cast<uint32_t>(b * BNT + col0) + (static_cast<uint32_t>(q * 32) << 16);
+        char* out = static_cast<char*>(a.out) + (static_cast<int64_t>(x.m0 + q * 32) * a.ld + x.n0 + col0) * 2;
+#pragma unroll 1
+        for (int p = 0; p < np; ++p) {
+          // every piece commits one group of stores, so the one before the latest is this slot's
+          unsigned char* piece = st + slot * kStageBytes;
+          if (lane == 0) { if (a.sbuf > 1) store_read_wait_but_one(); else store_read_wait(); }
+          slot = a.sbuf > 1 ? slot ^ 1 : 0;
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0u;
+            if (some) {
+              tmem_ld32(src + 64 * p + 32 * h, v);
+              tmem_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                asm volatile("" : "+r"(v[i]));
+                v[i] = __float_as_uint(alpha * __uint_as_float(v[i]));
+              }
+            }
+            if (rows16) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const __nv_bfloat162 b2 = __floats2bfloat162_rn(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+                  w[i] = *reinterpret_cast<const uint32_t*>(&b2);
+                }
+                *reinterpret_cast<uint4*>(piece + lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            } else {
+#pragma unroll
+              for (int c = 0; c < 32; c += 16)
+                put16(a, out, piece, v + c, 64 * p + 32 * h + c, left, nrows, lane);
+            }
+          }
+          if (some && p + 1 == np) release(b);
+          if (rows16) {
+            const bool whole = a.tma_out && nrows == 32;
+            if (whole) tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (!whole) store_rows(out + 128 * p, a.ld * 2, piece, nrows, (left - 64 * p) * 2, lane);
+            else if (lane == 0) tma_store_3d(&mapC, piece, x.n0 + col0 + 64 * p, x.m0 + q * 32, 0);
+            if (!whole && lane == 0) store_commit();
+          }
+        }
+        if (some) {
+          if (np == 0) release(b);
+          ++u;
+        }
+        continue;
+      }
       float acc[CPW];
       if (kb >= ke) {
 #pragma unroll
@@ -605,25 +737,20 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
             for (int i = 0; i < CPW; ++i) { asm volatile("" : "+r"(v[i])); acc[i] = __uint_as_float(v[i]); }
           } else {
 #pragma unroll
-            for (int c0 = 0; c0 < CPW; c0 += 32) {
-              uint32_t v[32];
-              tmem_ld32(src + c0, v);
+            for (int c0 = 0; c0 < CPW; c0 += 16) {
+              uint32_t v[16];
+              tmem_ld16(src + c0, v);
               tmem_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) { asm volatile("" : "+r"(v[i])); acc[c0 + i] += __uint_as_float(v[i]); }
+              for (int i = 0; i < 16; ++i) { asm volatile("" : "+r"(v[i])); acc[c0 + i] += __uint_as_float(v[i]); }
             }
           }
         }
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR) arrive_remote(map_rank(smem_u32(tempty + b), 0)); else mbar_arrive(tempty + b);
-        }
+        release(b);
       }
       if (!ok) break;
       char* out = static_cast<char*>(a.out);
       if (MODE == 1) out += static_cast<int64_t>(x.seg) * a.gstride * es;
-      const int nrows = min(32, x.valid - q * 32);             // this warp's rows that exist
       if (a.alpha != 1.f) {
 #pragma unroll
         for (int c = 0; c < CPW; ++c) acc[c] *= a.alpha;
@@ -691,96 +818,45 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
             p += a.ld;
           }
         }
-      } else if (a.vec && !a.accumulate && a.ndim * es % 16 == 0) {
-        // Pieces of 32 rows x 128 bytes; chunk j of row r lies at j ^ (r & 7), as the tensor map
-        // expects. a.sbuf of them are staged, fenced and sent together. A whole piece leaves by
-        // TMA; of a group's last rows eight lanes store each row.
+      } else if (rows16) {
+        // fp32 pieces of 32 rows x 128 bytes as above; a.sbuf of them are staged, fenced and sent
+        // together.
         const bool whole = a.tma_out && (MODE == 1 || nrows == 32);
-        char* base = out + (static_cast<int64_t>(x.m0 + q * 32) * a.ld + x.n0 + col0) * es;
-        unsigned char* mine = st + lane * 128;
-        const int per = a.out_f32 ? 32 : 64;              // columns of a piece
-        auto send = [&](int p0, int p1) {                 // pieces [p0, p1) are staged: send them
-          if (whole) {
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              for (int p = p0; p < p1; ++p)
-                tma_store_3d(&mapC, st + (p - p0) * kStageBytes, x.n0 + col0 + p * per, x.m0 + q * 32, MODE == 1 ? x.seg : 0);
-            }
-          } else {
-            __syncwarp();
-            const int j = lane & 7;
-            for (int p = p0; p < p1; ++p) {
-              const int left = (a.ndim - x.n0 - col0 - p * per) * es - 16 * j;
-              char* o = base + p * 128 + 16 * j + static_cast<int64_t>(lane >> 3) * a.ld * es;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3);
-                const uint4 v = *reinterpret_cast<const uint4*>(st + (p - p0) * kStageBytes + r * 128 + ((j ^ (r & 7)) << 4));
-                if (r < nrows && left > 0) *reinterpret_cast<uint4*>(o) = v;
-                o += 4 * a.ld * es;
-              }
-            }
-          }
-        };
-        const int np = min(CPW / per, (a.ndim - x.n0 - col0 + per - 1) / per);       // pieces with columns
+        char* base = out + (static_cast<int64_t>(x.m0 + q * 32) * a.ld + x.n0 + col0) * 4;
+        const int left = a.ndim - x.n0 - col0, np = min(CPW / 32, (left + 31) / 32);         // pieces with columns
         int from = 0;                                     // first piece of the batch
 #pragma unroll
-        for (int p = 0; p < CPW / 32; ++p) {              // bf16 has half as many
+        for (int p = 0; p < CPW / 32; ++p) {
           if (p < np) {
             if (p == from) {                              // the stores before have read the staging
               if (lane == 0) store_read_wait();
               __syncwarp();
             }
-            unsigned char* to = mine + (p - from) * kStageBytes;
-            if (a.out_f32) {
+            unsigned char* to = st + lane * 128 + (p - from) * kStageBytes;
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<float4*>(to + ((j ^ (lane & 7)) << 4)) =
-                    make_float4(acc[32 * p + 4 * j], acc[32 * p + 4 * j + 1], acc[32 * p + 4 * j + 2], acc[32 * p + 4 * j + 3]);
-            } else if (64 * p < CPW) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int c = (64 * p + 8 * j + 2 * i) % CPW;            // p < CPW / 64 here
-                  const __nv_bfloat162 b2 = __floats2bfloat162_rn(acc[c], acc[c + 1]);
-                  w[i] = *reinterpret_cast<const uint32_t*>(&b2);
-                }
-                *reinterpret_cast<uint4*>(to + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            }
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float4*>(to + ((j ^ (lane & 7)) << 4)) =
+                  make_float4(acc[32 * p + 4 * j], acc[32 * p + 4 * j + 1], acc[32 * p + 4 * j + 2], acc[32 * p + 4 * j + 3]);
             if (p + 1 - from == a.sbuf || p + 1 == np) {
-              send(from, p + 1);
+              if (whole) tc::fence_proxy_async_smem();
+              __syncwarp();
+              for (int k = from; k <= p; ++k) {
+                const unsigned char* piece = st + (k - from) * kStageBytes;
+                if (!whole) store_rows(base + k * 128, a.ld * 4, piece, nrows, (left - 32 * k) * 4, lane);
+                else if (lane == 0) tma_store_3d(&mapC, piece, x.n0 + col0 + 32 * k, x.m0 + q * 32, MODE == 1 ? x.seg : 0);
+              }
               from = p + 1;
             }
           }
         }
       } else {
-        // odd pitches and accumulation: 16 fp32 columns at a time through the staging, four lanes a row
-        char* base = out + static_cast<int64_t>(x.m0 + q * 32) * a.ld * es;
+        // odd pitches and accumulation
+        char* base = out + (static_cast<int64_t>(x.m0 + q * 32) * a.ld + x.n0 + col0) * es;
         if (lane == 0) store_read_wait();
         __syncwarp();
 #pragma unroll
-        for (int c0 = 0; c0 < CPW; c0 += 16) {
-          if (x.n0 + col0 + c0 < a.ndim) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<float4*>(st + lane * kStagePitch + j * 16) =
-                  make_float4(acc[c0 + 4 * j], acc[c0 + 4 * j + 1], acc[c0 + 4 * j + 2], acc[c0 + 4 * j + 3]);
-            __syncwarp();
-            const int n = x.n0 + col0 + c0 + (lane & 3) * 4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = i * 8 + (lane >> 2);
-              if (r < nrows && n < a.ndim)
-                put4(a, base + static_cast<int64_t>(r) * a.ld * es, n, a.ndim - n,
-                     *reinterpret_cast<const float4*>(st + r * kStagePitch + (lane & 3) * 16));
-            }
-            __syncwarp();
-          }
-        }
+        for (int c = 0; c < CPW; c += 16)
+          put16(a, base, st, reinterpret_cast<const uint32_t*>(acc + c), c, a.ndim - x.n0 - col0, nrows, lane);
       }
     }
     if (lane == 0) store_wait();        // the last pieces are written before the CTA ends

@@ -206,6 +206,30 @@ def test_wide_products(Gr, M, G, K, N, major):
     assert torch.equal(Gr.grouped_matmul(x, w, offs(edges)), Gr.grouped_matmul(x, w, offs(edges)))
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N", [48, 64, 100, 136, 264])
+def test_many_tiles_a_cta(Gr, dt, N):
+    # a CTA walks several tiles, whole and partial pieces in turn through the same staging
+    M, G, K = 20011, 37, 72
+    edges = split(M, G, "ragged", before=19, after=5)
+    x, w = rnd((M, K), 21), rnd((G, N, K), 22, K ** -0.5).transpose(1, 2)
+    buf = rnd((M, (N + 23) // 16 * 16), 23, dt=dt)
+    out, old = buf[:, :N], buf[:, :N].clone()
+    beside = buf[:, N:].clone()
+    Gr.grouped_matmul(x, w, offs(edges), out=out)
+    check_product(x, w, edges, out, old)
+    first = out.clone()
+    for _ in range(5):
+        out.copy_(old)
+        Gr.grouped_matmul(x, w, offs(edges), out=out)
+        assert torch.equal(out, first)
+    out.copy_(old)
+    Gr.grouped_matmul(x, w, offs(edges), out=out, alpha=1.5, accumulate=True)
+    check_product(x, w, edges, out, old, 1.5, True)
+    assert torch.equal(buf[:, N:], beside)
+    check_product(x, w, edges, Gr.grouped_matmul(x, w, offs(edges), out_dtype=dt))
+
+
 def test_no_rows(Gr):
     w = rnd((3, 16, 24), 22)
     assert Gr.grouped_matmul(rnd((0, 16), 1), w, offs([0, 0, 0, 0])).shape == (0, 24)
