@@ -18,8 +18,9 @@
 // formed again in fp64. A 7B set (161.5 M elements; bf16 gradients and shadow, 16 bytes an
 // element, 394 us at the measured copy rate) took 1634 us with everything in fp64, 1376 in
 // fp32 with blocks near a border done again whole, 723 with single elements done again, no
-// conversions and a path without bounds for whole blocks, 608 with packed arithmetic. What
-// bounds it is instruction issue and latency: 84 instructions an element, 32 warps an SM.
+// conversions and a path without bounds for whole blocks, 608 with packed arithmetic, 576 in
+// CTAs of two warps. What bounds it is instruction issue and latency: 84 instructions an
+// element, 32 warps an SM.
 // A block with a NaN or an infinity gets a scale that makes every element of the block NaN: the
 // whole block, not one element.
 //
@@ -39,7 +40,10 @@ namespace dsmz {
 namespace aw {
 
 constexpr int kBlock = 256;      // elements of one scale
-constexpr int kThreadsAW = 256;
+// Small CTAs start and end apart from each other, so that the loads of some fall into the
+// arithmetic of others: 608, 583 and 576 us for the 8-bit step with 256, 128 and 64 threads, 32 warps an
+// SM of 64 registers each (28 of 72: 624, 24 of 80: 663, 36 of 56: 635). fp32 states: 715 and 713.
+constexpr int kThreadsAW = 64;
 constexpr int kTile = 8 * kThreadsAW;   // elements of one CTA
 
 struct Tensor {
@@ -562,7 +566,7 @@ __device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, 
 
 // 8-bit states: four CTAs an SM (64 registers) took 628 us for a 7B set, three 739, five 840.
 template <int CAP, typename P, typename G, int BITS>
-__global__ void __launch_bounds__(kThreadsAW, BITS == 8 ? 4 : 1) k_adamw(const __grid_constant__ Args<CAP> a) {
+__global__ void __launch_bounds__(kThreadsAW, BITS == 8 ? 16 : 1) k_adamw(const __grid_constant__ Args<CAP> a) {
   const int ti = tensor_of(a, static_cast<int>(blockIdx.x));
   const Tensor& t = a.t[ti];
   const int lane = threadIdx.x & 31;

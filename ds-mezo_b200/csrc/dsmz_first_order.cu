@@ -42,7 +42,7 @@ constexpr int kSmall = 8, kLarge = 256;
 // (289 -> 267 us for a 7B set: a tile is short against finding its tensor in the arguments).
 // The step does not: a second tile's loads would wait for the first (8-bit 634 -> 784 us; with
 // them issued ahead and three CTAs an SM for the registers, 688).
-constexpr int64_t kManyTiles = 148 * 4 * 4;
+constexpr int64_t kManyTiles = 148 * 16 * 4;
 
 template <int CAP>
 void launch_adamw(const aw::Args<CAP>& a, int grid, int pdt, int gdt, int bits, cudaStream_t s) {
