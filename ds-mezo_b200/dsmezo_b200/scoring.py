@@ -11,6 +11,7 @@ counterpart).
 from __future__ import annotations
 
 import ctypes
+from itertools import accumulate
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -80,31 +81,31 @@ def contrastive_loss_grad(logits: torch.Tensor, seq_tokens: Sequence[int], advan
     n = len(seq_tokens)
     if n != len(advantages):
         raise ValueError("contrastive_loss_grad: one advantage per sequence")
-    ntok = int(sum(seq_tokens))
-    if logits.dim() != 2 or logits.shape[0] != ntok or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    edges = [0, *accumulate(map(int, seq_tokens))]
+    ntok = edges[-1]
+    shape, dtype, device = logits.shape, logits.dtype, logits.device
+    if len(shape) != 2 or shape[0] != ntok or (shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("contrastive_loss_grad: logits must be sum(seq_tokens) x V with unit column stride")
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("contrastive_loss_grad: logits must be float32 or bfloat16")
-    if targets.dtype != torch.int32 or targets.numel() != ntok or targets.device != logits.device:
+    if targets.dtype != torch.int32 or targets.numel() != ntok or targets.device != device:
         raise ValueError("contrastive_loss_grad: targets must be ntok int32 token ids on the logits' device")
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or \
-            (out.shape[1] > 1 and out.stride(1) != 1):
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif out.shape != shape or out.dtype != dtype or out.device != device or (shape[1] > 1 and out.stride(1) != 1):
         raise ValueError("contrastive_loss_grad: out must have the logits' shape, type, device and unit column stride")
-    V = logits.shape[1]
-    ld, ld_out = (max(t.stride(0), V) if ntok == 1 else t.stride(0) for t in (logits, out))
+    V, ld, ld_out = shape[1], logits.stride(0), out.stride(0)
+    if ntok == 1:                                # a single row has no pitch
+        ld, ld_out = max(ld, V), max(ld_out, V)
     tgt = targets.contiguous()
-    start = (ctypes.c_int64 * (n + 1))()
-    for i, k in enumerate(seq_tokens):
-        start[i + 1] = start[i] + int(k)
-    adv = (ctypes.c_double * max(n, 1))(*[float(a) for a in advantages])
+    start = (ctypes.c_int64 * (n + 1))(*edges)
+    adv = (ctypes.c_double * max(n, 1))(*map(float, advantages))
     L = lib()
     wsb = int(L.dsmz_contrastive_loss_grad_workspace_bytes(ntok))
-    ws = torch.empty(wsb, dtype=torch.uint8, device=logits.device)
-    loss = torch.empty(1, dtype=torch.float32, device=logits.device)
-    launch("contrastive_loss_grad", logits.device, L.dsmz_contrastive_loss_grad,
-           SCORE_LOGITS_F32 if logits.dtype == torch.float32 else SCORE_LOGITS_BF16, logits.data_ptr(), V, ld,
+    ws = torch.empty(wsb, dtype=torch.uint8, device=device)
+    loss = torch.empty(1, dtype=torch.float32, device=device)
+    launch("contrastive_loss_grad", device, L.dsmz_contrastive_loss_grad,
+           SCORE_LOGITS_F32 if dtype == torch.float32 else SCORE_LOGITS_BF16, logits.data_ptr(), V, ld,
            tgt.data_ptr(), ntok, start, adv, n, float(grad_scale), loss.data_ptr(), out.data_ptr(), ld_out,
            ws.data_ptr(), wsb)
     return loss, out
