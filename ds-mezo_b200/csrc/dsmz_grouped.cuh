@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
           tc::tc_fence_after();
         }
         const int left = a.ndim - x.n0 - col0;                 // columns from this warp's first
-        const int np = cols && nrows > 0 ? min(CPW / 64, (left + 63) / 64) : 0;
+        const int np = cols && nrows > 0 && left > 0 ? min(CPW / 64, (left + 63) / 64) : 0;
         const uint32_t src = tmem + static_cast<uint32_t>(b * BNT + col0) + (static_cast<uint32_t>(q * 32) << 16);
         char* out = static_cast<char*>(a.out) + (static_cast<int64_t>(x.m0 + q * 32) * a.ld + x.n0 + col0) * 2;
 #pragma unroll 1

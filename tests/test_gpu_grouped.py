@@ -190,7 +190,8 @@ def test_every_way_to_split(Gr, tiles, N):
 
 
 @pytest.mark.parametrize("major", ["k", "n"])
-@pytest.mark.parametrize("M,G,K,N", [(4096, 2, 512, 2560), (5000, 7, 776, 3000), (9000, 3, 1024, 1096), (2600, 4, 520, 8968)])
+@pytest.mark.parametrize("M,G,K,N", [(4096, 2, 512, 2560), (5000, 7, 776, 3000), (9000, 3, 1024, 1096), (2600, 4, 520, 8968),
+                                     (9000, 3, 520, 1025)])
 def test_wide_products(Gr, M, G, K, N, major):
     # long groups and wide outputs: pairs of CTAs on 256-row tiles, ragged in every dimension
     x = rnd((M, K), 45)
@@ -207,7 +208,7 @@ def test_wide_products(Gr, M, G, K, N, major):
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("N", [48, 64, 100, 136, 264])
+@pytest.mark.parametrize("N", [48, 64, 100, 136, 257, 264])      # 257: most warps have no column of the last tile
 def test_many_tiles_a_cta(Gr, dt, N):
     # a CTA walks several tiles, whole and partial pieces in turn through the same staging
     M, G, K = 20011, 37, 72
