@@ -195,25 +195,25 @@ int sm_count(int* sms) {
 }
 
 // Shared memory of a launch; sets a.sbuf and a.stages.
-template <int BNT, int MODE, bool PAIR>
+template <int BNT, int MODE, bool PAIR, int EW>
 size_t grouped_smem(gr::Args& a, int64_t nk) {
   constexpr int SB = gr::kABytes + (PAIR ? BNT / 2 : BNT) * gr::kBK * 2;
   constexpr int kSmem = 227 * 1024;
   // two staging pieces a warp let a store run while the next piece is staged; the widest tile
   // gives a stage of the ring for them, which pays where a tile has only a few k-steps
-  a.sbuf = BNT < 256 || PAIR || nk <= 4 ? 2 : 1;
-  const int scratch = a.split > 1 ? gr::split_bytes(a.split, BNT) : gr::kEpiWarps * gr::kStageBytes * a.sbuf;
+  a.sbuf = EW == 8 && (BNT < 256 || PAIR || nk <= 4) ? 2 : 1;
+  const int scratch = a.split > 1 ? gr::split_bytes(a.split, BNT) : EW * gr::kStageBytes * a.sbuf;
   const int fixed = 1024 + scratch + (((a.G + 3) * 8 + 15) & ~15) + 64 + 16 * 8;
   a.stages = (kSmem - fixed) / SB;
   if (a.stages > 8) a.stages = 8;
   return static_cast<size_t>(fixed) + static_cast<size_t>(a.stages) * SB;
 }
 
-template <int BNT, int MODE, bool PAIR, bool F32>
+template <int BNT, int MODE, bool PAIR, bool F32, int EW = 8>
 int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, int64_t tiles, int64_t nk,
                    int sms, const char* what, cudaStream_t s) {
-  const size_t smem = grouped_smem<BNT, MODE, PAIR>(a, nk);
-  auto* kernel = gr::k_grouped<BNT, MODE, PAIR, F32>;
+  const size_t smem = grouped_smem<BNT, MODE, PAIR, EW>(a, nk);
+  auto* kernel = gr::k_grouped<BNT, MODE, PAIR, F32, EW>;
   int* err = nullptr;
   int rc = wait_err(&err);
   if (rc) return rc;
@@ -230,7 +230,7 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
   const int64_t wave = sms / 2;                          // pairs: one a TPC
   cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * (tiles < wave ? tiles : wave)
                                                 : (a.split > 1 ? tiles * a.split : (tiles < sms ? tiles : sms))));
-  cfg.blockDim = dim3(gr::kThreadsG);
+  cfg.blockDim = dim3(32 * (gr::kFirstEpi + EW));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
@@ -271,7 +271,7 @@ int active_clusters(int s) {
     for (int c = 2; c <= 8; ++c) {
       cudaLaunchConfig_t cfg{};
       cfg.gridDim = dim3(static_cast<unsigned>(c * 256));
-      cfg.blockDim = dim3(gr::kThreadsG);
+      cfg.blockDim = dim3(32 * (gr::kFirstEpi + 8));
       cfg.dynamicSmemBytes = 200 * 1024;
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
@@ -279,7 +279,7 @@ int active_clusters(int s) {
       at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
       cfg.attrs = at;
       cfg.numAttrs = 1;
-      auto* kernel = gr::k_grouped<128, 0, false, false>;
+      auto* kernel = gr::k_grouped<128, 0, false, false, 8>;
       int n = 0;
       if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
           cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
@@ -430,6 +430,10 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     if (a.out_f32)
       return pair ? launch_grouped<256, 0, true, true>(a, A, B, C, tiles, nk, sms, what, s)
                   : launch_grouped_bn<0, true>(bnt, a, A, B, C, tiles, nk, sms, what, s);
+    // Few k-steps and short groups: a tile's epilogue sets the pace, and 16 warps shorten it. K = 64, N =
+    // 18944, 32 groups of 64, 127, 160 rows: 28.0, 45.5, 52.8 us with 16 and 31.8, 46.7, 56.0 with 8;
+    // with 192, 256 and 512 rows, where the stores' bandwidth does, 68, 83, 142 and 56, 81, 139.
+    if (bnt == 256 && nk <= 4 && M / G <= 160) return launch_grouped<256, 0, false, false, 16>(a, A, B, C, tiles, nk, sms, what, s);
     return pair ? launch_grouped<256, 0, true, false>(a, A, B, C, tiles, nk, sms, what, s)
                 : launch_grouped_bn<0, false>(bnt, a, A, B, C, tiles, nk, sms, what, s);
   });

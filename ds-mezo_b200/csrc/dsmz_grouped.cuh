@@ -9,12 +9,12 @@
 // outside every group are left as they were, or zeroed where the caller asks.
 //
 // A tile is 128 x BN: MODE 0 128 rows of one group, MODE 1 128 features of the wider operand.
-// Twelve warps:
+// Twelve warps (twenty where the epilogue sets the pace):
 //   warps 0, 2   TMA producers of A and of B: 64-wide k-steps into a ring of stages (issuing a
 //                copy costs its warp some 300 cycles, so one producer for both held the loop);
 //                warp 2 scans the offsets first
 //   warp 1       TMEM owner and MMA issuer (kind::f16, M = 128, N = BN), two accumulators
-//   warps 4-11   epilogue: TMEM -> registers -> shared memory -> TMA stores (whole 32-row
+//   warps 4-     epilogue: TMEM -> registers -> shared memory -> TMA stores (whole 32-row
 //                pieces of a group) or coalesced stores (its last rows, accumulation)
 // A tile that reaches past its group reads the neighbour's rows: harmless in MODE 0 (each
 // output row depends on its own input row; rows past the group are not stored), and cleared
@@ -33,7 +33,7 @@
 // What bounds it, on one B200 (floors at the measured copy and bf16 rates):
 //   8192 x 3584 x 18944, 8 groups     826 us of 664 (1014 of 802 sustained): the power cap and
 //                                     the empty rows of ragged last tiles
-//   4001 x 64 x 18944, 32 ragged      48 us of 36: the epilogue of half-filled last tiles, 5 us
+//   4001 x 64 x 18944, 32 ragged      45 us of 36: the epilogue of half-filled last tiles, 5 us
 //                                     until the first tile is stored
 //   4133 x 28672 x 128, 4 groups      54 us of 40: 36 tiles in clusters of 3 leave 40 SMs idle,
 //                                     5 us for the sum of the partial tiles
@@ -59,9 +59,7 @@ using tc::kBK;
 using tc::kBM;
 
 constexpr int kMaxGroups = 1024;
-constexpr int kEpiWarps = 8;
 constexpr int kFirstEpi = 4;            // first epilogue warp (a multiple of 4: warp % 4 is the TMEM lane quadrant)
-constexpr int kThreadsG = 32 * (kFirstEpi + kEpiWarps);
 constexpr int kChunk = 8;               // k-steps (512 products) an accumulator takes for fp32 outputs
 constexpr int kStagePitch = 80;         // bytes of a staged 64-byte row piece (conflict-free 16-byte accesses)
 constexpr int kStageBytes = 4096;       // staging of an epilogue warp: 32 rows of 128 bytes
@@ -395,19 +393,20 @@ __device__ __forceinline__ void put16(const Args& a, char* out, unsigned char* s
 
 // BNT: columns of the accumulators (64, 128 or 256; a.bn <= BNT). mapC: the output (3-D, boxes
 // of 32 rows x 128 bytes) where a.tma_out.
-// F32: the type of the output (MODE 1: fp32).
+// F32: the type of the output (MODE 1: fp32). EW: epilogue warps, 8, or 16 where a tile of 256 columns
+// has only a few k-steps and its epilogue sets the pace.
 // PAIR (MODE 0, BNT 256): a cluster of two CTAs computes 256 x 256 tiles with cta_group::2 MMAs.
 // Each loads its 128 rows of A and 128 of B's rows, so a k-step costs 32 KB a CTA instead of 48;
 // the CTA of rank 0 (the leader) waits for both CTAs' loads on its barriers and issues, each CTA's
 // epilogue drains its own half.
-template <int BNT, int MODE, bool PAIR, bool F32>
-__global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant__ CUtensorMap mapA,
+template <int BNT, int MODE, bool PAIR, bool F32, int EW>
+__global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __grid_constant__ CUtensorMap mapA,
                                                          const __grid_constant__ CUtensorMap mapB,
                                                          const __grid_constant__ CUtensorMap mapC,
                                                          const __grid_constant__ Args a, int* err) {
-  // columns of an epilogue warp: half a tile, or all of a narrow one whose rows may leave as
+  // columns of an epilogue warp: half a tile (a quarter), or all of a narrow one whose rows may leave as
   // 128 bytes of bf16
-  constexpr int CPW = BNT == 64 && MODE == 0 ? 64 : BNT / 2;
+  constexpr int CPW = BNT == 64 && MODE == 0 ? 64 : BNT * 4 / EW;
   constexpr int SB = kABytes + (PAIR ? BNT / 2 : BNT) * kBK * 2;
   constexpr int BM = PAIR ? 2 * kBM : kBM;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -415,7 +414,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
   const int S = BNT == 256 ? 1 : a.split, stages = a.stages;          // the widest tiles are never split
   unsigned char* scratch = smem + stages * SB;
   // split: partial tiles of the S CTAs for this CTA's rows; else: the epilogue's staging
-  const int scratch_bytes = S > 1 ? split_bytes(S, BNT) : kEpiWarps * kStageBytes * a.sbuf;
+  const int scratch_bytes = S > 1 ? split_bytes(S, BNT) : EW * kStageBytes * a.sbuf;
   int32_t* bnd = reinterpret_cast<int32_t*>(scratch + scratch_bytes);
   int32_t* tile0 = bnd + a.G + 3;
   uint64_t* full = reinterpret_cast<uint64_t*>(
@@ -447,7 +446,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
     }
   } else if (warp == 0 && lane == 0) {
     for (int s = 0; s < stages; ++s) { mbar_init(full + s, 2); mbar_init(empty + s, 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, (PAIR ? 2 : 1) * kEpiWarps); }
+    for (int b = 0; b < 2; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, (PAIR ? 2 : 1) * EW); }
     mbar_init(red_full, 1);
     mbar_init_fence();
     if (S > 1) {                        // the partial tiles of this CTA's rows, from each of the S CTAs
@@ -784,7 +783,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) k_grouped(const __grid_constant_
         if (!ok) break;
         const int first_row = rank * rows, nr = min(rows, kBM - first_row);     // the rows this CTA owns
         constexpr int NQ = BNT / 4;
-        for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstEpi; i < rows * NQ; i += 32 * kEpiWarps) {
+        for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstEpi; i < rows * NQ; i += 32 * EW) {
           // consecutive threads take consecutive columns of a row, or rows of a transposed output
           const int r = a.transposed ? i % rows : i / NQ;
           const int c = 4 * (a.transposed ? i / rows : i % NQ);

@@ -209,9 +209,10 @@ def test_wide_products(Gr, M, G, K, N, major):
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("N", [48, 64, 100, 136, 257, 264])      # 257: most warps have no column of the last tile
-def test_many_tiles_a_cta(Gr, dt, N):
+@pytest.mark.parametrize("G", [37, 150])                         # long and short groups
+def test_many_tiles_a_cta(Gr, dt, N, G):
     # a CTA walks several tiles, whole and partial pieces in turn through the same staging
-    M, G, K = 20011, 37, 72
+    M, K = 20011, 72
     edges = split(M, G, "ragged", before=19, after=5)
     x, w = rnd((M, K), 21), rnd((G, N, K), 22, K ** -0.5).transpose(1, 2)
     buf = rnd((M, (N + 23) // 16 * 16), 23, dt=dt)
