@@ -64,9 +64,10 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+// Not the .aligned forms: warps arrive from divergent code.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // 8-byte store to the same shared variable of CTA `rank` of the cluster.
 __device__ __forceinline__ void st_cluster(void* local, uint32_t rank, float a, float b) {
   uint32_t addr;
@@ -157,6 +158,9 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
   launch_dependents();                                // the sum's launch overlaps the rows
   const int tid = threadIdx.x, nt = blockDim.x;
   const uint32_t C = cluster_size(), rank = cluster_rank();
+  // Another CTA's shared memory may be written once that CTA is known to run: every thread says
+  // so here, and the wait comes after pass one, which hides it.
+  if (C > 1) cluster_arrive_relaxed();
   const int64_t row = blockIdx.x / C;
   int si = 0;                                         // the row's sequence
   while (si + 1 < seqs.n && seqs.start[si + 1] <= row) ++si;
@@ -222,8 +226,10 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
   if (C > 1) {
+    cluster_wait();                                   // every CTA of the cluster has started
     if (tid < static_cast<int>(C)) st_cluster(&part[rank], tid, m, s);
-    cluster_sync();
+    cluster_arrive();
+    cluster_wait();                                   // and has written its pair here
     m = lane < static_cast<int>(C) ? part[lane].x : -INFINITY;
     s = lane < static_cast<int>(C) ? part[lane].y : 0.f;
 #pragma unroll
