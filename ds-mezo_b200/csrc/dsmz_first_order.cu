@@ -1,5 +1,6 @@
 // C ABI of the first-order operators declared in dsmezo.h: products grouped by adapter copy,
 // the scoring loss with its gradient, and AdamW over many tensors.
+#include <atomic>
 #include <cmath>
 #include <exception>
 #include <vector>
@@ -148,8 +149,9 @@ int adamw_run(const dsmz_adamw_desc& d, const dsmz_adamw_tensor* tensors, int32_
       [&](const aw::Args<CAP>& a, int grid) { launch_adamw<CAP>(a, grid, d.param_dtype, d.grad_dtype, d.state_bits, s); });
 }
 
-// Error word of the bounded waits, one per device.
+// Error word of the bounded waits, one per device, and their limit.
 __device__ int g_wait_err;
+std::atomic<int64_t> g_wait_ns{static_cast<int64_t>(kTimeoutNs)};
 
 int wait_err(int** p) {
   void* q = nullptr;
@@ -213,6 +215,7 @@ template <int BNT, int MODE, bool PAIR, bool F32, int EW = 8>
 int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, int64_t tiles, int64_t nk,
                    int sms, const char* what, cudaStream_t s) {
   const size_t smem = grouped_smem<BNT, MODE, PAIR, EW>(a, nk);
+  a.wait_ns = static_cast<uint64_t>(g_wait_ns.load(std::memory_order_relaxed));
   auto* kernel = gr::k_grouped<BNT, MODE, PAIR, F32, EW>;
   int* err = nullptr;
   int rc = wait_err(&err);
@@ -502,6 +505,13 @@ int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, 
     }
     return launch_grouped_bn<1, true>(bnt, a, A, B, C, tiles, nk, sms, "dsmz_grouped_weight_grad", s);
   });
+}
+
+int dsmz_first_order_set_wait_limit(int64_t ns) {
+  if (ns < 0 || ns > int64_t{60} * 1000000000)
+    return fail(DSMZ_ERR_INVALID, "dsmz_first_order_set_wait_limit: 0 to 60 s");
+  g_wait_ns.store(ns, std::memory_order_relaxed);
+  return DSMZ_OK;
 }
 
 int32_t dsmz_first_order_device_error(dsmz_stream_t stream) {

@@ -41,8 +41,11 @@
 //                                     chain of offsets (2 us), 14 k-steps (4), partial sums (2)
 //   dW of 4096 x (18944, 64)          31 us of 25: HBM, 3 us of stores after the last k-step
 //
-// Every mbarrier wait gives up after ~1 s, sets the error word, and lets each role finish its
-// own copies before the CTA frees its TMEM.
+// Every mbarrier wait gives up after Args::wait_ns (1 s unless the caller set another limit). The CTA
+// then raises a flag of its own, at which its other roles give up too; an accumulator that lacks
+// products is never announced, the tiles not produced are stored as NaN, copies and MMAs in flight
+// are waited for, and the device's error word is set. The word is only a record: the next launch
+// starts afresh.
 #pragma once
 
 #include <cuda.h>
@@ -89,7 +92,11 @@ struct Args {
   int32_t out_f32, accumulate, zero_rest, vec;
   int32_t tma_out;                      // mapC is valid: whole pieces leave by TMA
   float alpha;
+  uint64_t wait_ns;                     // limit of a wait; 0: nothing is loaded, so that the waits run out
 };
+// What is in flight when a wait gave up gets this long to land: loads and copies between CTAs take
+// microseconds.
+constexpr uint64_t kLandNs = 10000000;
 
 // 32 lanes x 32 consecutive fp32 columns of TMEM into v[0..31]; complete after tmem_wait().
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
@@ -191,29 +198,37 @@ __device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* m
       "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
       : "memory");
 }
-// Bounded wait with cluster-scope acquire (arrivals come from other CTAs).
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
+// Whether the phase has completed, asleep for up to `ns` until it has; arrivals come from other CTAs.
+__device__ __forceinline__ bool try_cluster(uint64_t* bar, uint32_t parity, uint32_t ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, "
+      "p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(ns)
+      : "memory");
+  return ok != 0;
+}
+// Waits until the phase completes: false after `a.wait_ns`, or when another role of this CTA has given
+// up (`gone`, in shared memory).
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_for(const Args& a, uint64_t* bar, uint32_t parity, volatile int32_t* gone) {
+  if (!CLUSTER && mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = gtimer();
-  uint64_t tchk = t0;
   while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, "
-        "p;\n}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendNs)
-        : "memory");
-    if (ok) return true;
-    const uint64_t t = gtimer();
-    if (t - tchk > kPollNs) {
-      tchk = t;
-      if (*reinterpret_cast<volatile int*>(err) != 0) return false;
-      if (t - t0 > kTimeoutNs) {
-        atomicExch(err, 1);
-        return false;
-      }
+    if (CLUSTER ? try_cluster(bar, parity, kSuspendNs) : mbar_try_wait_sleep(bar, parity)) return true;
+    if (*gone != 0) return false;
+    if (gtimer() - t0 >= a.wait_ns) {
+      *gone = 1;
+      return false;
     }
   }
+}
+// For copies and MMAs in flight after a wait gave up: until they complete, kLandNs at most.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = gtimer();
+  while (!mbar_try_wait(bar, parity))
+    if (gtimer() - t0 > kLandNs) return;
 }
 
 // Row boundaries bnd[0..G+2] = 0, the offsets (clamped to [0, M], running maximum), M; segment
@@ -391,6 +406,19 @@ __device__ __forceinline__ void put16(const Args& a, char* out, unsigned char* s
   __syncwarp();
 }
 
+// Rows [r0, r1) and columns [c0, c1) of a tile that was not produced become NaN. One warp.
+template <int MODE>
+__device__ __noinline__ void fill_nan(const Args& a, int seg, int m0, int r0, int r1, int c0, int c1, int lane) {
+  const int64_t base = MODE == 1 ? static_cast<int64_t>(seg) * a.gstride : 0;
+  for (int r = r0; r < r1; ++r)
+    for (int c = c0 + lane; c < c1; c += 32) {
+      const int64_t m = m0 + r;
+      const int64_t i = base + (a.transposed ? c * a.ld + m : m * a.ld + c);
+      if (a.out_f32) static_cast<float*>(a.out)[i] = __int_as_float(0x7fc00000);
+      else static_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16_rn(__int_as_float(0x7fc00000));
+    }
+}
+
 // BNT: columns of the accumulators (64, 128 or 256; a.bn <= BNT). mapC: the output (3-D, boxes
 // of 32 rows x 128 bytes) where a.tma_out.
 // F32: the type of the output (MODE 1: fp32). EW: epilogue warps, 8, or 16 where a tile of 256 columns
@@ -423,7 +451,9 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
   uint64_t* tfull = empty + stages;     // [2]
   uint64_t* tempty = tfull + 2;         // [2]
   uint64_t* red_full = tempty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_full + 1);
+  uint64_t* dead = red_full + 1;        // the MMAs issued before a wait gave up
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dead + 1);
+  volatile int32_t* gone = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);      // a wait of this CTA gave up
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kCols = 2 * BNT;        // TMEM columns: two accumulators
   const int rank = PAIR ? static_cast<int>(blockIdx.x) & 1 : (S > 1 ? static_cast<int>(blockIdx.x) % S : 0);
@@ -448,6 +478,8 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
     for (int s = 0; s < stages; ++s) { mbar_init(full + s, 2); mbar_init(empty + s, 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(tfull + b, 1); mbar_init(tempty + b, (PAIR ? 2 : 1) * EW); }
     mbar_init(red_full, 1);
+    mbar_init(dead, 1);
+    *gone = 0;
     mbar_init_fence();
     if (S > 1) {                        // the partial tiles of this CTA's rows, from each of the S CTAs
       const int rows = (kBM + S - 1) / S;
@@ -476,7 +508,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
     const bool is_a = warp == 0;
     int s = 0, n = 0;                   // stage, k-steps issued
     uint32_t ph = 1;                    // parity of the wait for an empty stage (the first round passes)
-    bool ok = true;
+    bool ok = a.wait_ns != 0;
     Cursor<MODE, BM> cur(a);
     for (int t = first; t < total && ok; t += step) {
       const Tile y = cur.at(a, bnd, tile0, t);
@@ -493,7 +525,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
                                    : (MODE == 0 ? static_cast<uint32_t>((nba + nbp) * a.arows * 128) : 16384u);
       const int ke = k_end(nk);
       for (int k = k_begin(nk); k < ke; ++k) {
-        ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ph, err));
+        ok = __all_sync(0xffffffffu, wait_for(a, empty + s, ph, gone));
         if (!ok) break;
         unsigned char* dst = smem + s * SB + (is_a ? 0 : kABytes);
         uint64_t* bar = full + s;
@@ -547,7 +579,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
     // the leader, and neither CTA leaves before the other)
     if (!ok && rank * (PAIR ? 1 : 0) == 0)
       for (int i = (n > stages ? n - stages : 0); i < n; ++i)
-        mbar_drain(full + (i % stages), static_cast<uint32_t>(i / stages) & 1u);
+        drain(full + (i % stages), static_cast<uint32_t>(i / stages) & 1u);
   } else if (warp == 1 && PAIR && rank != 0) {
     // the leader issues for both
   } else if (warp == 1) {
@@ -558,7 +590,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
     const uint64_t a0 = MODE == 0 ? tc::sdesc(smem_u32(smem), 16, 1024) : tc::sdesc(smem_u32(smem), 8192, 1024);
     const uint64_t b0 = b_mn ? tc::sdesc(smem_u32(smem) + kABytes, 8192, 1024) : tc::sdesc(smem_u32(smem) + kABytes, 16, 1024);
     const uint32_t ka = MODE == 0 ? 2 : 128, kb_ = b_mn ? 128 : 2;        // a 16-wide slice of the k-step
-    int s = 0, u = 0, last = -1;        // stage, accumulators begun, the last one committed
+    int s = 0, u = 0;                   // stage, accumulators begun
     uint32_t ph = 0;
     bool ok = true;
     Cursor<MODE, BM> cur(a);
@@ -570,14 +602,14 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
         const int b = u & 1;
         if (u >= 2) {
           const uint32_t par = static_cast<uint32_t>((u >> 1) - 1) & 1u;
-          ok = __all_sync(0xffffffffu, PAIR ? mbar_wait_cluster(tempty + b, par, err) : mbar_wait(tempty + b, par, err));
+          ok = __all_sync(0xffffffffu, wait_for<PAIR>(a, tempty + b, par, gone));
         }
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t acc = tmem + static_cast<uint32_t>(b * BNT);
         const int cend = min(ke, c + a.chunk);
         for (int k = c; k < cend; ++k) {
-          ok = __all_sync(0xffffffffu, mbar_wait(full + s, ph, err));
+          ok = __all_sync(0xffffffffu, wait_for(a, full + s, ph, gone));
           if (!ok) break;
           const uint64_t da = a0 + static_cast<uint32_t>(s * (SB >> 4)), db = b0 + static_cast<uint32_t>(s * (SB >> 4));
           const uint32_t more = k > c ? 1u : 0u;
@@ -610,13 +642,18 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
           }
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
-        if (elect_one()) {                             // on an error too: it completes once the issued MMAs have
+        if (!ok) break;                                // an accumulator that lacks products is not announced
+        if (elect_one()) {
           if (PAIR) tc::mma_commit_pair(tfull + b); else tc::mma_commit(tfull + b);
         }
-        last = u;
       }
     }
-    if (!ok && last >= 0) mbar_drain(tfull + (last & 1), static_cast<uint32_t>(last >> 1) & 1u);
+    if (!ok) {                                         // let the MMAs already issued end
+      if (elect_one()) {
+        if (PAIR) tc::mma_commit_pair(dead, 1); else tc::mma_commit(dead);
+      }
+      drain(dead, 0);
+    }
   } else if (warp >= kFirstEpi) {
     const int q = warp & 3;             // TMEM lane quadrant
     const int col0 = ((warp - kFirstEpi) >> 2) * CPW;
@@ -636,8 +673,9 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
     };
     int u = 0, slot = 0;
     bool ok = true;
+    int t = first;
     Cursor<MODE, BM> cur(a);
-    for (int t = first; t < total && ok; t += step) {
+    for (; t < total; t += step) {
       Tile x = cur.at(a, bnd, tile0, t);
       if (PAIR) {                       // this CTA's half of the rows
         x.m0 += kBM * rank;
@@ -653,7 +691,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
         const bool some = x.nk > 0;                            // else the rows outside the groups: zeros
         const int b = u & 1;
         if (some) {
-          ok = __all_sync(0xffffffffu, mbar_wait(tfull + b, static_cast<uint32_t>(u >> 1) & 1u, err));
+          ok = __all_sync(0xffffffffu, wait_for(a, tfull + b, static_cast<uint32_t>(u >> 1) & 1u, gone));
           if (!ok) break;
           tc::tc_fence_after();
         }
@@ -722,7 +760,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
       }
       for (int c = kb; c < ke; c += a.chunk, ++u) {
         const int b = u & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(tfull + b, static_cast<uint32_t>(u >> 1) & 1u, err));
+        ok = __all_sync(0xffffffffu, wait_for(a, tfull + b, static_cast<uint32_t>(u >> 1) & 1u, gone));
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t src = tmem + static_cast<uint32_t>(b * BNT + col0) + (static_cast<uint32_t>(q * 32) << 16);
@@ -747,7 +785,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
         }
         release(b);
       }
-      if (!ok) break;
+      if (S == 1 && !ok) break;
       char* out = static_cast<char*>(a.out);
       if (MODE == 1) out += static_cast<int64_t>(x.seg) * a.gstride * es;
       if (a.alpha != 1.f) {
@@ -761,7 +799,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
         // every MMA is done) and copies the rows of each owner as one block.
         const int rows = (kBM + S - 1) / S, half = col0 / CPW;
         constexpr int RB = CPW * 4, H = BNT / CPW;       // bytes of a staged row, column halves
-        if (cols) {
+        if (cols && ok) {
           unsigned char* mine = smem + ((warp - kFirstEpi) >> 2) * (kBM * RB) + row * RB;
 #pragma unroll
           for (int c = 0; c < CPW; c += 4)
@@ -769,7 +807,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
           tc::fence_proxy_async_smem();
         }
         __syncwarp();
-        if (cols && lane == 0) {
+        if (cols && ok && lane == 0) {
           int r = q * 32;
           while (r < q * 32 + 32) {
             const int to = r / rows, upto = min(min(q * 32 + 32, (to + 1) * rows), kBM);
@@ -779,8 +817,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
             r = upto;
           }
         }
-        ok = __all_sync(0xffffffffu, mbar_wait_cluster(red_full, 0, err));
-        if (!ok) break;
+        if (ok) ok = __all_sync(0xffffffffu, wait_for<true>(a, red_full, 0, gone));
         const int first_row = rank * rows, nr = min(rows, kBM - first_row);     // the rows this CTA owns
         constexpr int NQ = BNT / 4;
         for (int i = static_cast<int>(threadIdx.x) - 32 * kFirstEpi; i < rows * NQ; i += 32 * EW) {
@@ -791,6 +828,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
           if (r >= nr || m >= x.valid || c >= a.bn || n >= a.ndim) continue;
           const unsigned char* part = scratch + ((c / CPW) * rows + r) * RB + ((((c % CPW) >> 2) ^ (m & 7)) << 4);
           float4 v = *reinterpret_cast<const float4*>(part);
+          if (!ok) v.x = v.y = v.z = v.w = __int_as_float(0x7fc00000);     // a partial tile is missing
           for (int p = 1; p < S; ++p) {
             const float4 w = *reinterpret_cast<const float4*>(part + p * H * rows * RB);
             v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
@@ -859,6 +897,15 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
       }
     }
     if (lane == 0) store_wait();        // the last pieces are written before the CTA ends
+    if (S == 1 && !ok) {
+      __syncwarp();
+      for (; t < total; t += step) {    // this warp's part of every tile it did not get
+        const Tile x = cur.at(a, bnd, tile0, t);
+        const int top = PAIR ? kBM * rank : 0;
+        fill_nan<MODE>(a, x.seg, x.m0 + top, q * 32, min(q * 32 + 32, x.valid - top), x.n0 + col0,
+                       min(x.n0 + min(col0 + CPW, a.bn), a.ndim), lane);
+      }
+    }
   }
   __syncwarp();
   // A CTA's sends, MMAs and arrivals at others all come before its arrival here, and no CTA leaves
@@ -871,6 +918,12 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
     if (!PAIR) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
   }
   if (C > 1) cluster_wait();
+  if (*gone != 0 && threadIdx.x == 0) {
+    atomicExch(err, 1);
+    // Every CTA of the cluster has issued all that it will: what still travels to this one lands.
+    const uint64_t t0 = gtimer();
+    while (gtimer() - t0 < kLandNs) __nanosleep(100000);
+  }
   __syncwarp();
   if (PAIR && warp == 1)                // once both CTAs are done with the pair's accumulators
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");

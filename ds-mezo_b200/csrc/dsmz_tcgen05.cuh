@@ -48,13 +48,13 @@ __device__ __forceinline__ void mma_bf16_pair(uint32_t tmem_d, uint64_t a, uint6
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-// Arrives on the barrier at this shared-memory offset of both CTAs of a pair once the MMAs that
-// this thread issued are done.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// Arrives on the barrier at this shared-memory offset of both CTAs of a pair (or those of the mask)
+// once the MMAs that this thread issued are done.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint16_t ctas = 3) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3))
+      "h"(ctas)
       : "memory");
 }
 // Instruction descriptor, kind::tf32: tf32 A and B (32-bit operands whose low 13 mantissa

@@ -158,6 +158,7 @@ SIGNATURES = {
     "dsmz_grouped_weight_grad": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32,
                                            c_void_p, c_void_p, c_float, c_uint32, c_void_p]),
     "dsmz_first_order_device_error": (c_int32, [c_void_p]),
+    "dsmz_first_order_set_wait_limit": (c_int32, [c_int64]),
     "dsmz_contrastive_loss_grad_workspace_bytes": (c_size_t, [c_int64]),
     "dsmz_contrastive_loss_grad": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, POINTER(c_int64),
                                              POINTER(c_double), c_int32, c_double, c_void_p, c_void_p, c_int64,

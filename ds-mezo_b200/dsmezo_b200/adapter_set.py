@@ -274,7 +274,8 @@ class AdapterSet:
         x: rows x d_in, bf16. which: 'shadow' (the factors as last updated) or 'pos' / 'neg',
         whose ``directions`` copies each own the rows [row_offsets[k], row_offsets[k + 1]) (int32
         on the device; may be left out for a single copy). out, accumulate: add to the base
-        module's output in place. Runs on the current stream; see ``grouped.adapter_forward``."""
+        module's output in place. Runs on the current stream; see ``grouped.adapter_forward``. NaN
+        where a wait of a kernel ran out of time (``device_error``)."""
         A, B = self._copies(i, which)
         return grouped.adapter_forward(x, A, B, self._rows(x, row_offsets, A.shape[0]), out=out, alpha=alpha,
                                        accumulate=accumulate)
@@ -282,7 +283,8 @@ class AdapterSet:
     def delta_backward(self, i: int, dy: torch.Tensor, x: torch.Tensor, t: torch.Tensor, grad: torch.Tensor, *,
                        alpha: float = 1.0, accumulate: bool = False, need_dx: bool = True) -> Optional[torch.Tensor]:
         """Gradients of ``delta(i, x, 'shadow')``: writes (accumulate: adds) those of A and B into
-        module i's part of the gradient arena and returns the one in x (None without need_dx)."""
+        module i's part of the gradient arena and returns the one in x (None without need_dx).
+        NaN where a wait of a kernel ran out of time (``device_error``)."""
         A, B = self._copies(i, "shadow")
         if grad.dtype != torch.float32 or grad.dim() != 1 or grad.numel() < self.numel or not grad.is_contiguous():
             raise ValueError("delta_backward: grad is a gradient arena (grad_arena())")
@@ -384,8 +386,11 @@ class AdapterSet:
         return int(lib().dsmz_plan_uses_tensor_cores(self._plan)) == 2
 
     def device_error(self) -> int:
-        """Reads and clears the device error word (synchronises the stream)."""
-        return int(lib().dsmz_plan_device_error(self._plan, self._stream()))
+        """Reads and clears this set's device error word and the device's word of the products
+        through the adapters (``grouped.device_error``): nonzero when either is. Synchronises the
+        stream."""
+        products = grouped.device_error(self.device)
+        return int(lib().dsmz_plan_device_error(self._plan, self._stream())) or products
 
     def factor_norms(self) -> torch.Tensor:
         """Frobenius norms of the fp32 masters, A then B of each module (device, fp32)."""

@@ -6,6 +6,10 @@ copy. ``grouped_matmul`` multiplies every group of rows by its own matrix, ``gro
 forms the gradient of every matrix, and ``adapter_forward`` / ``adapter_backward`` combine them
 to the rank-r product of an adapter and its gradients. One launch for all groups; bf16
 operands, fp32 sums on the tensor cores. The same entry points serve any set of experts.
+
+A kernel whose barriers do not complete within a limit (``set_wait_limit``, 1 s at first: a
+preempted device, a defect) returns all the same: the parts of its output that it did not produce
+are NaN, and ``device_error`` (or ``AdapterSet.device_error``) tells of it. Later calls run as usual.
 """
 from __future__ import annotations
 
@@ -13,9 +17,10 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._lib import DSMZ_BF16, DSMZ_F32, GROUPED_ACCUMULATE, GROUPED_ZERO_REST, MAX_GROUPS, launch, lib
+from ._lib import DSMZ_BF16, DSMZ_F32, GROUPED_ACCUMULATE, GROUPED_ZERO_REST, MAX_GROUPS, check, launch, lib
 
-__all__ = ["grouped_matmul", "grouped_weight_grad", "adapter_forward", "adapter_backward", "device_error"]
+__all__ = ["grouped_matmul", "grouped_weight_grad", "adapter_forward", "adapter_backward", "device_error",
+           "set_wait_limit"]
 
 _DT = {torch.float32: DSMZ_F32, torch.bfloat16: DSMZ_BF16}
 
@@ -71,7 +76,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, row_offsets: torch.Tensor, 
     input gradient). row_offsets: G + 1 int32 on the device, ascending; values beyond [0, M]
     or below an earlier one are clamped. out: M x N, bf16 or fp32, any row pitch; rows outside
     every group stay as they are. Without out a new tensor of ``out_dtype`` is returned whose
-    rows outside every group are zero. accumulate: add to out (fp32 sum, rounded once)."""
+    rows outside every group are zero. accumulate: add to out (fp32 sum, rounded once). NaN
+    where a wait of the kernel ran out of time: ``device_error`` tells."""
     me = "grouped_matmul"
     x = _rows(x, me)
     if not isinstance(w, torch.Tensor) or w.dim() != 3 or w.dtype != torch.bfloat16 or w.device != x.device:
@@ -106,7 +112,8 @@ def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, row_offsets: torch.Te
     """dw[g] = alpha * x[rows of g].T @ dy[rows of g]: the gradient of ``grouped_matmul`` in w.
 
     x: M x K and dy: M x N, bf16. out: G x K x N contiguous fp32 (new unless given); a group
-    without rows gives zeros. accumulate: add to out."""
+    without rows gives zeros. accumulate: add to out. NaN where a wait of the kernel ran out of
+    time: ``device_error`` tells."""
     me = "grouped_weight_grad"
     x, dy = _rows(x, me), _rows(dy, me)
     M, K = x.shape
@@ -155,6 +162,15 @@ def adapter_backward(dy: torch.Tensor, x: torch.Tensor, t: torch.Tensor, A: torc
 
 def device_error(device=None) -> int:
     """Reads and clears the device's error word of the grouped products (synchronises the
-    current stream): nonzero when a kernel's barrier wait ran out of time."""
+    current stream): nonzero when a kernel's barrier wait has run out of time since the last
+    reading. Its output holds NaN where it was not produced."""
     with torch.cuda.device(device):
         return int(lib().dsmz_first_order_device_error(torch.cuda.current_stream().cuda_stream))
+
+
+def set_wait_limit(seconds: float) -> None:
+    """Limit of the barrier waits inside the grouped products, for the calls (and captures) that
+    follow in this process: 0 to 60 s, 1 s at first. It counts wall time, so a device that other
+    processes preempt for longer needs more. At 0 the kernels load nothing, so that their waits
+    run out: how a program tries what it does about ``device_error``."""
+    check(lib().dsmz_first_order_set_wait_limit(round(float(seconds) * 1e9)), "set_wait_limit")

@@ -380,7 +380,9 @@ int dsmz_step_update_directions(const dsmz_plan* plan, const float* dd, int32_t 
  * y: BF16 or F32, pitch ld_out. Rows outside every group stay as they are, or become zero
  * with DSMZ_GROUPED_ZERO_REST. x and w: 16-byte aligned, pitches and group stride multiples
  * of 8 elements (K and N themselves may be any size). y must not overlap x or w.
- * Deterministic; no workspace. */
+ * Deterministic; no workspace. A barrier wait inside the kernel that passes its limit (see
+ * dsmz_first_order_set_wait_limit) leaves NaN in every part of y that was not produced and sets
+ * the error word that dsmz_first_order_device_error reads; later calls are not affected. */
 #define DSMZ_MAX_GROUPS 1024
 #define DSMZ_MAX_GROUPED_DIM 1073741824
 #define DSMZ_GROUPED_ACCUMULATE 1u
@@ -395,9 +397,14 @@ int dsmz_grouped_weight_grad(const void* x, int64_t M, int64_t K, int64_t ld_x, 
                              int32_t G, const int32_t* row_offsets, float* out, float alpha, uint32_t flags,
                              dsmz_stream_t stream);
 /* Reads and clears the current device's error word of the first-order kernels (synchronises the
- * stream): 1 when a kernel gave up on a barrier wait after its time limit, -1 when the word
- * could not be read. */
+ * stream): 1 when a kernel since the last reading gave up on a barrier wait after its time limit,
+ * -1 when the word could not be read. */
 int32_t dsmz_first_order_device_error(dsmz_stream_t stream);
+/* Limit of the barrier waits of the grouped products launched (or captured) from now on, in this
+ * process: 0 to 60 s, 1 s unless set. The limit counts wall time, so a device that other
+ * processes preempt for longer needs more. At 0 the kernels load nothing, so that their waits run
+ * out: how a program tries what it does about the error word. */
+int dsmz_first_order_set_wait_limit(int64_t ns);
 
 /* The contrastive scoring loss (dsmz_contrastive_loss) with its gradient in the logits:
  *   loss[0] (device F32; the terms and their sum are fp64) = sum_i a_i mean_{t in i} nll_t
