@@ -281,14 +281,16 @@ class AdapterSet:
                                        accumulate=accumulate)
 
     def delta_backward(self, i: int, dy: torch.Tensor, x: torch.Tensor, t: torch.Tensor, grad: torch.Tensor, *,
-                       alpha: float = 1.0, accumulate: bool = False, need_dx: bool = True) -> Optional[torch.Tensor]:
-        """Gradients of ``delta(i, x, 'shadow')``: writes (accumulate: adds) those of A and B into
-        module i's part of the gradient arena and returns the one in x (None without need_dx).
+                       row_offsets: Optional[torch.Tensor] = None, alpha: float = 1.0, accumulate: bool = False, need_dx: bool = True) -> Optional[torch.Tensor]:
+        """Gradients of ``delta(i, x, 'shadow', row_offsets)``: writes (accumulate: adds) those of A and
+        B into module i's part of the gradient arena and returns the one in x (None without need_dx;
+        zero in rows outside the offsets). row_offsets: those that ``delta`` was given; rows outside
+        them had no part in its output, so their dy has none in the gradients.
         NaN where a wait of a kernel ran out of time (``device_error``)."""
         A, B = self._copies(i, "shadow")
         if grad.dtype != torch.float32 or grad.dim() != 1 or grad.numel() < self.numel or not grad.is_contiguous():
             raise ValueError("delta_backward: grad is a gradient arena (grad_arena())")
-        dx, _, _ = grouped.adapter_backward(dy, x, t, A, B, self._rows(x, None, 1), alpha=alpha,
+        dx, _, _ = grouped.adapter_backward(dy, x, t, A, B, self._rows(x, row_offsets, 1), alpha=alpha,
                                             dA=self.A(i, grad).unsqueeze(0), dB=self.B(i, grad).unsqueeze(0),
                                             accumulate=accumulate, need_dx=need_dx)
         return dx
