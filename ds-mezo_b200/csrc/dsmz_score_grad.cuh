@@ -8,7 +8,7 @@
 // (max, sum) through distributed shared memory; pass two reads the slice again, from L2 (a
 // cluster's barrier empties L1), and writes the gradient. HBM sees each logit once in and each
 // gradient once out, which is the floor: 190 us for 2048 rows of 152064 bf16 logits, of which
-// this takes 260 (0.73). The unit that makes exponentials and packs bf16 pairs is busy two
+// this takes 256 (0.74). The unit that makes exponentials and packs bf16 pairs is busy two
 // thirds of the time (2.5 operations a logit), the rest is the latency between a slice's two
 // passes. A variant that streamed whole rows through a shared-memory ring, one CTA a row, took
 // 244 us there but 119 against 113 for 2048 rows of 65536; it did not stay. A short call (8
@@ -17,6 +17,12 @@
 // Rows need not be aligned: a slice has a scalar head up to the first 16-byte boundary,
 // 16-byte accesses, and a scalar tail. The target's logit is read before the exchange, so
 // the gradient may overwrite the logits.
+//
+// The target is left out of maximum and sum (it counts as -inf there) and joins at the end: with
+// R = sum over the others and e = exp(x_target - m),
+//   d loss / d x_target = -a_i / n_i R / (R + e),   nll = log1p(R) where the target is the maximum.
+// A likely token has R far below 1; a sum that holds its 1 keeps R to 6e-8 only, and p - 1 and
+// log(sum) lose the rest (a tenth of both at 1 - p = 1e-6, all of them below 6e-8).
 //
 // The maximum is subtracted before the scaling by log2 e: with the product first (one FMA a
 // logit less) masks at the type's lowest value overflow, and logits past 2^24 lose the
@@ -128,25 +134,57 @@ __device__ __forceinline__ F2 exp2_of(F2 a) {
   a.split(x, y);
   return F2(ex2(x), ex2(y));
 }
-// One 16-byte vector as pairs.
-__device__ __forceinline__ void load_pairs(const float* p, F2 (&x)[2], float& top) {
-  const float4 u = *reinterpret_cast<const float4*>(p);
-  top = fmaxf(top, fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w)));
-  x[0] = F2(u.x, u.y);
-  x[1] = F2(u.z, u.w);
-}
-__device__ __forceinline__ void load_pairs(const __nv_bfloat16* p, F2 (&x)[4], float& top) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// The largest of t and the elements of UN 16-byte vectors, NaN aside.
+template <int UN>
+__device__ __forceinline__ float top_of(const uint4* raw, float t, float) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float a = __uint_as_float(w[q] << 16), b = __uint_as_float(w[q] & 0xFFFF0000u);
-    top = fmaxf(top, fmaxf(a, b));
-    x[q] = F2(a, b);
-  }
+  for (int u = 0; u < UN; ++u)
+    t = fmaxf(t, fmaxf(fmaxf(__uint_as_float(raw[u].x), __uint_as_float(raw[u].y)),
+                       fmaxf(__uint_as_float(raw[u].z), __uint_as_float(raw[u].w))));
+  return t;
+}
+template <int UN>
+__device__ __forceinline__ float top_of(const uint4* raw, float t, __nv_bfloat16) {
+  auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+  __nv_bfloat162 p = __hmax2(__hmax2(pair(raw[0].x), pair(raw[0].y)), __hmax2(pair(raw[0].z), pair(raw[0].w)));
+#pragma unroll
+  for (int u = 1; u < UN; ++u)
+    p = __hmax2(p, __hmax2(__hmax2(pair(raw[u].x), pair(raw[u].y)), __hmax2(pair(raw[u].z), pair(raw[u].w))));
+  return fmaxf(t, fmaxf(__low2float(p), __high2float(p)));
+}
+// Pair k of a 16-byte vector (4 floats or 8 bf16).
+template <typename T>
+__device__ __forceinline__ F2 pair_of(const uint4& u, int k) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if (sizeof(T) == 4) return F2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+  return F2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xFFFF0000u));
 }
 
-// The packed instructions (273 -> 260 us) leave registers for a fifth CTA an SM.
+// This CTA's columns [c0, c1) of a row at x; from v0 on they hold nv whole 16-byte vectors. Slices
+// meet at 16-byte boundaries.
+template <typename T>
+struct Slice { int c0, c1, v0, nv; };
+template <typename T>
+__device__ __forceinline__ Slice<T> slice_of(const T* x, int64_t V) {
+  constexpr int N = Vec<T>::N;
+  const uint32_t C = cluster_size(), rank = cluster_rank();
+  const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T);   // to the row's first boundary
+  const int64_t per = ((V + C - 1) / C + N - 1) / N * N;
+  auto cut = [&](uint32_t r) {
+    const int64_t c = r == 0 ? 0 : head + r * per;
+    return static_cast<int>(c < V ? (r == C ? V : c) : V);            // V < 2^31
+  };
+  Slice<T> s;
+  s.c0 = cut(rank);
+  s.c1 = cut(rank + 1);
+  s.v0 = rank == 0 ? min(static_cast<int>(head), s.c1) : s.c0;
+  s.nv = (s.c1 - s.v0) / N;
+  return s;
+}
+
+// The packed instructions (273 -> 260 us) leave registers for a fifth CTA an SM. 48 registers are all
+// there are: a vector stays as it was read until its exponentials are formed, and the largest of bf16 is
+// taken two by two, or the loops spill (272 us).
 // grid: ntok * cluster size; row = blockIdx.x / cluster size.
 template <typename T>
 __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t ld, int64_t V,
@@ -162,55 +200,79 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
   // so here, and the wait comes after pass one, which hides it.
   if (C > 1) cluster_arrive_relaxed();
   const int64_t row = blockIdx.x / C;
-  int si = 0;                                         // the row's sequence
-  while (si + 1 < seqs.n && seqs.start[si + 1] <= row) ++si;
-  const double w = seqs.w[si];
   const T* x = logits + row * ld;
-  T* g = grad + row * ld_grad;
   const int32_t target = targets[row];
-  const bool valid = target >= 0 && target < V;
 
-  // this CTA's columns [c0, c1); [v0, v1) of them are whole 16-byte vectors
-  const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T);   // to the row's first boundary
-  const int64_t per = ((V + C - 1) / C + N - 1) / N * N;
-  auto cut = [&](int64_t r) {                         // slices meet at 16-byte boundaries
-    const int64_t c = r == 0 ? 0 : head + r * per;
-    return c < V ? (r == C ? V : c) : V;
-  };
-  const int64_t c0 = cut(rank), c1 = cut(rank + 1);
-  const int64_t v0 = rank == 0 ? (head < c1 ? head : c1) : c0;
-  const int64_t nvec = (c1 - v0) / N, v1 = v0 + nvec * N;
-  const bool same = (reinterpret_cast<uintptr_t>(g + v0) & 15) == 0;   // the gradient's row has the same phase
-
-  const float xt = (tid == 0 && valid) ? Vec<T>::one(x + target) : 0.f;
+  __shared__ float target_logit;
+  __shared__ double row_weight;
   float m = -INFINITY, s = 0.f;
-  const T* xv = x + v0;
-  const int nv = static_cast<int>(nvec);
-  // UN vectors a thread: one maximum and one rescaling of the running sum for all of them
-  auto block = [&](auto un, int i) {
+  const Slice<T> sl = slice_of(x, V);
+  const T* xv = x + sl.v0;
+  const int nv = sl.nv;
+  auto vec = [&](int i) { return *reinterpret_cast<const uint4*>(xv + static_cast<int64_t>(i) * N); };
+  // UN vectors of a thread join (m, s): one maximum and one rescaling of the running sum for all of them
+  auto joined = [&](auto un, const uint4* raw) {
     constexpr int UN = decltype(un)::value;
-    F2 y[UN][N / 2];
-    float t = m;
-#pragma unroll
-    for (int u = 0; u < UN; ++u) load_pairs(xv + static_cast<int64_t>(i + u * nt) * N, y[u], t);
+    const float t = top_of<UN>(raw, m, T());
     const float b = t == -INFINITY ? 0.f : t;         // -inf logits alone: every exponential is 0
     const F2 nb(-b, -b), le(kLog2e, kLog2e);
     F2 acc(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
-      for (int k = 0; k < N / 2; ++k) acc = acc + exp2_of((y[u][k] + nb) * le);
+      for (int k = 0; k < N / 2; ++k) acc = acc + exp2_of((pair_of<T>(raw[u], k) + nb) * le);
     float a0, a1;
     acc.split(a0, a1);
-    s = s * exp_of(m - b) + (a0 + a1);
-    m = t;
+    return make_float2(t, s * exp_of(m - b) + (a0 + a1));
   };
+  // The first loads are under way before anything asks for the target's id.
   int i = tid;
-  for (; i + 3 * nt < nv; i += 4 * nt) block(std::integral_constant<int, 4>{}, i);
-  for (; i < nv; i += nt) block(std::integral_constant<int, 1>{}, i);
-  if (tid < 2 * N) {                                  // head and tail, one element a thread
-    const int64_t c = tid < N ? c0 + tid : v1 + (tid - N);
-    if (c < (tid < N ? v0 : c1)) {
+  uint4 raw[4];
+  const bool blocks = i + 3 * nt < nv;
+  if (blocks) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) raw[u] = vec(i + u * nt);
+  }
+  const bool valid = target >= 0 && target < V;
+  const float xt0 = tid == 0 && valid ? Vec<T>::one(x + target) : -INFINITY;
+  // The vector that holds the target (-1: none of this slice): the loops leave it out, and its other
+  // elements are taken one by one.
+  const int tv = valid && target >= sl.v0 && target < sl.v0 + nv * N ? (target - sl.v0) / N : -1;
+  // and the first vector of this thread's block with it (nt is a power of two)
+  const int hit = tv >= 0 && ((tv - tid) & (nt - 1)) == 0 ? tv - ((tv - tid) & (4 * nt - 1)) : -1;
+  if (blocks)
+    while (true) {
+      if (i == hit) {
+        const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;              // -inf
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i + u * nt == tv) raw[u] = make_uint4(none, none, none, none);
+      }
+      const float2 z = joined(std::integral_constant<int, 4>{}, raw);
+      m = z.x;
+      s = z.y;
+      i += 4 * nt;
+      if (i + 3 * nt >= nv) break;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) raw[u] = vec(i + u * nt);
+    }
+#pragma unroll
+  for (int u = 0; u < 3; ++u) raw[u] = i + u * nt < nv ? vec(i + u * nt) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int u = 0; u < 3; ++u)
+    if (i + u * nt < nv && i + u * nt != tv) {
+      const float2 z = joined(std::integral_constant<int, 1>{}, raw + u);
+      m = z.x;
+      s = z.y;
+    }
+  const int64_t c0 = sl.c0, c1 = sl.c1, v0 = sl.v0, v1 = v0 + static_cast<int64_t>(nv) * N;
+  T* g = grad + row * ld_grad;
+  const bool same = (reinterpret_cast<uintptr_t>(g + v0) & 15) == 0;   // the gradient's row has the same phase
+  if (tid < (tv < 0 ? 2 : 3) * N) {                   // head, tail and target's vector, one element a thread
+    int64_t c = c0 + tid, end = v0;
+    if (tid >= N) c = v1 + (tid - N), end = c1;
+    if (tid >= 2 * N) c = v0 + static_cast<int64_t>(tv) * N + (tid - 2 * N), end = v1;
+    if (c < end && (c != target || !valid)) {
       const float y = Vec<T>::one(x + c);
       merge(m, s, y, y == -INFINITY ? 0.f : (y == y ? 1.f : y));
     }
@@ -218,6 +280,12 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
   if ((tid & 31) == 0) red[tid >> 5] = make_float2(m, s);
+  if (tid == 0) {
+    target_logit = xt0;
+    int si = 0;                                       // the row's sequence
+    while (si + 1 < seqs.n && seqs.start[si + 1] <= row) ++si;
+    row_weight = seqs.w[si];
+  }
   __syncthreads();
   // every warp merges the warps' pairs, then the CTAs' (lanes past them hold the empty pair)
   const int lane = tid & 31;
@@ -237,10 +305,17 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
     m = __shfl_sync(0xffffffffu, m, 0);
     s = __shfl_sync(0xffffffffu, s, 0);
   }
+  // the target joins: s = rest + its exponential
+  const float xt = target_logit, top = fmaxf(m, xt);
+  const float rest = m == -INFINITY ? s : s * exp_of(m - top);          // nothing but the target: 0, or a NaN
+  s = rest + exp_of(xt - top);
+  m = top;
+  const double w = row_weight;
   const float bad = __int_as_float(0x7fc00000);
   if (rank == 0 && tid == 0) {
     // the difference first: at the type's lowest value even fp64 would swallow log s
-    const double nll = (static_cast<double>(m) - static_cast<double>(xt)) + log(static_cast<double>(s));
+    const double nll = m == xt && s == s ? log1p(static_cast<double>(rest))
+                                         : (static_cast<double>(m) - static_cast<double>(xt)) + log(static_cast<double>(s));
     term[row] = valid ? nll * w : static_cast<double>(bad);
   }
   const float wf = valid ? static_cast<float>(w * grad_scale) : bad;
@@ -251,9 +326,12 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
     auto pass = [&](auto un, int i) {
       constexpr int UN = decltype(un)::value;
       F2 y[UN][N / 2];
-      float unused = 0.f;
 #pragma unroll
-      for (int u = 0; u < UN; ++u) load_pairs(xv + static_cast<int64_t>(i + u * nt) * N, y[u], unused);
+      for (int u = 0; u < UN; ++u) {
+        const uint4 q = vec(i + u * nt);
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) y[u][k] = pair_of<T>(q, k);
+      }
       const F2 nm(-m, -m), le(kLog2e, kLog2e), ww(wf * inv, wf * inv);
 #pragma unroll
       for (int u = 0; u < UN; ++u) {
@@ -280,7 +358,7 @@ __global__ void __launch_bounds__(256, 5) k_loss_grad(const T* logits, int64_t l
   }
   __syncthreads();                                    // the target's element, once the slice is written
   // xt was read before the first barrier, so before any gradient was written
-  if (tid == 0 && valid && target >= c0 && target < c1) Vec<T>::put(g + target, wf * (exp_of(xt - m) * inv - 1.f));
+  if (tid == 0 && valid && target >= c0 && target < c1) Vec<T>::put(g + target, -wf * (rest / s));
 }
 
 // loss[0] = the terms' sum in fp64 in token order (each thread a contiguous run, the runs in
