@@ -211,12 +211,12 @@ size_t grouped_smem(gr::Args& a, int64_t nk) {
   return static_cast<size_t>(fixed) + static_cast<size_t>(a.stages) * SB;
 }
 
-template <int BNT, int MODE, bool PAIR, bool F32, int EW = 8>
+template <int BNT, int MODE, bool PAIR, bool SUM, int EW = 8>
 int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, int64_t tiles, int64_t nk,
                    int sms, const char* what, cudaStream_t s) {
   const size_t smem = grouped_smem<BNT, MODE, PAIR, EW>(a, nk);
   a.wait_ns = static_cast<uint64_t>(g_wait_ns.load(std::memory_order_relaxed));
-  auto* kernel = gr::k_grouped<BNT, MODE, PAIR, F32, EW>;
+  auto* kernel = gr::k_grouped<BNT, MODE, PAIR, SUM, EW>;
   int* err = nullptr;
   int rc = wait_err(&err);
   if (rc) return rc;
@@ -248,12 +248,12 @@ int launch_grouped(gr::Args a, const CUtensorMap& A, const CUtensorMap& B, const
   return e == cudaSuccess ? DSMZ_OK : cuda_fail(what, e);
 }
 
-template <int MODE, bool F32>
+template <int MODE, bool SUM>
 int launch_grouped_bn(int bnt, const gr::Args& a, const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C,
                       int64_t tiles, int64_t nk, int sms, const char* what, cudaStream_t s) {
-  if (bnt == 64) return launch_grouped<64, MODE, false, F32>(a, A, B, C, tiles, nk, sms, what, s);
-  if (bnt == 128) return launch_grouped<128, MODE, false, F32>(a, A, B, C, tiles, nk, sms, what, s);
-  return launch_grouped<256, MODE, false, F32>(a, A, B, C, tiles, nk, sms, what, s);
+  if (bnt == 64) return launch_grouped<64, MODE, false, SUM>(a, A, B, C, tiles, nk, sms, what, s);
+  if (bnt == 128) return launch_grouped<128, MODE, false, SUM>(a, A, B, C, tiles, nk, sms, what, s);
+  return launch_grouped<256, MODE, false, SUM>(a, A, B, C, tiles, nk, sms, what, s);
 }
 
 // Accumulator width for n output columns and `rows` row tiles: 256 columns where that still
@@ -394,13 +394,14 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     a.zero_rest = (flags & DSMZ_GROUPED_ZERO_REST) && !a.accumulate;
     a.vec = aligned(out, 16) && (ld_out * es) % 16 == 0;
     a.alpha = alpha;
-    a.chunk = a.out_f32 ? gr::kChunk : 0x3fffffff;
     const int64_t rows = (M + gr::kBM - 1) / gr::kBM + (G < M ? G : M) - 1;      // most row tiles the groups can have
     const int bnt = columns_for(N, rows, sms);
     a.bn = static_cast<int32_t>(N >= bnt ? bnt : (N + 15) / 16 * 16);
     a.ntn = static_cast<int32_t>((N + a.bn - 1) / a.bn);
     const int64_t nk = (K + gr::kBK - 1) / gr::kBK;
     a.split = split_for(bnt, rows * a.ntn, nk);
+    const bool sum = a.out_f32 || (nk + a.split - 1) / a.split > gr::kLong;
+    a.chunk = sum ? gr::kChunk : 0x3fffffff;
     // Pairs of CTAs where the products, not the output, take a tile's time and the groups are long
     // enough for 256-row tiles. 8192 x 3584 x 18944 in 8 ragged groups (9% of the tiles' rows are
     // empty, 5% with 128-row tiles): 826 us with pairs and 856 without in a short run, 1014 and
@@ -423,14 +424,14 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
         !(a.b_slabs ? encode_map(&B, w, 4, ds, ss, 64, 64, false, (bcols + 63) / 64)
                     : encode_map(&B, w, 3, db, sb, 64, w_n_contiguous ? 64 : bcols)))
       return fail(DSMZ_ERR_CUDA, me + "the driver refused a tensor map");
-    if (a.vec && !a.accumulate && a.split == 1) {
+    if (a.vec && !a.accumulate && a.split == 1 && (a.out_f32 || !sum)) {
       const uint64_t dc[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(M), 1};
       const uint64_t sc[2] = {static_cast<uint64_t>(ld_out) * es, static_cast<uint64_t>(ld_out) * es * M};
       a.tma_out = encode_map(&C, out, 3, dc, sc, 128 / es, 32, a.out_f32 != 0);
     }
     const char* what = "dsmz_grouped_matmul";
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a.out_f32)
+    if (sum)
       return pair ? launch_grouped<256, 0, true, true>(a, A, B, C, tiles, nk, sms, what, s)
                   : launch_grouped_bn<0, true>(bnt, a, A, B, C, tiles, nk, sms, what, s);
     // Few k-steps and short groups: a tile's epilogue sets the pace, and 16 warps shorten it. K = 64, N =

@@ -20,10 +20,11 @@
 // output row depends on its own input row; rows past the group are not stored), and cleared
 // in shared memory before the last k-step's MMAs in MODE 1, where they would be summed.
 //
-// fp32 outputs: the tensor core's accumulator rounds towards zero, which shows after some
-// hundred additions; every kChunk k-steps the epilogue therefore takes the accumulator into
-// registers and adds the chunks with rounding to nearest. bf16 outputs (half a step 2^-9 of
-// the value) do not need it.
+// The tensor core's accumulator rounds towards zero: an addition of 16 products loses 2^-22.3 of the
+// running sum on average (measured: 5% of a sum of one sign after 2^19 additions). For fp32 outputs
+// the epilogue therefore takes the accumulator into registers every kChunk k-steps and adds the
+// chunks with rounding to nearest. bf16 outputs do without up to kLong k-steps a CTA, where a sum of
+// one sign has lost 2^-12 of itself (half a step is 2^-9 to 2^-8), and are summed likewise beyond.
 //
 // Few tiles (narrow outputs): a cluster of 2 to 8 CTAs splits the contraction; each CTA copies its
 // partial tile to the CTAs that own the rows (bulk copies through distributed shared memory,
@@ -63,7 +64,8 @@ using tc::kBM;
 
 constexpr int kMaxGroups = 1024;
 constexpr int kFirstEpi = 4;            // first epilogue warp (a multiple of 4: warp % 4 is the TMEM lane quadrant)
-constexpr int kChunk = 8;               // k-steps (512 products) an accumulator takes for fp32 outputs
+constexpr int kChunk = 8;               // k-steps (512 products) an accumulator takes where chunks are summed
+constexpr int kLong = 512;              // k-steps of a CTA beyond which bf16 outputs are summed in chunks
 constexpr int kStagePitch = 80;         // bytes of a staged 64-byte row piece (conflict-free 16-byte accesses)
 constexpr int kStageBytes = 4096;       // staging of an epilogue warp: 32 rows of 128 bytes
 constexpr int kABytes = kBM * kBK * 2;
@@ -421,13 +423,13 @@ __device__ __noinline__ void fill_nan(const Args& a, int seg, int m0, int r0, in
 
 // BNT: columns of the accumulators (64, 128 or 256; a.bn <= BNT). mapC: the output (3-D, boxes
 // of 32 rows x 128 bytes) where a.tma_out.
-// F32: the type of the output (MODE 1: fp32). EW: epilogue warps, 8, or 16 where a tile of 256 columns
+// SUM: accumulators are summed in registers (fp32 outputs; bf16 ones of long contractions). EW: epilogue warps, 8, or 16 where a tile of 256 columns
 // has only a few k-steps and its epilogue sets the pace.
 // PAIR (MODE 0, BNT 256): a cluster of two CTAs computes 256 x 256 tiles with cta_group::2 MMAs.
 // Each loads its 128 rows of A and 128 of B's rows, so a k-step costs 32 KB a CTA instead of 48;
 // the CTA of rank 0 (the leader) waits for both CTAs' loads on its barriers and issues, each CTA's
 // epilogue drains its own half.
-template <int BNT, int MODE, bool PAIR, bool F32, int EW>
+template <int BNT, int MODE, bool PAIR, bool SUM, int EW>
 __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __grid_constant__ CUtensorMap mapA,
                                                          const __grid_constant__ CUtensorMap mapB,
                                                          const __grid_constant__ CUtensorMap mapC,
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
       }
       const int kb = k_begin(x.nk), ke = k_end(x.nk);
       const int nrows = min(32, x.valid - q * 32);             // this warp's rows that exist
-      if (!F32 && S == 1) {
+      if (!SUM && S == 1) {
         // One accumulator a tile: it goes from TMEM to the output in pieces of 32 rows x 64 columns,
         // so that few registers are live. All of a warp's columns at once needed more than 168;
         // the spilled ones go to L2, since shared memory takes nearly all of L1 (4064 x 64 x 18944
@@ -855,7 +857,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
             p += a.ld;
           }
         }
-      } else if (rows16) {
+      } else if (rows16 && a.out_f32) {
         // fp32 pieces of 32 rows x 128 bytes as above; a.sbuf of them are staged, fenced and sent
         // together.
         const bool whole = a.tma_out && (MODE == 1 || nrows == 32);
@@ -887,7 +889,7 @@ __global__ void __launch_bounds__(32 * (kFirstEpi + EW), 1) k_grouped(const __gr
           }
         }
       } else {
-        // odd pitches and accumulation
+        // odd pitches, accumulation, and bf16 sums of chunks
         char* base = out + (static_cast<int64_t>(x.m0 + q * 32) * a.ld + x.n0 + col0) * es;
         if (lane == 0) store_read_wait();
         __syncwarp();
