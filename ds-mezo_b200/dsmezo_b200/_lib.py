@@ -209,6 +209,14 @@ def current_stream(index: int) -> int:
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
+def capturing(device) -> bool:
+    """Whether the stream that ``launch`` uses on this device is being captured."""
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device.index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def launch(what: str, device, fn, *args) -> None:
     """fn(*args, stream) on the device's current stream, with that device current; raises on an
     error status. The device is switched only where another is current: the switch costs a few

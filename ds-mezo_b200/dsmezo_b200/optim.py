@@ -197,7 +197,7 @@ class AdamW:
         if [p.data_ptr() for p in self._params] != self._pointers:
             raise RuntimeError("AdamW: a parameter's memory has been replaced since it was bound")
         d = self._desc
-        if self._counter is None and torch.cuda.is_current_stream_capturing():
+        if self._counter is None and _lib.capturing(self.device):
             raise RuntimeError("AdamW: a captured step would repeat one step number at every replay; "
                                "construct with capturable=True")
         d.lr_device = self._scalar(lr, "lr") if isinstance(lr, torch.Tensor) else None
