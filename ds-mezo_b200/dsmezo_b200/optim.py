@@ -129,8 +129,9 @@ class AdamW:
         self._counter = torch.full((1,), int(step), dtype=torch.int64, device=self.device) if capturable else None
         self._grads = None
         if grads is not None:
-            self._bind(grads)
             self._grads = tuple(grads)
+            self._check_grads(self._grads)
+            self._put_grads(self._grads)
 
     # The C table holds their addresses, so what they refer to is not exchanged.
     params = property(lambda self: self._params)
@@ -161,7 +162,7 @@ class AdamW:
         if s.bits != self.state_bits:
             raise ValueError("AdamW: states must be all fp32 or all 8-bit")
 
-    def _bind(self, grads: Sequence[torch.Tensor]) -> None:
+    def _check_grads(self, grads: Sequence[torch.Tensor]) -> None:
         if len(grads) != len(self.params):
             raise ValueError("AdamW: one gradient a parameter")
         dt = grads[0].dtype
@@ -173,9 +174,12 @@ class AdamW:
             k = bisect.bisect_left(self._starts, hi)       # the last written range that starts before g ends
             if lo < hi and k > 0 and self._written[k - 1][1] > lo:
                 raise ValueError("AdamW: a gradient overlaps a parameter, state or shadow")
-        for e, g in zip(self._table, grads):               # only once all are good: a refused call changes nothing
+
+    def _put_grads(self, grads: Sequence[torch.Tensor]) -> None:
+        """Into the C table."""
+        for e, g in zip(self._table, grads):
             e.grad = g.data_ptr()
-        self._desc.grad_dtype = _DT[dt]
+        self._desc.grad_dtype = _DT[grads[0].dtype]
 
     def _scalar(self, t: Optional[torch.Tensor], what: str) -> Optional[int]:
         if t is None:
@@ -190,8 +194,8 @@ class AdamW:
         one-element fp32 device tensor; grad_scale: one-element fp32 device tensor that
         multiplies every gradient (a clipping or loss-scale factor)."""
         if grads is not None:
-            self._bind(grads)
-            self._grads = None                   # a later step() must be given its own again
+            grads = tuple(grads)
+            self._check_grads(grads)
         elif self._grads is None:
             raise ValueError("AdamW: no gradients bound; give them to step()")
         if [p.data_ptr() for p in self._params] != self._pointers:
@@ -211,8 +215,17 @@ class AdamW:
         if d.step_counter or d.lr_device:
             ws = torch.empty(_lib.ADAMW_WORKSPACE_BYTES, dtype=torch.uint8, device=self.device)
             nbytes = ws.numel()
-        _lib.launch("adamw_step", self.device, lib().dsmz_adamw_step, ctypes.byref(d), self._table, len(self.params),
-                    None if ws is None else ws.data_ptr(), nbytes)
+        if grads is not None:
+            self._put_grads(grads)
+        try:
+            _lib.launch("adamw_step", self.device, lib().dsmz_adamw_step, ctypes.byref(d), self._table,
+                        len(self.params), None if ws is None else ws.data_ptr(), nbytes)
+        except _lib.DsmzError:
+            if grads is not None and self._grads is not None:
+                self._put_grads(self._grads)     # a refused step changes nothing
+            raise
+        if grads is not None:
+            self._grads = None                   # a later step() must be given its own again
         if self._counter is None:
             self.step_count += 1
 
