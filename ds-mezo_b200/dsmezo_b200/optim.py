@@ -52,6 +52,10 @@ class AdamWState:
         return 32 if self.m.dtype == torch.float32 else 8
 
 
+def _addresses(tensors: Sequence[torch.Tensor]) -> list:
+    return list(map(torch.Tensor.data_ptr, tensors))     # 60 ns a tensor
+
+
 def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
 
@@ -67,7 +71,11 @@ class AdamW:
     and capturing a step is refused, since its replays would repeat one step number.
 
     The tensors are bound once (``params``, ``states``, ``shadows``, ``grads`` and
-    ``step_counter`` are read-only; what they hold may be written). ``lr``, ``betas``, ``eps``,
+    ``step_counter`` are read-only; what they hold may be written). A step that finds the memory
+    of one exchanged (``tensor.data = ...``) is refused: that of a parameter, gradient or shadow at
+    once, that of a state within len(params) / 4 steps (each step looks at four parameters' states;
+    until then it works on the old memory, which stays allocated). A captured step cannot look.
+    ``lr``, ``betas``, ``eps``,
     ``weight_decay`` and ``step_count`` may be set between steps.
     """
 
@@ -124,7 +132,13 @@ class AdamW:
             if sh is not None:
                 e.shadow = sh.data_ptr()
         self._desc = AdamWDesc(param_dtype=_DT[p0.dtype], state_bits=self.state_bits)
-        self._pointers = [p.data_ptr() for p in self.params]
+        # what the table holds the addresses of: a tensor's memory may be exchanged under it
+        self._state_tensors = tuple(t for s in self.states for t in (s.m, s.v, s.m_scale, s.v_scale) if t is not None)
+        self._state_pointers = _addresses(self._state_tensors)
+        self._kept = tuple(map(torch.Tensor.untyped_storage, self._state_tensors))
+        self._window, self._look = 4 * (2 if self.state_bits == 32 else 4), 0
+        self._bound = (*self.params, *(t for t in self.shadows if t is not None))
+        self._pointers = _addresses(self._bound)
         self.step_count = int(step)              # steps taken (host count; not moved when capturable)
         self._counter = torch.full((1,), int(step), dtype=torch.int64, device=self.device) if capturable else None
         self._grads = None
@@ -132,6 +146,7 @@ class AdamW:
             self._grads = tuple(grads)
             self._check_grads(self._grads)
             self._put_grads(self._grads)
+            self._grad_pointers = _addresses(self._grads)
 
     # The C table holds their addresses, so what they refer to is not exchanged.
     params = property(lambda self: self._params)
@@ -198,8 +213,13 @@ class AdamW:
             self._check_grads(grads)
         elif self._grads is None:
             raise ValueError("AdamW: no gradients bound; give them to step()")
-        if [p.data_ptr() for p in self._params] != self._pointers:
-            raise RuntimeError("AdamW: a parameter's memory has been replaced since it was bound")
+        elif _addresses(self._grads) != self._grad_pointers:
+            raise RuntimeError("AdamW: a gradient's memory has been replaced since it was bound")
+        if _addresses(self._bound) != self._pointers:
+            raise RuntimeError("AdamW: the memory of a parameter or shadow has been replaced since it was bound")
+        a, b = self._look, self._look + self._window           # all of them would cost a small step a quarter more
+        if _addresses(self._state_tensors[a:b]) != self._state_pointers[a:b]:
+            raise RuntimeError("AdamW: a state's memory has been replaced since it was bound")
         d = self._desc
         if self._counter is None and _lib.capturing(self.device):
             raise RuntimeError("AdamW: a captured step would repeat one step number at every replay; "
@@ -224,6 +244,7 @@ class AdamW:
             if grads is not None and self._grads is not None:
                 self._put_grads(self._grads)     # a refused step changes nothing
             raise
+        self._look = b if b < len(self._state_tensors) else 0
         if grads is not None:
             self._grads = None                   # a later step() must be given its own again
         if self._counter is None:
@@ -237,10 +258,10 @@ class AdamW:
         n = len(self.params)
         if len(m_out) != n or len(v_out) != n:
             raise ValueError("AdamW: one output a parameter")
-        index = self.device.index
+        at, T = [self.device.index] * n, torch.Tensor
         for outs in (m_out, v_out):
-            if [t.numel() for t in outs] != self._numels or any(
-                    t.dtype != torch.float32 or t.get_device() != index or not t.is_contiguous() for t in outs):
+            if list(map(T.numel, outs)) != self._numels or list(map(T.get_device, outs)) != at or \
+                    {t.dtype for t in outs} != {torch.float32} or not all(map(T.is_contiguous, outs)):
                 raise ValueError("AdamW: state values go to contiguous float32 tensors of the parameters' sizes")
         table = type(self._table).from_buffer_copy(self._table)
         words = np.frombuffer(table, dtype=np.int64).reshape(n, -1)       # rows of 64-bit words: no loop over tensors
