@@ -275,13 +275,15 @@ class AdapterSet:
         whose ``directions`` copies each own the rows [row_offsets[k], row_offsets[k + 1]) (int32
         on the device; may be left out for a single copy). out, accumulate: add to the base
         module's output in place. Runs on the current stream; see ``grouped.adapter_forward``. NaN
-        where a wait of a kernel ran out of time (``device_error``)."""
+        where a wait of a kernel ran out of time (``device_error``). Records no autograd graph, and
+        refuses tensors that ask for one: call it under ``torch.no_grad()``."""
         A, B = self._copies(i, which)
         return grouped.adapter_forward(x, A, B, self._rows(x, row_offsets, A.shape[0]), out=out, alpha=alpha,
                                        accumulate=accumulate)
 
     def delta_backward(self, i: int, dy: torch.Tensor, x: torch.Tensor, t: torch.Tensor, grad: torch.Tensor, *,
-                       row_offsets: Optional[torch.Tensor] = None, alpha: float = 1.0, accumulate: bool = False, need_dx: bool = True) -> Optional[torch.Tensor]:
+                       row_offsets: Optional[torch.Tensor] = None, alpha: float = 1.0, accumulate: bool = False,
+                       need_dx: bool = True) -> Optional[torch.Tensor]:
         """Gradients of ``delta(i, x, 'shadow', row_offsets)``: writes (accumulate: adds) those of A and
         B into module i's part of the gradient arena and returns the one in x (None without need_dx;
         zero in rows outside the offsets). row_offsets: those that ``delta`` was given; rows outside

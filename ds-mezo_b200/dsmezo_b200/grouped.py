@@ -10,6 +10,11 @@ operands, fp32 sums on the tensor cores. The same entry points serve any set of 
 A kernel whose barriers do not complete within a limit (``set_wait_limit``, 1 s at first: a
 preempted device, a defect) returns all the same: the parts of its output that it did not produce
 are NaN, and ``device_error`` (or ``AdapterSet.device_error``) tells of it. Later calls run as usual.
+
+Nothing here records an autograd graph. A forward product of tensors that require grad, with grad
+mode on, is refused, since its result would silently drop out of the graph: call it under
+``torch.no_grad()`` and take the gradients from ``grouped_matmul`` of the other layout and
+``grouped_weight_grad``, for instance in the backward of a ``torch.autograd.Function``.
 """
 from __future__ import annotations
 
@@ -98,6 +103,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, row_offsets: torch.Tensor, 
     elif tuple(out.shape) != (M, N) or out.dtype not in _DT or out.device != x.device or \
             (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
         raise ValueError(f"{me}: out must be M x N float32 or bfloat16 with unit column stride, on x's device")
+    if (x.requires_grad or w.requires_grad or out.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError(f"{me} records no autograd graph: call it under torch.no_grad(), or in the forward of a "
+                           "torch.autograd.Function whose backward calls grouped_matmul and grouped_weight_grad")
     if M == 0:
         return out
     w, gs, ld, nc = _weights(w, me)

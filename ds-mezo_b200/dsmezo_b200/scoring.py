@@ -75,7 +75,8 @@ def contrastive_loss_grad(logits: torch.Tensor, seq_tokens: Sequence[int], advan
     the logits' shape and type, grad_scale * d loss / d logits, written on the current stream.
     out: where the gradient goes; it may be the logits themselves. NaN where a target lies
     outside the vocabulary (the loss and that row). A likely token's loss and gradient, 1 - p, are
-    right to their own size, however small. seq_tokens, advantages and grad_scale are
+    right to their own size, however small. Neither result records an autograd graph: the backward
+    pass goes on with ``logits.backward(grad)``. seq_tokens, advantages and grad_scale are
     read during the call: a captured call replays with the same ones."""
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
         raise ValueError("contrastive_loss_grad takes CUDA tensors only (no CPU fallback)")
