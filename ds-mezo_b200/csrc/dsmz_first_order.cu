@@ -306,10 +306,17 @@ int split_for(int bnt, int64_t tiles, int64_t nk) {
   return 1;
 }
 
-bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
+// Whether `rows` rows of `na` bytes at a and of `nb` bytes at b share a byte; rows of one pitch may lie
+// side by side in a wider buffer. With two pitches: whether their ranges meet.
+bool rows_meet(const void* a, int64_t na, int64_t pitch_a, const void* b, int64_t nb, int64_t pitch_b, int64_t rows) {
+  const int64_t x = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a)), y = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b));
+  const int64_t all_a = (rows - 1) * pitch_a + na, all_b = (rows - 1) * pitch_b + nb;
+  if (x + all_a <= y || y + all_b <= x) return false;
+  if (rows < 2 || pitch_a != pitch_b) return true;
+  const int64_t d = ((y - x) % pitch_a + pitch_a) % pitch_a;   // where b's rows begin between two of a's
+  return d < na || d + nb > pitch_a;
 }
+bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) { return rows_meet(a, na, 0, b, nb, 0, 1); }
 
 // ------------------------------------------------------------------ scoring loss with its gradient
 template <typename T>
@@ -375,7 +382,7 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
     if (!aligned(out, es) || !aligned(row_offsets, 4)) return fail(DSMZ_ERR_INVALID, me + "a pointer is not aligned to its type");
     if (!std::isfinite(alpha)) return fail(DSMZ_ERR_INVALID, me + "alpha must be finite");
     const int64_t nout = ((M - 1) * ld_out + N) * es;
-    if (overlaps(out, nout, x, ((M - 1) * ld_x + K) * 2) || overlaps(out, nout, w, ((G - 1) * w_group_stride + (wo - 1) * w_ld + wi) * 2))
+    if (rows_meet(out, N * es, ld_out * es, x, K * 2, ld_x * 2, M) || overlaps(out, nout, w, ((G - 1) * w_group_stride + (wo - 1) * w_ld + wi) * 2))
       return fail(DSMZ_ERR_INVALID, me + "out overlaps an operand");
     int sms = 0, rc = sm_count(&sms);
     if (rc) return rc;
@@ -552,9 +559,7 @@ int dsmz_contrastive_loss_grad(int32_t kind, const void* logits, int64_t V, int6
     const int64_t es = kind == DSMZ_SCORE_LOGITS_F32 ? 4 : 2;
     if (!aligned(logits, es) || !aligned(grad, es) || !aligned(targets, 4) || !aligned(loss, 4))
       return fail(DSMZ_ERR_INVALID, me + "a pointer is not aligned to its element type");
-    const uintptr_t a = reinterpret_cast<uintptr_t>(logits), b = reinterpret_cast<uintptr_t>(grad);
-    const uintptr_t na = static_cast<uintptr_t>(((ntok - 1) * ld + V) * es), nb = static_cast<uintptr_t>(((ntok - 1) * ld_grad + V) * es);
-    if (a < b + nb && b < a + na && !(a == b && (ld == ld_grad || ntok == 1)))
+    if (rows_meet(logits, V * es, ld * es, grad, V * es, ld_grad * es, ntok) && !(logits == grad && (ld == ld_grad || ntok == 1)))
       return fail(DSMZ_ERR_INVALID, me + "the gradient may overwrite the logits in place, not overlap them otherwise");
     sg::Seqs q{};
     q.n = nseq;

@@ -379,7 +379,8 @@ int dsmz_step_update_directions(const dsmz_plan* plan, const float* dd, int32_t 
  *                                              first with the same memory)
  * y: BF16 or F32, pitch ld_out. Rows outside every group stay as they are, or become zero
  * with DSMZ_GROUPED_ZERO_REST. x and w: 16-byte aligned, pitches and group stride multiples
- * of 8 elements (K and N themselves may be any size). y must not overlap x or w.
+ * of 8 elements (K and N themselves may be any size). y must share no element with x
+ * (rows of one pitch may lie side by side in a wider buffer) and not overlap w.
  * Deterministic; no workspace. A barrier wait inside the kernel that passes its limit (see
  * dsmz_first_order_set_wait_limit) leaves NaN in every part of y that was not produced and sets
  * the error word that dsmz_first_order_device_error reads; later calls are not affected. */
@@ -411,7 +412,7 @@ int dsmz_first_order_set_wait_limit(int64_t ns);
  *   grad[t][c] = grad_scale a_i / n_i (softmax(logits row t)[c] - [c == targets[t]])
  * logits (kind DSMZ_SCORE_LOGITS_F32 / _BF16) and grad have one type and unit column stride,
  * row pitches ld and ld_grad >= V, any alignment of their element type. grad may be the
- * logits' own buffer (same pitch); other overlaps are refused. Sequences, advantages and the
+ * logits' own buffer (same pitch) or lie beside it in a wider one; other overlaps are refused. Sequences, advantages and the
  * order of the sums as for dsmz_contrastive_loss; both are host arrays, so a captured call
  * keeps the ones it was captured with. A target outside [0, V) makes the loss and its row of
  * grad NaN. Deterministic. */
