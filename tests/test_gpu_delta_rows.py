@@ -52,6 +52,7 @@ def test_rows_outside_the_copy(first, end, accumulate):
     tol = torch.zeros_like(want)
     tol[s] = edt @ B.abs() + UB * (want[s].abs() + edt @ B.abs()) + 2 * aset.rank * U * (dt.abs() @ B.abs())
     assert bool(((dx.double() - want).abs() <= tol).all())           # zero outside the copy's rows
+    assert aset.device_error() == 0
 
 
 def test_without_offsets_every_row_counts():
@@ -64,3 +65,40 @@ def test_without_offsets_every_row_counts():
     dxa = aset.delta_backward(0, dy, x, t, a)
     dxb = aset.delta_backward(0, dy, x, t, b, row_offsets=off)
     assert torch.equal(a, b) and torch.equal(dxa, dxb)
+
+
+def test_a_captured_step_takes_new_offsets():
+    """Product, its gradients and AdamW in one graph, replayed with other offsets: as the same steps made
+    one by one on a second set."""
+    from dsmezo_b200 import AdamW
+    sets, opts, grads = [], [], []
+    for _ in range(2):
+        aset, g = make_set()
+        grad = aset.grad_arena()
+        sets.append(aset)
+        grads.append(grad)
+        opts.append(AdamW.for_adapters(aset, grad, lr=1e-2, capturable=True))
+    i = next(k for k, m in enumerate(sets[0].modules) if m.name == "gate_proj")
+    m = sets[0].modules[i]
+    x = torch.randn(26, m.d_in, generator=g, device=DEV).bfloat16()
+    dy = torch.randn(26, m.d_out, generator=g, device=DEV).bfloat16()
+    off = torch.tensor([0, 26], dtype=torch.int32, device=DEV)
+
+    def step(k, offsets):
+        _, t = sets[k].delta(i, x, row_offsets=offsets)
+        dx = sets[k].delta_backward(i, dy, x, t, grads[k], row_offsets=offsets)
+        opts[k].step()
+        return dx
+
+    step(0, off)                                          # outside the graph, as a program warms up
+    step(1, off)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx0 = step(0, off)
+    for first, end in ((2, 20), (0, 26), (25, 26), (7, 7), (0, 13)):
+        off.copy_(torch.tensor([first, end], dtype=torch.int32))
+        graph.replay()
+        dx1 = step(1, off.clone())
+        assert torch.equal(dx0, dx1) and torch.equal(grads[0], grads[1])
+        assert torch.equal(sets[0].factors, sets[1].factors) and torch.equal(sets[0].shadow, sets[1].shadow)
+    assert sets[0].device_error() == 0 and sets[1].device_error() == 0
