@@ -1,4 +1,4 @@
-// AdamW over many tensors in one launch, with fp32 or 8-bit states.
+// AdamW over many tensors, up to 256 in one launch, with fp32 or 8-bit states.
 //
 //   m <- b1 m + (1 - b1) g           v <- b2 v + (1 - b2) g^2
 //   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
@@ -20,7 +20,8 @@
 // fp32 with blocks near a border done again whole, 723 with single elements done again, no
 // conversions and a path without bounds for whole blocks, 608 with packed arithmetic, 576 in
 // CTAs of two warps. What bounds it is instruction issue and latency: 84 instructions an
-// element, 32 warps an SM.
+// element, 32 warps an SM of 64 registers, out of which a thread spills 64 to 72 bytes (116 to 136
+// read back) for its eight elements.
 // A block with a NaN or an infinity gets a scale that makes every element of the block NaN: the
 // whole block, not one element.
 //
@@ -564,7 +565,8 @@ __device__ __forceinline__ void step_block(const Args<CAP>& a, const Tensor& t, 
   }
 }
 
-// 8-bit states: four CTAs an SM (64 registers) took 628 us for a 7B set, three 739, five 840.
+// 8-bit states: 32 warps an SM, 64 registers a thread. (In CTAs of 256 threads, before packed
+// arithmetic: 628 us for a 7B set so, 739 with 24 warps, 840 with 40.)
 template <int CAP, typename P, typename G, int BITS>
 __global__ void __launch_bounds__(kThreadsAW, BITS == 8 ? 16 : 1) k_adamw(const __grid_constant__ Args<CAP> a) {
   const int ti = tensor_of(a, static_cast<int>(blockIdx.x));

@@ -443,7 +443,8 @@ int dsmz_grouped_matmul(const void* x, int64_t M, int64_t K, int64_t ld_x, const
                   : launch_grouped_bn<0, true>(bnt, a, A, B, C, tiles, nk, sms, what, s);
     // Few k-steps and short groups: a tile's epilogue sets the pace, and 16 warps shorten it. K = 64, N =
     // 18944, 32 groups of 64, 127, 160 rows: 28.0, 45.5, 52.8 us with 16 and 31.8, 46.7, 56.0 with 8;
-    // with 192, 256 and 512 rows, where the stores' bandwidth does, 68, 83, 142 and 56, 81, 139.
+    // with 192, 256 and 512 rows, where the stores' bandwidth does, 68, 83, 142 and 56, 81, 139. (Rows of
+    // no group count in M / G: the host does not know the offsets.)
     if (bnt == 256 && nk <= 4 && M / G <= 160) return launch_grouped<256, 0, false, false, 16>(a, A, B, C, tiles, nk, sms, what, s);
     return pair ? launch_grouped<256, 0, true, false>(a, A, B, C, tiles, nk, sms, what, s)
                 : launch_grouped_bn<0, false>(bnt, a, A, B, C, tiles, nk, sms, what, s);

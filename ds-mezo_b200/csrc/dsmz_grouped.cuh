@@ -31,16 +31,20 @@
 // counted on the owner's barrier), and the owner adds the partials in rank order. No atomics:
 // results are the same on every run.
 //
-// What bounds it, on one B200 (floors at the measured copy and bf16 rates):
-//   8192 x 3584 x 18944, 8 groups     826 us of 664 (1014 of 802 sustained): the power cap and
+// What bounds it, on one B200 (the public call back to back, of the floor at the measured copy and
+// bf16 rates):
+//   8192 x 3584 x 18944, 8 groups     942 us of 664 (802 at the sustained rate): the power cap and
 //                                     the empty rows of ragged last tiles
-//   4001 x 64 x 18944, 32 ragged      45 us of 36: the epilogue of half-filled last tiles, 5 us
+//   4001 x 64 x 18944, 32 ragged      47.6 us of 35.6: the epilogue of half-filled last tiles, 5 us
 //                                     until the first tile is stored
-//   4133 x 28672 x 128, 4 groups      54 us of 40: 36 tiles in clusters of 3 leave 40 SMs idle,
+//   4133 x 28672 x 128, 4 groups      60.6 us of 39.7: 36 tiles in clusters of 3 leave 40 SMs idle,
 //                                     5 us for the sum of the partial tiles
-//   4096 x 3584 x 64, 2 groups        11 us of 5; one row for each of 32 groups 11 us of 2: the
-//                                     chain of offsets (2 us), 14 k-steps (4), partial sums (2)
-//   dW of 4096 x (18944, 64)          31 us of 25: HBM, 3 us of stores after the last k-step
+//   4096 x 3584 x 64, 2 groups        11.7 us of 4.7; one row for each of 32 groups 11.7 us of 2.3: the
+//                                     host's call (12), and on the device the chain of offsets (2 us),
+//                                     14 k-steps (4), partial sums (2)
+//   dW of 4096 x (18944, 64)          31.6 us of 25.2: HBM, 3 us of stores after the last k-step
+// Accumulation leaves through put4, old values read beside the stores that follow them: 4001 x 64 x
+// 18944 takes 263 us (bf16) and 462 us (fp32; a new fp32 output 75).
 //
 // Every mbarrier wait gives up after Args::wait_ns (1 s unless the caller set another limit). The CTA
 // then raises a flag of its own, at which its other roles give up too; an accumulator that lacks

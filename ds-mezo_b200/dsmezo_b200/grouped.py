@@ -1,8 +1,8 @@
 """Matrix products grouped by adapter copy, with ragged rows (no reference counterpart).
 
-A scoring batch holds the rollouts of the + and - copies one behind the other (2K copies with
-K directions): rows sorted by copy, a device vector of row offsets, and one factor matrix a
-copy. ``grouped_matmul`` multiplies every group of rows by its own matrix, ``grouped_weight_grad``
+A scoring batch holds the rollouts of perturbed copies one behind the other: rows sorted by copy,
+a device vector of row offsets, and one factor matrix a copy (an AdapterSet's K + copies lie in one
+arena and its K - copies in another: a call for each). ``grouped_matmul`` multiplies every group of rows by its own matrix, ``grouped_weight_grad``
 forms the gradient of every matrix, and ``adapter_forward`` / ``adapter_backward`` combine them
 to the rank-r product of an adapter and its gradients. One launch for all groups; bf16
 operands, fp32 sums on the tensor cores. The same entry points serve any set of experts.

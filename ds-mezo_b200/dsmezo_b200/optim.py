@@ -1,8 +1,8 @@
-"""AdamW over many tensors in one launch, with fp32 or 8-bit states (first-order counterpart of
-the ZO-Muon update; the reference has none).
+"""AdamW over many tensors, up to 256 in one launch, with fp32 or 8-bit states (first-order
+counterpart of the ZO-Muon update; the reference has none).
 
 ``AdamW`` binds a list of parameters, their states and optionally fixed gradient buffers, as a
-plan binds an adapter set, and steps them all with one kernel (``dsmz_adamw_step``). An
+plan binds an adapter set, and steps them all in one call (``dsmz_adamw_step``). An
 ``AdapterSet`` goes in as one flat arena (``AdamW.for_adapters``): fp32 masters updated in
 place and the bf16 shadow that the rollout loads rewritten in the same pass, as the
 zeroth-order update does.
