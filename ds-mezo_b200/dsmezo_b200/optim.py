@@ -72,9 +72,9 @@ class AdamW:
 
     The tensors are bound once (``params``, ``states``, ``shadows``, ``grads`` and
     ``step_counter`` are read-only; what they hold may be written). A step that finds the memory
-    of one exchanged (``tensor.data = ...``) is refused: that of a parameter, gradient or shadow at
-    once, that of a state within len(params) / 4 steps (each step looks at four parameters' states;
-    until then it works on the old memory, which stays allocated). A captured step cannot look.
+    of one exchanged (``tensor.data = ...``) is refused: that of a parameter or gradient at once,
+    that of a state or shadow when its turn comes (each step looks at sixteen of these; until
+    then it works on the old memory, which stays allocated). A captured step cannot look.
     ``lr``, ``betas``, ``eps``,
     ``weight_decay`` and ``step_count`` may be set between steps.
     """
@@ -133,12 +133,11 @@ class AdamW:
                 e.shadow = sh.data_ptr()
         self._desc = AdamWDesc(param_dtype=_DT[p0.dtype], state_bits=self.state_bits)
         # what the table holds the addresses of: a tensor's memory may be exchanged under it
-        self._state_tensors = tuple(t for s in self.states for t in (s.m, s.v, s.m_scale, s.v_scale) if t is not None)
-        self._state_pointers = _addresses(self._state_tensors)
-        self._kept = tuple(map(torch.Tensor.untyped_storage, self._state_tensors))
-        self._window, self._look = 4 * (2 if self.state_bits == 32 else 4), 0
-        self._bound = (*self.params, *(t for t in self.shadows if t is not None))
-        self._pointers = _addresses(self._bound)
+        self._pointers = _addresses(self.params)
+        self._others = tuple(t for s, sh in zip(self.states, self.shadows)
+                             for t in (s.m, s.v, s.m_scale, s.v_scale, sh) if t is not None)
+        self._other_pointers, self._look = _addresses(self._others), 0
+        self._kept = tuple(map(torch.Tensor.untyped_storage, self._others))
         self.step_count = int(step)              # steps taken (host count; not moved when capturable)
         self._counter = torch.full((1,), int(step), dtype=torch.int64, device=self.device) if capturable else None
         self._grads = None
@@ -215,11 +214,11 @@ class AdamW:
             raise ValueError("AdamW: no gradients bound; give them to step()")
         elif _addresses(self._grads) != self._grad_pointers:
             raise RuntimeError("AdamW: a gradient's memory has been replaced since it was bound")
-        if _addresses(self._bound) != self._pointers:
-            raise RuntimeError("AdamW: the memory of a parameter or shadow has been replaced since it was bound")
-        a, b = self._look, self._look + self._window           # all of them would cost a small step a quarter more
-        if _addresses(self._state_tensors[a:b]) != self._state_pointers[a:b]:
-            raise RuntimeError("AdamW: a state's memory has been replaced since it was bound")
+        if _addresses(self._params) != self._pointers:
+            raise RuntimeError("AdamW: a parameter's memory has been replaced since it was bound")
+        a, b = self._look, self._look + 16       # all of them would double the host's time for many small tensors
+        if _addresses(self._others[a:b]) != self._other_pointers[a:b]:
+            raise RuntimeError("AdamW: the memory of a state or shadow has been replaced since it was bound")
         d = self._desc
         if self._counter is None and _lib.capturing(self.device):
             raise RuntimeError("AdamW: a captured step would repeat one step number at every replay; "
@@ -244,7 +243,7 @@ class AdamW:
             if grads is not None and self._grads is not None:
                 self._put_grads(self._grads)     # a refused step changes nothing
             raise
-        self._look = b if b < len(self._state_tensors) else 0
+        self._look = b if b < len(self._others) else 0
         if grads is not None:
             self._grads = None                   # a later step() must be given its own again
         if self._counter is None:

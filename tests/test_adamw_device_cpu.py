@@ -32,7 +32,7 @@ def stepped(monkeypatch, current, capturing, home, counter=None):
     made = []
     monkeypatch.setattr(_lib, "launch", lambda what, device, *a: made.append((what, device.index)))
     opt = optim.AdamW.__new__(optim.AdamW)
-    opt.__dict__.update(_params=(), _states=(), _shadows=(), _grads=(), _pointers=[], _numels=[], _bound=(), _grad_pointers=[], _state_tensors=(), _state_pointers=[], _window=8, _look=0, _table=None,
+    opt.__dict__.update(_params=(), _states=(), _shadows=(), _grads=(), _pointers=[], _numels=[], _grad_pointers=[], _others=(), _other_pointers=[], _look=0, _table=None,
                         _desc=optim.AdamWDesc(), _counter=counter, device=torch.device("cuda", home), lr=1e-3,
                         betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, step_count=0, state_bits=32)
     opt.step()
