@@ -239,7 +239,7 @@ class AdamW:
         try:
             _lib.launch("adamw_step", self.device, lib().dsmz_adamw_step, ctypes.byref(d), self._table,
                         len(self.params), None if ws is None else ws.data_ptr(), nbytes)
-        except _lib.DsmzError:
+        except BaseException:
             if grads is not None and self._grads is not None:
                 self._put_grads(self._grads)     # a refused step changes nothing
             raise
